@@ -1,0 +1,368 @@
+"""linear and gated_linear: refusals on the CPU, and on the MI355X against the formulas in 64 bits.
+
+Tolerance, element by element. With u = 2^-24 and S = sum |x w| (+ |bias|) of an output, a sum of K
+exact products in FP32, in any order and with chopped or rounded additions, is off by at most
+2 (K + 1) u S. The activation (steepest slope 1.13) passes that on and adds its own error: its
+exponential's argument is rounded, which moves the result by |z| u relative, z < 104 wherever the
+result is not zero, plus a few u: 128 u of its value. The row gate's sigmoid likewise, and the
+residual's addition u of the larger operand. Last the output's rounding: half a step of its type,
+finfo.eps / 2 of the value or half of the smallest subnormal.
+"""
+
+import ctypes
+
+import numpy as np
+import pytest
+import torch
+
+from gpu_helpers import announce
+from uniserve_moe import abi, ops
+
+U = 2.0**-24
+BF16, F16, F32 = torch.bfloat16, torch.float16, torch.float32
+
+
+def activated(y, activation):
+    if activation == "silu":
+        return y * torch.special.expit(y)
+    if activation == "gelu_tanh":
+        return 0.5 * y * (1.0 + torch.tanh((2.0 / torch.pi) ** 0.5 * (y + 0.044715 * y**3)))
+    return y
+
+
+def rounding(y, dtype):
+    info = torch.finfo(dtype)
+    return torch.maximum(y.abs() * (info.eps / 2), torch.full_like(y, info.tiny * info.eps / 2))
+
+
+def reference(x, w, bias=None, activation=None, gate=None, residual=None, out_dtype=None, gated=False):
+    """The output in 64 bits and how far the kernel may be from it, both on the CPU."""
+    out_dtype = out_dtype or x.dtype
+    x, w = x.double().cpu(), w.double().cpu()
+    y, s = x @ w.t(), x.abs() @ w.abs().t()
+    if bias is not None:
+        y, s = y + bias.double().cpu(), s + bias.double().cpu().abs()
+    off = 2 * (x.shape[1] + 1) * U * s
+    slope = 1.13
+    if gated:
+        n = w.shape[0] // 2
+        up, g = y[:, :n], y[:, n:]
+        act = activated(g, activation)
+        off = act.abs() * off[:, :n] + slope * off[:, n:] * (up.abs() + off[:, :n])
+        y = up * act
+        off = off + 128 * U * y.abs()
+    else:
+        y = activated(y, activation)
+        off = (off * slope if activation else off) + (128 * U * y.abs() if activation else 0.0)
+    if gate is not None:
+        factor = torch.special.expit(gate.double().cpu())
+        off, y = off * factor + 128 * U * (y * factor).abs(), y * factor
+    if residual is not None:
+        r = residual.double().cpu()
+        off, y = off + U * (y.abs() + r.abs()), y + r
+    return y, off + U * off + rounding(y.abs() + off, out_dtype)
+
+
+def assert_near(got, want, what=""):
+    y, tolerance = want
+    off = (got.double().cpu() - y).abs()
+    assert got.shape == y.shape and torch.isfinite(got).all(), what
+    worst = (off / tolerance).max().item() if off.numel() else 0.0
+    assert worst <= 1.0, f"{what}: {worst:.3f} of the tolerance"
+
+
+def normal(shape, seed, std=1.0, dtype=BF16, device="cuda"):
+    g = torch.Generator(device=device).manual_seed(seed)
+    return (torch.randn(shape, generator=g, device=device) * std).to(dtype)
+
+
+# ---- without a GPU ----------------------------------------------------------------------------------
+
+
+def filled_call(gated=False):
+    call = abi.LinearCall()
+    call.input, call.weight, call.out = 1 << 20, 2 << 20, 3 << 20
+    call.m, call.n, call.k = 4, 32, 64
+    call.input_row_stride, call.weight_row_stride, call.out_row_stride = 64, 64, 32
+    call.dtype = call.bias_dtype = call.out_dtype = abi.DTYPE["bf16"]
+    call.activation = abi.ACTIVATION["silu"] if gated else -1
+    return call
+
+
+REFUSED = [
+    ({"m": -1}, "positive"), ({"n": 0}, "positive"), ({"k": 0}, "positive"),
+    ({"input": None}, "needs"), ({"weight": None}, "needs"), ({"out": None}, "needs"),
+    ({"dtype": abi.DTYPE["f32"]}, "bf16 or f16"), ({"out_dtype": abi.DTYPE["f16"]}, "inputs' type"),
+    ({"bias": 8 << 20, "bias_dtype": abi.DTYPE["f16"]}, "bias"), ({"activation": 2}, "gelu_tanh"),
+    ({"input_row_stride": 63}, "strides"), ({"weight_row_stride": 63}, "strides"), ({"out_row_stride": 31}, "strides"),
+    ({"k": 1 << 31, "input_row_stride": 1 << 31, "weight_row_stride": 1 << 31}, "int32"),
+    ({"input_row_stride": 1 << 60}, "too large"), ({"weight_row_stride": 1 << 60}, "too large"),
+    # Outputs over an input: whole, in part, from below, and rows that meet within a shared buffer.
+    ({"out": 1 << 20}, "overlaps"), ({"out": (1 << 20) + 130}, "overlaps"), ({"out": (1 << 20) - 254}, "overlaps"),
+    ({"out": 2 << 20}, "overlaps"), ({"out": (2 << 20) + 4094}, "overlaps"),
+    ({"bias": (3 << 20) + 2}, "overlaps"),
+    ({"out": (1 << 20) + 126, "out_row_stride": 96, "input_row_stride": 96}, "overlaps"),
+    ({"out": (1 << 20) + 130, "out_row_stride": 96, "input_row_stride": 96}, "overlaps"),
+]
+
+
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("fields, says", REFUSED)
+def test_refusals(gated, fields, says):
+    call = filled_call(gated)
+    for name, value in fields.items():
+        setattr(call, name, value)
+    entry = abi.library().uniserve_gated_linear if gated else abi.library().uniserve_linear
+    assert entry(ctypes.byref(call), None) != 0
+    assert says in call.error.decode()
+
+
+@pytest.mark.parametrize("fields, says", [
+    ({"gate": 8 << 20, "gate_stride": -1}, "gate stride"),
+    ({"gate": (3 << 20) + 2, "gate_stride": 1}, "overlaps"),
+    ({"residual": 8 << 20, "residual_row_stride": 31}, "strides"),
+    ({"residual": (3 << 20) + 2, "residual_row_stride": 32}, "residual"),
+    ({"residual": 3 << 20, "residual_row_stride": 40}, "residual"),
+])
+def test_linear_refusals(fields, says):
+    call = filled_call()
+    for name, value in fields.items():
+        setattr(call, name, value)
+    assert abi.library().uniserve_linear(ctypes.byref(call), None) != 0
+    assert says in call.error.decode()
+
+
+@pytest.mark.parametrize("fields, says", [
+    ({"activation": -1}, "silu or gelu_tanh"), ({"out_dtype": abi.DTYPE["f32"]}, "inputs' type"),
+    ({"gate": 8 << 20}, "no row gate"), ({"residual": 8 << 20}, "no residual"),
+])
+def test_gated_linear_refusals(fields, says):
+    call = filled_call(gated=True)
+    for name, value in fields.items():
+        setattr(call, name, value)
+    assert abi.library().uniserve_gated_linear(ctypes.byref(call), None) != 0
+    assert says in call.error.decode()
+
+
+def test_no_rows_launch_nothing():
+    call = filled_call()
+    call.m, call.input, call.out = 0, None, None
+    assert abi.library().uniserve_linear(ctypes.byref(call), None) == 0
+    assert abi.library().uniserve_linear(None, None) != 0
+
+
+def test_python_refusals():
+    with pytest.raises(ValueError, match="on a GPU"):
+        ops.linear(torch.zeros(2, 8, dtype=BF16), torch.zeros(4, 8, dtype=BF16))
+    with pytest.raises(ValueError, match="up rows"):
+        ops.gated_linear(torch.zeros(2, 8, dtype=BF16), torch.zeros(5, 8, dtype=BF16))
+
+
+# ---- on the MI355X ----------------------------------------------------------------------------------
+
+#: m, n, k: one row to several tiles, odd extents, single columns and elements, whole tiles.
+SHAPES = [(1, 1, 1), (1, 2048, 1408), (1, 5, 4096), (2, 16, 8), (3, 1000, 72), (5, 33, 1000), (7, 64, 8192), (16, 256, 128),
+          (17, 130, 264), (31, 96, 96), (33, 512, 520), (48, 2048, 64), (64, 128, 2048), (65, 65, 65), (100, 1, 2048),
+          (129, 257, 384), (200, 704, 1024), (256, 256, 256), (257, 384, 1984), (300, 1001, 1000), (512, 1408, 192),
+          (1000, 300, 128), (1025, 640, 640), (2048, 264, 2048)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m, n, k", SHAPES)
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_linear_plain(device, m, n, k, dtype):
+    announce("linear", m, n, k, dtype)
+    x, w = normal((m, k), m + k, dtype=dtype), normal((n, k), n + k + 1, 0.05, dtype)
+    assert_near(ops.linear(x, w), reference(x, w))
+    assert_near(ops.linear(x, w, out_dtype=F32), reference(x, w, out_dtype=F32), "f32")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m, n, k", SHAPES)
+@pytest.mark.parametrize("dtype, activation", [(BF16, "silu"), (F16, "gelu_tanh")])
+def test_linear_with_everything(device, m, n, k, dtype, activation):
+    announce("linear epilogue", m, n, k, dtype)
+    x, w = normal((m, k), m + k, dtype=dtype), normal((n, k), n + k + 1, 0.05, dtype)
+    gate, residual = normal((m, 1), 3, 2.0, dtype), normal((m, n), 4, 1.0, dtype)
+    bias = normal((n,), 5, 0.5, F32 if n % 2 else dtype)
+    got = ops.linear(x, w, bias=bias, activation=activation, gate=gate, residual=residual)
+    assert_near(got, reference(x, w, bias, activation, gate, residual))
+    wide = residual.float()
+    out = ops.linear(x, w, bias=bias, activation=activation, gate=gate, residual=wide, out=wide)  # in place, f32
+    assert out is wide
+    assert_near(out, reference(x, w, bias, activation, gate, residual.float(), out_dtype=F32), "f32 in place")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m, n, k", SHAPES)
+@pytest.mark.parametrize("dtype, activation", [(BF16, "gelu_tanh"), (F16, "silu")])
+def test_gated_linear(device, m, n, k, dtype, activation):
+    announce("gated_linear", m, n, k, dtype)
+    x, w = normal((m, k), m + k, dtype=dtype), normal((2 * n, k), n + k + 1, 0.05, dtype)
+    assert_near(ops.gated_linear(x, w, activation=activation), reference(x, w, None, activation, gated=True))
+    bias = normal((2 * n,), 5, 0.5, dtype if n % 2 else F32)
+    assert_near(ops.gated_linear(x, w, bias=bias, activation=activation), reference(x, w, bias, activation, gated=True), "bias")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m, n, k", [(1, 40, 128), (4, 72, 320), (40, 136, 256), (130, 200, 192), (700, 264, 512)])
+@pytest.mark.parametrize("shift", [0, 1, 8])
+def test_strides_and_alignments(device, m, n, k, shift):
+    """Column slices of wider buffers, shifted by whole 16 bytes or by one element; what lies beside
+    the output stays as it was."""
+    announce("linear strides", m, n, k, shift)
+    wide_x, wide_w = normal((m, k + 24), 1), normal((2 * n, k + 40), 2, 0.05)
+    x, w = wide_x[:, shift:shift + k], wide_w[:, shift:shift + k]
+    wide_out = normal((m, n + 16), 3)
+    before = wide_out.clone()
+    out = wide_out[:, shift:shift + n]
+    residual = normal((m, n + 9), 4)[:, :n]
+    gate = normal((m, 7), 5)[:, 3:4]
+    assert ops.linear(x, w[:n], gate=gate, residual=residual, out=out).data_ptr() == out.data_ptr()
+    assert_near(out, reference(x, w[:n], gate=gate, residual=residual))
+    assert torch.equal(wide_out[:, :shift], before[:, :shift]) and torch.equal(wide_out[:, shift + n:], before[:, shift + n:])
+    wide_out.copy_(before)
+    ops.linear(x, w[:n], residual=out, out=out)  # in place
+    assert_near(out, reference(x, w[:n], residual=before[:, shift:shift + n]), "in place")
+    wide_out.copy_(before)
+    ops.gated_linear(x, w, out=out)
+    assert_near(out, reference(x, w, None, "silu", gated=True), "gated")
+    assert torch.equal(wide_out[:, :shift], before[:, :shift]) and torch.equal(wide_out[:, shift + n:], before[:, shift + n:])
+
+
+@pytest.mark.gpu
+def test_output_beside_its_input_in_one_buffer(device):
+    """Interleaved rows share no byte and are served; a shared gate (stride 0) too."""
+    announce("linear interleaved")
+    buffer = normal((50, 96 + 64), 6)
+    x, out = buffer[:, :96], buffer[:, 96:]
+    w, kept = normal((64, 96), 7, 0.05), buffer[:, :96].clone()
+    gate = normal((1, 1), 8).expand(50, 1)
+    ops.linear(x, w, gate=gate, out=out)
+    assert_near(out, reference(kept, w, gate=gate))
+    assert torch.equal(buffer[:, :96], kept)
+    with pytest.raises(RuntimeError, match="overlaps"):
+        ops.linear(x, w, out=buffer[:, 95:159])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m", [3, 40, 200])
+def test_arrays_past_4_gib(device, m):
+    """Rows of the input, the weight, the residual and the output lie beyond 32-bit byte offsets."""
+    announce("linear far rows", m)
+    k, n = 256, 136
+    stride = (5 << 30) // 2 // m // 8 * 8 + 8  # the last row starts past 4 GiB
+
+    def spread(rows, columns, source):
+        far = torch.empty(rows * stride, dtype=BF16, device=device).as_strided((rows, columns), (stride, 1))
+        return far.copy_(source)
+
+    x, w = normal((m, k), 1), normal((n, k), 2, 0.05)
+    w_far = spread(m, k, w[:m] if m <= n else torch.cat([w, w])[:m])
+    x_far, residual = spread(m, k, x), spread(m, n, normal((m, n), 3))
+    got = ops.linear(x_far, w, residual=residual, out=residual.clone() if m < 3 else residual)
+    assert_near(got, reference(x, w, residual=normal((m, n), 3)), "far input and output")
+    assert_near(ops.linear(x, w_far), reference(x, w_far), "far weight")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m, n, k", [(1, 64, 128), (64, 256, 512), (300, 320, 256)])
+def test_infinities_and_nans_stay_in_their_rows(device, m, n, k):
+    """A row's NaN or infinity reaches that row's outputs and no other's; a weight row's its column."""
+    announce("linear non-finite", m, n, k)
+    x, w = normal((m, k), 1), normal((n, k), 2, 0.05)
+    want, tolerance = reference(x, w)
+    x[m // 2, k - 1] = float("nan")
+    w[n - 1, 0] = float("inf")
+    got = ops.linear(x, w).double().cpu()
+    rows = [r for r in range(m) if r != m // 2]
+    assert torch.isnan(got[m // 2]).all()
+    if rows:
+        assert not torch.isfinite(got[rows][:, n - 1]).any()
+        assert ((got[rows][:, :n - 1] - want[rows][:, :n - 1]).abs() <= tolerance[rows][:, :n - 1]).all()
+
+
+@pytest.mark.gpu
+def test_f16_overflow_and_large_activations(device):
+    announce("linear overflow")
+    x = torch.full((9, 64), 200.0, dtype=F16, device=device)
+    w = torch.full((16, 64), 10.0, dtype=F16, device=device)
+    w[8:] = -10.0
+    got = ops.linear(x, w)
+    assert (got[:, :8] == float("inf")).all() and (got[:, 8:] == -float("inf")).all()
+    for activation in ("silu", "gelu_tanh"):
+        act = ops.linear(x, w, activation=activation, out_dtype=F32)
+        assert (act[:, :8] == 128000.0).all() and (act[:, 8:] == 0.0).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m, n, k", [(1, 512, 1024), (60, 256, 1024), (640, 512, 512)])
+def test_results_repeat_and_rows_do_not_depend_on_the_batch_s_other_rows(device, m, n, k):
+    announce("linear repeats", m, n, k)
+    x, w = normal((m, k), 1), normal((n, k), 2, 0.05)
+    first = ops.linear(x, w)
+    for _ in range(3):
+        assert torch.equal(ops.linear(x, w), first)
+    x[0] = 0
+    assert torch.equal(ops.linear(x, w)[1:], first[1:])
+
+
+@pytest.mark.gpu
+def test_captured_replays_and_other_streams(device):
+    announce("linear graph")
+    x, up_gate, down = normal((48, 256), 1), normal((384, 256), 2, 0.05), normal((256, 192), 3, 0.05)
+    gate, residual = normal((48, 1), 4), normal((48, 256), 5)
+    one, one_out = x[:1].clone(), torch.empty((1, 256), dtype=BF16, device=device)
+
+    def step():
+        ops.linear(ops.gated_linear(one, up_gate), down, out=one_out)
+        return ops.linear(ops.gated_linear(x, up_gate), down, gate=gate, residual=residual)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(side):
+        step()
+        side.synchronize()
+        with torch.cuda.graph(graph, stream=side):
+            got = step()
+    torch.cuda.current_stream().wait_stream(side)
+    for seed in (10, 11, 12):
+        x.copy_(normal((48, 256), seed))
+        one.copy_(x[:1])
+        graph.replay()
+        torch.cuda.synchronize()
+        replayed, replayed_one = got.clone(), one_out.clone()
+        assert torch.equal(step(), replayed) and torch.equal(one_out, replayed_one)
+        torch.cuda.synchronize()
+
+
+@pytest.mark.gpu
+def test_no_rows(device):
+    w = normal((32, 64), 1)
+    assert ops.linear(torch.empty((0, 64), dtype=BF16, device=device), w).shape == (0, 32)
+    assert ops.gated_linear(torch.empty((0, 64), dtype=BF16, device=device), w).shape == (0, 16)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("arguments, says", [
+    (dict(weight=torch.zeros(8, 16, dtype=F16)), "input's type"), (dict(weight=torch.zeros(8, 16, dtype=BF16)), "device"),
+    (dict(weight="narrow"), "weight"), (dict(activation="relu"), "activation"), (dict(bias="short"), "bias"),
+    (dict(bias="half"), "bias"), (dict(gate="flat"), "gate"), (dict(gate="host"), "gate"), (dict(residual="short"), "residual"),
+    (dict(residual="wide"), "residual"), (dict(out="wide", out_dtype=BF16), "output"), (dict(out="short"), "output"),
+    (dict(out="columns"), "output"), (dict(out_dtype=torch.int32), "output"),
+])
+def test_python_refusals_of_device_calls(device, arguments, says):
+    made = {
+        "weight.narrow": lambda: normal((8, 15), 1), "bias.short": lambda: normal((7,), 1),
+        "bias.half": lambda: normal((8,), 1, dtype=F16), "gate.flat": lambda: normal((4,), 1),
+        "gate.host": lambda: torch.zeros((4, 1), dtype=BF16), "residual.short": lambda: normal((3, 8), 1),
+        "residual.wide": lambda: normal((4, 8), 1, dtype=F32), "out.wide": lambda: normal((4, 8), 1, dtype=F32),
+        "out.short": lambda: normal((4, 7), 1), "out.columns": lambda: normal((8, 4), 1).t(),
+    }
+    arguments = {k: made[f"{k}.{v}"]() if f"{k}.{v}" in made else v for k, v in arguments.items()}
+    weight = arguments.pop("weight", None)
+    if weight is not None and weight.dtype == F16:
+        weight = weight.to(device)
+    with pytest.raises((ValueError, RuntimeError), match=says):
+        ops.linear(normal((4, 16), 1), normal((8, 16), 2) if weight is None else weight, **arguments)

@@ -9,11 +9,13 @@ loudly when the shared object has not been built.
 
 from .abi import (  # noqa: F401
     DTYPE,
+    ExpertTopkCall,
     GatherCall,
     GatherFp8Call,
     GemmCall,
     LayerCall,
     LayerViews,
+    LinearCall,
     QuantizeFp8Call,
     MxStageScalesCall,
     QuantizeMxfp8Call,

@@ -13,6 +13,10 @@ from pathlib import Path
 # FC1's gate (uniserve_activation); the FC1 entries take it by name, the layer call as a field.
 ACTIVATION = {"silu": 0, "gelu_tanh": 1}
 ENTRY_SUFFIX = {"silu": "", "gelu_tanh": "_gelu_tanh"}
+# The dense products also go without (UNISERVE_ACTIVATION_NONE).
+LINEAR_ACTIVATION = {None: -1, **ACTIVATION}
+# expert_topk's scores (uniserve_scoring).
+SCORING = {"softmax": 0, "sigmoid": 1}
 
 DTYPE = {
     "u8": 0,
@@ -355,6 +359,58 @@ class LayerViews(ctypes.Structure):
     ]
 
 
+class ExpertTopkCall(ctypes.Structure):
+    """``uniserve_expert_topk_call``."""
+
+    _fields_ = [
+        ("scores", _P),
+        ("bias", _P),
+        ("map", _P),
+        ("live", _P),
+        ("load", _P),
+        ("ids", _P),
+        ("weights", _P),
+        ("row_stride", _I64),
+        ("rows", _I64),
+        ("experts", _I64),
+        ("top", _I64),
+        ("groups", _I64),
+        ("top_groups", _I64),
+        ("group_top", _I64),
+        ("score_dtype", _I64),
+        ("scoring", _I64),
+        ("renormalize", _I64),
+        ("factor", ctypes.c_float),
+        ("error", _ERR),
+    ]
+
+
+class LinearCall(ctypes.Structure):
+    """``uniserve_linear_call``."""
+
+    _fields_ = [
+        ("input", _P),
+        ("weight", _P),
+        ("bias", _P),
+        ("gate", _P),
+        ("residual", _P),
+        ("out", _P),
+        ("m", _I64),
+        ("n", _I64),
+        ("k", _I64),
+        ("input_row_stride", _I64),
+        ("weight_row_stride", _I64),
+        ("gate_stride", _I64),
+        ("residual_row_stride", _I64),
+        ("out_row_stride", _I64),
+        ("dtype", _I64),
+        ("bias_dtype", _I64),
+        ("out_dtype", _I64),
+        ("activation", _I64),
+        ("error", _ERR),
+    ]
+
+
 def max_tiles(tokens, top, local_experts, tile=128):
     """``ops::moe::max_tiles`` (crates/ops/src/moe/mod.rs:63-70)."""
     expanded = tokens * top
@@ -401,6 +457,9 @@ _ENTRIES = {
     "uniserve_gather_gemm_mx_gelu_tanh": GatherMxCall,
     "uniserve_route_gemm_mx": RouteMxCall,
     "uniserve_mx_stage_major_scales": MxStageScalesCall,
+    "uniserve_expert_topk": ExpertTopkCall,
+    "uniserve_linear": LinearCall,
+    "uniserve_gated_linear": LinearCall,
 }
 
 

@@ -16,11 +16,15 @@ from .abi import (
     DTYPE,
     ENTRY_SUFFIX,
     LAYOUT_PERMUTED,
+    LINEAR_ACTIVATION,
+    SCORING,
+    ExpertTopkCall,
     GatherCall,
     GatherFp8Call,
     GemmCall,
     LayerCall,
     LayerViews,
+    LinearCall,
     QuantizeFp8Call,
     MxStageScalesCall,
     QuantizeMxfp8Call,
@@ -79,6 +83,127 @@ def topk_softmax(scores, top, renormalize=True, scale=None, mapping=None, live=N
     return ids, weights
 
 
+def _enter(entry, call, device, name):
+    """Calls ``entry`` on the device's current stream, with that device current."""
+    if device.index == torch.cuda.current_device():
+        _check(entry(ctypes.byref(call), _stream(device)), call, name)
+        return
+    with torch.cuda.device(device):
+        _check(entry(ctypes.byref(call), _stream(device)), call, name)
+
+
+def _matrix(tensor, rows, columns, what):
+    """Refuses a tensor that is no [rows, columns] matrix of contiguous rows."""
+    if tensor.shape != (rows, columns) or (columns > 1 and tensor.stride(1) != 1):
+        raise ValueError(f"{what} is [{rows}, {columns}], its rows contiguous: got {tuple(tensor.shape)}, "
+                         f"strides {tensor.stride()}")
+
+
+def _vector(tensor, count, dtypes, device, what):
+    if tensor.shape != (count,) or tensor.dtype not in dtypes or tensor.device != device or not tensor.is_contiguous():
+        raise ValueError(f"{what} is [{count}] of {' or '.join(str(d) for d in dtypes)} on {device}, contiguous")
+
+
+def expert_topk(scores, top, scoring="sigmoid", bias=None, groups=1, top_groups=1, group_top=2, renormalize=True,
+                factor=1.0, mapping=None, live=None, load=None):
+    """The expert choice of routers with sigmoid scores, a balance bias or expert groups: ids
+    ``[T, top]`` int32 and weights f32 from the logits ``scores`` ``[T, E]`` (f32, bf16 or f16).
+
+    An expert's score is the sigmoid of its logit or its share of the row's softmax; ``bias`` (f32
+    ``[E]``) is added to the scores for the choice alone. With ``groups`` > 1 only the experts of the
+    ``top_groups`` best groups (E / groups consecutive experts each, ranked by the sum of their best
+    ``group_top`` choices, 1 or 2) are chosen from. Equal choices go to the lower id. The weights are
+    the chosen experts' scores, divided by their sum where ``renormalize``, times ``factor``.
+
+    A logit (or a bias) of -inf or NaN takes its expert out; where too few are left, ids are -1 with
+    weight 0, which ``moe_sort`` skips. ``mapping``, ``live`` and ``load`` are ``topk_softmax``'s."""
+    if scores.dim() != 2 or scores.dtype not in _ELEMENT or not scores.is_cuda:
+        raise ValueError("expert_topk: the scores are [tokens, experts] of f32, bf16 or f16 on a GPU")
+    if scoring not in SCORING:
+        raise ValueError(f"expert_topk: scoring is one of {sorted(SCORING)}, got {scoring!r}")
+    tokens, experts = scores.shape
+    device = scores.device
+    _matrix(scores, tokens, experts, "expert_topk: scores")
+    if bias is not None:
+        _vector(bias, experts, (torch.float32,), device, "expert_topk: bias")
+    if mapping is not None:
+        _vector(mapping, experts, (torch.int32,), device, "expert_topk: mapping")
+    if load is not None:
+        _vector(load, experts, (torch.int64,), device, "expert_topk: load")
+    if live is not None and (live.numel() != 1 or live.dtype not in (torch.int32, torch.uint32) or live.device != device):
+        raise ValueError("expert_topk: live is one int32 on the scores' device")
+    ids = torch.empty((tokens, max(top, 0)), dtype=torch.int32, device=device)
+    weights = torch.empty((tokens, max(top, 0)), dtype=torch.float32, device=device)
+    call = ExpertTopkCall(scores.data_ptr(), _ptr(bias), _ptr(mapping), _ptr(live), _ptr(load), ids.data_ptr(),
+                          weights.data_ptr(), scores.stride(0), tokens, experts, top, groups, top_groups, group_top,
+                          _ELEMENT[scores.dtype], SCORING[scoring], 1 if renormalize else 0, factor)
+    _enter(library().uniserve_expert_topk, call, device, "expert_topk")
+    return ids, weights
+
+
+def _product(entry, name, x, weight, columns, bias, activation, gate, residual, out, out_dtype):
+    if x.dim() != 2 or x.dtype not in _PRODUCT or not x.is_cuda:
+        raise ValueError(f"{name}: the input is [tokens, width] of bf16 or f16 on a GPU")
+    if weight.dtype != x.dtype or weight.device != x.device:
+        raise ValueError(f"{name}: the weight is the input's type, on its device")
+    if activation not in LINEAR_ACTIVATION:
+        raise ValueError(f"{name}: activation is one of silu, gelu_tanh or none, got {activation!r}")
+    tokens, width = x.shape
+    device = x.device
+    _matrix(x, tokens, width, f"{name}: the input")
+    _matrix(weight, weight.shape[0], width, f"{name}: the weight")
+    if out_dtype is None:
+        out_dtype = x.dtype if out is None else out.dtype
+    if out is None:
+        out = torch.empty((tokens, columns), dtype=out_dtype, device=device)
+    elif out.dtype != out_dtype or out.device != device:
+        raise ValueError(f"{name}: the output is {out_dtype} on {device}")
+    else:
+        _matrix(out, tokens, columns, f"{name}: the output")
+    if out_dtype not in _ELEMENT:
+        raise ValueError(f"{name}: the output is the input's type or f32")
+    if bias is not None:
+        _vector(bias, weight.shape[0], (x.dtype, torch.float32), device, f"{name}: the bias")
+    if gate is not None:
+        if gate.shape != (tokens, 1) or gate.dtype != x.dtype or gate.device != device:
+            raise ValueError(f"{name}: the gate is one logit per row, [tokens, 1] of the input's type on its device")
+    if residual is not None:
+        if residual.dtype != out_dtype or residual.device != device:
+            raise ValueError(f"{name}: the residual is of the output's type, on its device")
+        _matrix(residual, tokens, columns, f"{name}: the residual")
+    element = _ELEMENT[x.dtype]
+    call = LinearCall(x.data_ptr(), weight.data_ptr(), _ptr(bias), _ptr(gate), _ptr(residual), out.data_ptr(), tokens,
+                      columns, width, x.stride(0), weight.stride(0), 0 if gate is None else gate.stride(0),
+                      0 if residual is None else residual.stride(0), out.stride(0), element,
+                      element if bias is None else _ELEMENT[bias.dtype], _ELEMENT[out_dtype],
+                      LINEAR_ACTIVATION[activation])
+    _enter(entry, call, device, name)
+    return out
+
+
+def linear(x, weight, bias=None, activation=None, gate=None, residual=None, out=None, out_dtype=None):
+    """``act(x @ weight.T + bias) * sigmoid(gate) + residual`` ``[T, N]``: ``x`` ``[T, K]`` and ``weight``
+    ``[N, K]`` bf16 or f16, FP32 sums, one rounding into ``x``'s type (or f32, ``out_dtype``: a router's
+    logits). ``bias`` is ``[N]`` of ``x``'s type or f32, ``activation`` None, "silu" or "gelu_tanh",
+    ``gate`` one logit per row (``[T, 1]``, a shared expert's), ``residual`` ``[T, N]`` of the output's
+    type; ``out`` may be the residual itself, in place."""
+    if weight.dim() != 2:
+        raise ValueError("linear: the weight is [rows, width]")
+    return _product(library().uniserve_linear, "linear", x, weight, weight.shape[0], bias, activation, gate, residual,
+                    out, out_dtype)
+
+
+def gated_linear(x, up_gate, bias=None, activation="silu", out=None):
+    """``(x @ up.T + up_bias) * act(x @ gate.T + gate_bias)`` ``[T, I]``: an MLP's first product, with
+    ``up_gate`` ``[2 I, K]`` the up rows and then the gate rows (an expert's FC1 order), ``bias``
+    ``[2 I]`` likewise and ``activation`` "silu" or "gelu_tanh"."""
+    if up_gate.dim() != 2 or up_gate.shape[0] % 2 != 0:
+        raise ValueError("gated_linear: the weight is [2 I, width], the up rows and then the gate rows")
+    return _product(library().uniserve_gated_linear, "gated_linear", x, up_gate, up_gate.shape[0] // 2, bias,
+                    activation, None, None, out, None)
+
+
+_PRODUCT = (torch.bfloat16, torch.float16)
 _ELEMENT = {torch.bfloat16: DTYPE["bf16"], torch.float16: DTYPE["f16"], torch.float32: DTYPE["f32"]}
 
 
