@@ -22,11 +22,13 @@ struct LinearParams {
   int32_t bias_f32;
   int32_t out_f32;
   int32_t activation;
-  int32_t rows_of_16;    ///< input and weight rows start at 16-byte aligned addresses and k is whole 8
-  int32_t out_of_4;      ///< out (and residual) rows take four columns at an aligned address
+  int32_t by_dma;        ///< input and weight rows suit the tile kernels' loads
+  int32_t out_of_8;      ///< out (and residual) rows start at 16-byte aligned addresses
 };
 
 struct Bf16 {
+  static __device__ __forceinline__ float low(uint32_t pair) { return __uint_as_float(pair << 16); }
+  static __device__ __forceinline__ float high(uint32_t pair) { return __uint_as_float(pair & 0xffff0000u); }
   static __device__ __forceinline__ float to_f32(uint16_t bits) { return bf16_to_f32(bits); }
   static __device__ __forceinline__ uint16_t from_f32(float v) { return f32_to_bf16(v); }
   static __device__ __forceinline__ uint32_t pack2(float lo, float hi) { return pack_bf16x2(lo, hi); }
@@ -35,6 +37,8 @@ struct Bf16 {
 
 struct F16 {
   typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+  static __device__ __forceinline__ float low(uint32_t pair) { return to_f32(static_cast<uint16_t>(pair)); }
+  static __device__ __forceinline__ float high(uint32_t pair) { return to_f32(static_cast<uint16_t>(pair >> 16)); }
   static __device__ __forceinline__ float to_f32(uint16_t bits) { return static_cast<float>(__builtin_bit_cast(_Float16, bits)); }
   static __device__ __forceinline__ uint16_t from_f32(float v) { return __builtin_bit_cast(uint16_t, static_cast<_Float16>(v)); }
   static __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
@@ -51,74 +55,151 @@ __device__ __forceinline__ float bias_at(const LinearParams &p, int64_t n) {
   return p.bias_f32 ? static_cast<const float *>(p.bias)[n] : T::to_f32(static_cast<const uint16_t *>(p.bias)[n]);
 }
 
-/// The row's factor: sigmoid of its gate logit, or 1.
+template <class T>
+__device__ __forceinline__ float residual_at(const LinearParams &p, int64_t m, int64_t n) {
+  const int64_t at = m * p.residual_stride + n;
+  return p.out_f32 ? static_cast<const float *>(p.residual)[at] : T::to_f32(static_cast<const uint16_t *>(p.residual)[at]);
+}
+
+/// Elements at .. at + 7 of a row of `width`, zeros past its end; one 16-byte load at any alignment where
+/// all eight lie in the row.
+__device__ __forceinline__ u32x4 load8(const uint16_t *row, int64_t at, int64_t width) {
+  u32x4 v;
+  if (at + 8 <= width) {
+    __builtin_memcpy(&v, row + at, 16);
+    return v;
+  }
+  uint32_t e[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) e[i] = at + i < width ? row[at + i] : 0u;
+  return u32x4{e[0] | (e[1] << 16), e[2] | (e[3] << 16), e[4] | (e[5] << 16), e[6] | (e[7] << 16)};
+}
+
+/// The row's factor: sigmoid of its gate logit.
 template <class T>
 __device__ __forceinline__ float row_gate(const LinearParams &p, int64_t m) {
-  if (p.gate == nullptr) return 1.0f;
   const float g = T::to_f32(p.gate[m * p.gate_stride]);
   return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-g * 1.4426950408889634f));
 }
 
-/// Columns n .. n + 3 (those below p.n) of row m from their four sums (gated: the up halves' and the
-/// gate halves'): bias, activation, row gate, residual, one rounding.
+/// The epilogue of eight consecutive columns n .. n + 7 (those below p.n) of some rows: the columns'
+/// biases, loaded once, and what turns a row's sums into its outputs - bias, activation, row gate,
+/// residual, one rounding.
 template <class T, bool kGated>
-__device__ __forceinline__ void finish4(const LinearParams &p, int64_t m, int64_t n, const floatx4 &sums,
-                                        const floatx4 &gate_sums, float factor) {
-  const int count = p.n - n < 4 ? static_cast<int>(p.n - n) : 4;
-  if (count <= 0) return;
-  float v[4];
+struct Columns8 {
+  float bias[kGated ? 16 : 8];
+  int count;
+  bool vectors;  ///< all eight columns, at 16-byte aligned addresses
+
+  __device__ __forceinline__ Columns8(const LinearParams &p, int64_t n) {
+    count = p.n - n < 8 ? (p.n > n ? static_cast<int>(p.n - n) : 0) : 8;
+    vectors = p.out_of_8 && count == 8;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    v[i] = sums[i];
-    if (p.bias != nullptr && i < count) v[i] += bias_at<T>(p, n + i);
+    for (int i = 0; i < 8; ++i) {
+      bias[i] = p.bias != nullptr && i < count ? bias_at<T>(p, n + i) : 0.0f;
+      if constexpr (kGated) bias[8 + i] = p.bias != nullptr && i < count ? bias_at<T>(p, p.n + n + i) : 0.0f;
+    }
   }
+
+  /// What kRows rows m[i] read besides their sums: the loads go out together, so their latencies do not add up.
+  template <int kRows>
+  struct Extras {
+    u32x4 residual[kRows][2];
+    float factor[kRows];
+  };
+  template <int kRows>
+  __device__ __forceinline__ void load(const LinearParams &p, const int64_t (&m)[kRows], int64_t n, Extras<kRows> &e) const {
+    if constexpr (kGated) return;
+    if (p.residual != nullptr && vectors) {
+      if (p.out_f32) {
+#pragma unroll
+        for (int i = 0; i < kRows; ++i) {
+          const u32x4 *from = reinterpret_cast<const u32x4 *>(static_cast<const float *>(p.residual) + m[i] * p.residual_stride + n);
+          e.residual[i][0] = from[0];
+          e.residual[i][1] = from[1];
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < kRows; ++i)
+          e.residual[i][0] = *reinterpret_cast<const u32x4 *>(static_cast<const uint16_t *>(p.residual) + m[i] * p.residual_stride + n);
+      }
+    }
+    if (p.gate != nullptr) {
+#pragma unroll
+      for (int i = 0; i < kRows; ++i) e.factor[i] = row_gate<T>(p, m[i]);
+    }
+  }
+
+  /// Row m's outputs from its sums (gated: the up halves' and the gate halves').
+  __device__ __forceinline__ void finish(const LinearParams &p, int64_t m, int64_t n, const floatx4 (&sums)[2],
+                                         const floatx4 (&gates)[2], const u32x4 (&residual)[2], float factor) const {
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = sums[i / 4][i % 4] + bias[i];
+    if constexpr (kGated) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] *= gate(gates[i / 4][i % 4] + bias[8 + i], p.activation);
+    } else {
+      if (p.activation != UNISERVE_ACTIVATION_NONE) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = gate(v[i], p.activation);
+      }
+      if (p.gate != nullptr) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] *= factor;
+      }
+      if (p.residual != nullptr) {
+        if (!vectors) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (i < count) v[i] += residual_at<T>(p, m, n + i);
+        } else if (p.out_f32) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) v[i] += __uint_as_float(residual[i / 4][i % 4]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) v[2 * i] += T::low(residual[0][i]), v[2 * i + 1] += T::high(residual[0][i]);
+        }
+      }
+    }
+    if (p.out_f32) {
+      float *out = static_cast<float *>(p.out) + m * p.out_stride + n;
+      if (vectors) {
+        *reinterpret_cast<floatx4 *>(out) = floatx4{v[0], v[1], v[2], v[3]};
+        *reinterpret_cast<floatx4 *>(out + 4) = floatx4{v[4], v[5], v[6], v[7]};
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (i < count) out[i] = v[i];
+      }
+    } else {
+      uint16_t *out = static_cast<uint16_t *>(p.out) + m * p.out_stride + n;
+      if (vectors) {
+        *reinterpret_cast<u32x4 *>(out) =
+            u32x4{T::pack2(v[0], v[1]), T::pack2(v[2], v[3]), T::pack2(v[4], v[5]), T::pack2(v[6], v[7])};
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (i < count) out[i] = T::from_f32(v[i]);
+      }
+    }
+  }
+};
+
+/// One output from its sum (gated: and its gate's), as Columns8 does eight.
+template <class T, bool kGated>
+__device__ __forceinline__ void finish1(const LinearParams &p, int64_t m, int64_t n, float v, float gate_sum) {
+  if (p.bias != nullptr) v += bias_at<T>(p, n);
   if constexpr (kGated) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      float g = gate_sums[i];
-      if (p.bias != nullptr && i < count) g += bias_at<T>(p, p.n + n + i);
-      v[i] *= gate(g, p.activation);
-    }
-  } else if (p.activation != UNISERVE_ACTIVATION_NONE) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = gate(v[i], p.activation);
+    v *= gate(p.bias != nullptr ? gate_sum + bias_at<T>(p, p.n + n) : gate_sum, p.activation);
+  } else {
+    if (p.activation != UNISERVE_ACTIVATION_NONE) v = gate(v, p.activation);
+    if (p.gate != nullptr) v *= row_gate<T>(p, m);
   }
+  if (p.residual != nullptr) v += residual_at<T>(p, m, n);
   const int64_t at = m * p.out_stride + n;
-  const int64_t from = m * p.residual_stride + n;
-  if (!kGated) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] *= factor;
-  }
-  if (p.out_f32) {
-    float *out = static_cast<float *>(p.out) + at;
-    const float *residual = static_cast<const float *>(p.residual) + from;
-    if (p.out_of_4 && count == 4) {
-      floatx4 r = {0.0f, 0.0f, 0.0f, 0.0f};
-      if (p.residual != nullptr) r = *reinterpret_cast<const floatx4 *>(residual);
-      *reinterpret_cast<floatx4 *>(out) = floatx4{v[0] + r[0], v[1] + r[1], v[2] + r[2], v[3] + r[3]};
-      return;
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (i < count) out[i] = p.residual != nullptr ? v[i] + residual[i] : v[i];
-    return;
-  }
-  uint16_t *out = static_cast<uint16_t *>(p.out) + at;
-  const uint16_t *residual = static_cast<const uint16_t *>(p.residual) + from;
-  if (p.out_of_4 && count == 4) {
-    if (p.residual != nullptr) {
-      const uint2 r = *reinterpret_cast<const uint2 *>(residual);
-      v[0] += T::to_f32(static_cast<uint16_t>(r.x));
-      v[1] += T::to_f32(static_cast<uint16_t>(r.x >> 16));
-      v[2] += T::to_f32(static_cast<uint16_t>(r.y));
-      v[3] += T::to_f32(static_cast<uint16_t>(r.y >> 16));
-    }
-    *reinterpret_cast<uint2 *>(out) = uint2{T::pack2(v[0], v[1]), T::pack2(v[2], v[3])};
-    return;
-  }
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    if (i < count) out[i] = T::from_f32(p.residual != nullptr ? v[i] + T::to_f32(residual[i]) : v[i]);
+  if (p.out_f32) static_cast<float *>(p.out)[at] = v;
+  else static_cast<uint16_t *>(p.out)[at] = T::from_f32(v);
 }
 
 }  // namespace linear
