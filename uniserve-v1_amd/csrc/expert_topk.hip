@@ -3,14 +3,24 @@
 // expert_topk on gfx950: softmax or sigmoid scores, a balance bias, groups, top-k and weights
 // (include/uniserve_expert_topk.h states the operator).
 //
-// One wavefront per row; lane l holds experts l + 64 i. Scores and choices are doubles: two choices
-// a few 1e-9 apart are common among 128 to 512 experts over thousands of rows, and an FP32 sigmoid
-// plus bias orders such a pair by its rounding.
+// One wavefront per row. With G groups of S experts the 64 lanes are dealt to the groups, P = 64 over G
+// rounded up to a power of two each: lane g P + q holds the group's experts q, q + P, q + 2 P, .. (one group:
+// lane l holds l, l + 64, ..), so a group's rank meets in P neighbouring lanes and no choice passes LDS.
+//
+// The choice is defined in 64 bits: two choices a few 1e-9 apart are common among hundreds of experts over
+// thousands of rows, and an FP32 sigmoid plus bias orders such a pair by its rounding. Doubles everywhere
+// cost 22.9 us at 8192 x 256 (8 groups, top 8), most of it in their lane exchanges. So a row is first chosen
+// from in FP32, whose error is bounded, one pick further than asked; where every two neighbouring picks (and
+// the groups at the edge of the kept ones) are further apart than twice that error, the doubles would choose
+// the same, and only the picked scores are evaluated in 64 bits. Other rows (one in a few hundred with FP32
+// logits; exact ties, so every other with bf16 logits and no bias) choose again from doubles.
 #include "common.hpp"
 #include "uniserve_expert_topk.h"
 
 #include <cfloat>
+#include <climits>
 #include <cmath>
+#include <type_traits>
 
 namespace uniserve {
 namespace {
@@ -32,6 +42,8 @@ struct ChoiceParams {
   int groups;
   int top_groups;
   int group_top;
+  int size;       ///< experts of a group
+  int lane_bits;  ///< a group has 2^lane_bits lanes
   int kind;  ///< UNISERVE_DTYPE_F32, _BF16 or _F16
   int sigmoid;
   int renormalize;
@@ -44,125 +56,316 @@ __device__ __forceinline__ float load_logit(const void *data, int kind, int64_t 
   return bf16_to_f32(static_cast<const uint16_t *>(data)[index]);
 }
 
-__device__ __forceinline__ double wave_max(double x) {
-#pragma unroll
-  for (int offset = 32; offset > 0; offset /= 2) {
-    const double other = __shfl_xor(x, offset);
+/// The maximum over the wavefront, as a scalar: DPP shifts carry it to lane 15 of each 16-lane row, broadcasts
+/// from row to row to lane 63.
+__device__ __forceinline__ int wave_max(int x) {
+  auto step = [&](auto control) {
+    const int other = __builtin_amdgcn_update_dpp(INT_MIN, x, decltype(control)::value, 0xf, 0xf, false);
     x = x < other ? other : x;
-  }
-  return x;
+  };
+  step(std::integral_constant<int, 0x111>{});  // row_shr 1, 2, 4, 8
+  step(std::integral_constant<int, 0x112>{});
+  step(std::integral_constant<int, 0x114>{});
+  step(std::integral_constant<int, 0x118>{});
+  step(std::integral_constant<int, 0x142>{});  // row_bcast15, row_bcast31
+  step(std::integral_constant<int, 0x143>{});
+  return __builtin_amdgcn_readlane(x, 63);
 }
 
-__device__ __forceinline__ double wave_sum(double x) {
+/// Integers that order as the floats do (and -0 below 0).
+__device__ __forceinline__ int ordered(float x) {
+  const int bits = __float_as_int(x);
+  return bits ^ ((bits >> 31) & INT_MAX);
+}
+__device__ __forceinline__ float unordered(int key) { return __int_as_float(key ^ ((key >> 31) & INT_MAX)); }
+__device__ __forceinline__ float wave_max(float x) { return unordered(wave_max(ordered(x))); }
+
+template <class F>
+__device__ __forceinline__ F wave_sum(F x) {
 #pragma unroll
   for (int offset = 32; offset > 0; offset /= 2) x += __shfl_xor(x, offset);
   return x;
 }
 
+/// The lane's logits first, first + lanes, .. of a row (expert 0's in the place of those from `past` on): all
+/// loads in flight together.
+template <int kIter>
+__device__ __forceinline__ void load_row(const ChoiceParams &p, int64_t row, int first, int lanes, int past, float (&logit)[kIter]) {
+  int at[kIter];
+#pragma unroll
+  for (int i = 0; i < kIter; ++i) at[i] = first + i * lanes < past ? first + i * lanes : 0;
+  if (p.kind == UNISERVE_DTYPE_F32) {
+    const float *scores = static_cast<const float *>(p.scores) + row * p.row_stride;
+#pragma unroll
+    for (int i = 0; i < kIter; ++i) logit[i] = scores[at[i]];
+    return;
+  }
+  const uint16_t *scores = static_cast<const uint16_t *>(p.scores) + row * p.row_stride;
+  uint16_t bits[kIter];
+#pragma unroll
+  for (int i = 0; i < kIter; ++i) bits[i] = scores[at[i]];
+#pragma unroll
+  for (int i = 0; i < kIter; ++i)
+    logit[i] = p.kind == UNISERVE_DTYPE_F16 ? static_cast<float>(__builtin_bit_cast(_Float16, bits[i])) : bf16_to_f32(bits[i]);
+}
+
+/// The best two of two pairs (the larger first).
+template <class F>
+__device__ __forceinline__ void merge_best(F &best, F &second, F other, F other_second) {
+  const F low = best < other ? best : other;
+  best = best < other ? other : best;
+  second = second < other_second ? other_second : second;
+  second = second < low ? low : second;
+}
+
+/// Each lane's group's rank from the lane's choices: the group's best, plus its second where there is one and
+/// `group_top` is 2. `lanes`: P.
+template <int kIter, class F>
+__device__ __forceinline__ F group_rank(const F (&choice)[kIter], int lanes, int group_top) {
+  const F out = -static_cast<F>(__builtin_inff());
+  F best = out, second = out;
+#pragma unroll
+  for (int i = 0; i < kIter; ++i) merge_best(best, second, choice[i], out);
+  if constexpr (sizeof(F) == 4) {
+    // Quads, then the other quad of eight and the other eight of sixteen (all of a half hold the same by then).
+    auto step = [&](auto control) {
+      constexpr int kControl = decltype(control)::value;
+      merge_best(best, second, __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(best), kControl, 0xf, 0xf, false)),
+                 __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(second), kControl, 0xf, 0xf, false)));
+    };
+    if (lanes > 1) step(std::integral_constant<int, 0xb1>{});   // quad_perm [1, 0, 3, 2]
+    if (lanes > 2) step(std::integral_constant<int, 0x4e>{});   // quad_perm [2, 3, 0, 1]
+    if (lanes > 4) step(std::integral_constant<int, 0x141>{});  // row_half_mirror
+    if (lanes > 8) step(std::integral_constant<int, 0x140>{});  // row_mirror
+    for (int offset = 16; offset < lanes; offset *= 2) {
+      const F other = __shfl_xor(best, offset), other_second = __shfl_xor(second, offset);
+      merge_best(best, second, other, other_second);
+    }
+  } else {
+    for (int offset = 1; offset < lanes; offset *= 2) {
+      const F other = __shfl_xor(best, offset), other_second = __shfl_xor(second, offset);
+      merge_best(best, second, other, other_second);
+    }
+  }
+  return group_top == 2 && second > out ? best + second : best;
+}
+
+/// The lane's keys in descending order (Batcher's odd-even merge sort, kIter a power of two).
+template <int kIter>
+__device__ __forceinline__ void sort_descending(int (&key)[kIter]) {
+#pragma unroll
+  for (int run = 1; run < kIter; run *= 2)
+#pragma unroll
+    for (int step = run; step >= 1; step /= 2)
+#pragma unroll
+      for (int i = step % run; i + step < kIter; ++i) {
+        if ((i - step % run) / step % 2 != 0 || i / (2 * run) != (i + step) / (2 * run)) continue;
+        const int high = key[i] < key[i + step] ? key[i + step] : key[i];
+        key[i + step] = key[i] < key[i + step] ? key[i] : key[i + step];
+        key[i] = high;
+      }
+}
+
+/// The whole choice in 64 bits: lane j < top answers pick j's expert, or -1. A round takes the largest choice
+/// rounded to FP32 (which keeps the order or makes a tie) and, where several candidates share it, the largest
+/// double and the lowest expert among them.
+template <int kIter, class Score>
+__device__ __forceinline__ int choose_exactly(const ChoiceParams &p, int lane, int group, int first, int lanes,
+                                                        const float (&logit)[kIter], const float (&bias)[kIter],
+                                                        const Score &exact_score, double sum) {
+  const double out = -__builtin_inf();
+  double choice[kIter];
+#pragma unroll
+  for (int i = 0; i < kIter; ++i)
+    choice[i] = logit[i] > -__builtin_inff() ? exact_score(logit[i]) / sum + static_cast<double>(bias[i]) : out;
+  if (p.groups > 1) {
+    const double rank = group_rank(choice, lanes, p.group_top);
+    int ahead = 0;
+    for (int g = 0; g < p.groups; ++g) {
+      const double other = __shfl(rank, g << p.lane_bits);
+      ahead += other > rank || (other == rank && g < group);
+    }
+    if (ahead >= p.top_groups) {
+#pragma unroll
+      for (int i = 0; i < kIter; ++i) choice[i] = out;
+    }
+  }
+  int id = -1;
+  for (int j = 0; j < p.top; ++j) {
+    float own = -__builtin_inff();
+#pragma unroll
+    for (int i = 0; i < kIter; ++i) own = own < static_cast<float>(choice[i]) ? static_cast<float>(choice[i]) : own;
+    const float best = wave_max(own);
+    if (!(best > -__builtin_inff())) break;
+    // The lane's best candidate among those that round to `best`: the first of equal ones has the lower id.
+    double mine = out;
+    int expert = INT_MAX;
+#pragma unroll
+    for (int i = 0; i < kIter; ++i)
+      if (static_cast<float>(choice[i]) == best && choice[i] > mine) {
+        mine = choice[i];
+        expert = first + i * lanes;
+      }
+    const uint64_t holders = ballot(expert != INT_MAX);
+    if (__popcll(holders) > 1) {
+#pragma unroll
+      for (int offset = 32; offset > 0; offset /= 2) {
+        const double other = __shfl_xor(mine, offset);
+        const int other_expert = __shfl_xor(expert, offset);
+        if (other > mine || (other == mine && other_expert < expert)) {
+          mine = other;
+          expert = other_expert;
+        }
+      }
+    } else {
+      expert = __builtin_amdgcn_readlane(expert, __builtin_ctzll(holders));
+    }
+    if (lane == j) id = expert;
+#pragma unroll
+    for (int i = 0; i < kIter; ++i)
+      if (first + i * lanes == expert) choice[i] = out;
+  }
+  return id;
+}
+
 /// kIter: experts per lane.
 template <int kIter>
 __global__ void __launch_bounds__(kChoiceWaves *kWave) expert_topk_kernel(ChoiceParams p) {
-  extern __shared__ double choices[];  // [waves][experts], where the experts are in groups
   const int wave = static_cast<int>(threadIdx.x) / kWave;
   const int lane = lane_id();
   const int64_t row = static_cast<int64_t>(blockIdx.x) * kChoiceWaves + wave;
   if (row >= p.rows) return;
-  const double out = -__builtin_inf();
+  constexpr float kOut = -__builtin_inff();
+  const int lanes = 1 << p.lane_bits;
+  const int group = lane >> p.lane_bits;
+  const int first = group * p.size + (lane & (lanes - 1));  // the lane's expert i is first + i lanes
+  const int past = group < p.groups ? (group + 1) * p.size : 0;
 
-  double score[kIter], choice[kIter];
-  double maximum = out;
+  // Logits and biases; no candidate (comparisons with NaN are false) has a logit of -inf.
+  float logit[kIter], bias[kIter];
+  load_row<kIter>(p, row, first, lanes, past, logit);
+#pragma unroll
+  for (int i = 0; i < kIter; ++i) bias[i] = 0.0f;
+  if (p.bias != nullptr) {
+#pragma unroll
+    for (int i = 0; i < kIter; ++i) bias[i] = p.bias[first + i * lanes < past ? first + i * lanes : 0];
+  }
+  float maximum = kOut;
 #pragma unroll
   for (int i = 0; i < kIter; ++i) {
-    const int e = lane + kWave * i;
-    float logit = -__builtin_inff(), bias = 0.0f;
-    if (e < p.experts) {
-      logit = load_logit(p.scores, p.kind, row * p.row_stride + e);
-      if (p.bias != nullptr) bias = p.bias[e];
-    }
-    // Comparisons with NaN are false: a NaN logit or bias is no candidate either.
-    const bool candidate = logit > -__builtin_inff() && bias > -__builtin_inff();
-    logit = logit > FLT_MAX ? FLT_MAX : logit;
-    score[i] = candidate ? static_cast<double>(logit) : out;
-    choice[i] = candidate ? static_cast<double>(bias) : out;
-    maximum = maximum < score[i] ? score[i] : maximum;
+    const bool candidate = first + i * lanes < past && logit[i] > kOut && bias[i] > kOut;
+    logit[i] = candidate ? (logit[i] < FLT_MAX ? logit[i] : FLT_MAX) : kOut;
+    maximum = maximum < logit[i] ? logit[i] : maximum;
   }
+
+  // ---- the choice in FP32 ----
+  // A sigmoid here is off by less than 2^-22: in steps of 2^-24 the exponent's rounding gives 1.5 |l| s (1 - s)
+  // < 0.34, the exponential 0.5, 1 + e and the reciprocal 3. A softmax's probability is off by less than
+  // kIter + 12 steps of the row's largest: its sum adds kIter + 6 times, the exponent's rounding gives 2.5 x e^-x
+  // < 0.92, the exponential 2, the quotient and the product 2. The bias's addition rounds by half a step of the
+  // choice, and the slot in a key's low bits moves it by 2 kSlots. Two choices further apart than twice all
+  // this are ordered as in 64 bits.
+  constexpr int kSlotBits = kIter <= 1 ? 0 : kIter <= 2 ? 1 : kIter <= 4 ? 2 : kIter <= 8 ? 3 : kIter <= 16 ? 4 : 5;
+  constexpr int kSlots = (1 << kSlotBits) - 1;
+  float key[kIter];
+  float unsure;  // how far apart two scores have to be
   if (p.sigmoid) {
 #pragma unroll
-    for (int i = 0; i < kIter; ++i) score[i] = 1.0 / (1.0 + exp(-score[i]));
+    for (int i = 0; i < kIter; ++i)
+      key[i] = logit[i] > kOut ? __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.4426950408889634f * logit[i])) : kOut;
+    unsure = 0x1p-20f;
   } else {
     maximum = wave_max(maximum);
-    double sum = 0.0;
+    float sum = 0.0f;
 #pragma unroll
     for (int i = 0; i < kIter; ++i) {
-      score[i] = score[i] > out ? exp(score[i] - maximum) : 0.0;
-      sum += score[i];
+      key[i] = logit[i] > kOut ? __builtin_amdgcn_exp2f(1.4426950408889634f * (logit[i] - maximum)) : kOut;
+      sum += logit[i] > kOut ? key[i] : 0.0f;
     }
-    sum = wave_sum(sum);
+    const float scale = 1.0f / wave_sum(sum);
 #pragma unroll
-    for (int i = 0; i < kIter; ++i) score[i] = score[i] / sum;
+    for (int i = 0; i < kIter; ++i) key[i] *= scale;  // (-inf stays: the scale is positive, or the row is empty)
+    unsure = 2.0f * (kIter + 12) * 0x1p-24f * scale;
   }
 #pragma unroll
-  for (int i = 0; i < kIter; ++i) choice[i] = choice[i] > out ? score[i] + choice[i] : out;
+  for (int i = 0; i < kIter; ++i) key[i] = logit[i] > kOut ? key[i] + bias[i] : kOut;
+  constexpr float kUnsureOf = (8.0f + 8.0f * kSlots) * 0x1p-24f;  // of a choice's own size
 
+  bool sure = true;
   if (p.groups > 1) {
-    // Lane g ranks group g; a group's rank is the number of groups before it.
-    double *own = choices + wave * p.experts;
+    const float rank = group_rank(key, lanes, p.group_top);
+    const float size = __builtin_fabsf(rank);
+    const float margin = 2.0f * unsure + 0x1p-20f * wave_max(size < __builtin_inff() ? size : 0.0f);
+    // Lane (g, q) compares group g with the groups q, q + P, ..; the ballots hold the P lanes' answers of a group
+    // side by side. `near` counts the groups that may lie ahead, its own among them.
+    const float above = rank + margin, below = rank - margin;
+    const uint64_t mine = (lanes < kWave ? (1ull << lanes) - 1ull : ~0ull) << (group << p.lane_bits);
+    int ahead = 0, near = -1;
+    for (int g = 0; g < p.groups; g += lanes) {
+      const int with = g + (lane & (lanes - 1));
+      const float other = __shfl(rank, (with << p.lane_bits) & (kWave - 1));
+      ahead += __popcll(ballot(with < p.groups && other > above) & mine);
+      near += __popcll(ballot(with < p.groups && other >= below) & mine);
+    }
+    const bool out = ahead >= p.top_groups;
+    sure = ballot(rank > kOut && !out && near >= p.top_groups) == 0;
+    if (out) {
 #pragma unroll
-    for (int i = 0; i < kIter; ++i) {
-      const int e = lane + kWave * i;
-      if (e < p.experts) own[e] = choice[i];
-    }
-    __builtin_amdgcn_wave_barrier();
-    const int size = p.experts / p.groups;
-    double best = out, second = out;
-    if (lane < p.groups) {
-      for (int e = lane * size; e < (lane + 1) * size; ++e) {
-        const double c = own[e];
-        second = c > best ? best : (c > second ? c : second);
-        best = c > best ? c : best;
-      }
-    }
-    const double rank = p.group_top == 2 && second > out ? best + second : best;
-    int ahead = 0;
-    for (int g = 0; g < p.groups; ++g) {
-      const double other = __shfl(rank, g);
-      ahead += other > rank || (other == rank && g < lane);
-    }
-    const uint64_t kept = ballot(lane < p.groups && ahead < p.top_groups);
-#pragma unroll
-    for (int i = 0; i < kIter; ++i) {
-      const int e = lane + kWave * i;
-      if (e < p.experts && !((kept >> (e / size)) & 1u)) choice[i] = out;
+      for (int i = 0; i < kIter; ++i) key[i] = kOut;
     }
   }
 
-  // `top` rounds: the largest choice left, the lowest expert holding it; lane j keeps round j's.
-  double picked = 0.0;
   int id = -1;
-  for (int j = 0; j < p.top; ++j) {
-    double best = choice[0];
+  if (sure) {
+    // The lane's choices as ordered integers, the slot in the low bits, in descending order; a round's offer is
+    // the lane's first, and only the lane whose offer won moves on. Lane j keeps pick j and its lane.
+    int order[kIter];
 #pragma unroll
-    for (int i = 1; i < kIter; ++i) best = best < choice[i] ? choice[i] : best;
-    best = wave_max(best);
-    if (!(best > out)) break;
-    bool found = false;
+    for (int i = 0; i < kIter; ++i) order[i] = key[i] > kOut ? (ordered(key[i]) & ~kSlots) | i : INT_MIN;
+    sort_descending(order);
+    int pick = INT_MIN, holder_of = 0;
+    for (int j = 0; j <= p.top; ++j) {
+      const int best = wave_max(order[0]);
+      if (best == INT_MIN) break;
+      const int holder = __builtin_ctzll(ballot(order[0] == best));
+      pick = lane == j ? best : pick;
+      holder_of = lane == j ? holder : holder_of;
+      if (lane == holder) {
 #pragma unroll
-    for (int i = 0; i < kIter; ++i) {
-      const uint64_t holders = ballot(choice[i] == best);
-      if (found || holders == 0) continue;
-      found = true;
-      const int holder = __builtin_ctzll(holders);
-      const double s = __shfl(score[i], holder);
-      if (lane == j) {
-        picked = s;
-        id = holder + kWave * i;
+        for (int i = 0; i + 1 < kIter; ++i) order[i] = order[i + 1];
+        order[kIter - 1] = INT_MIN;
       }
-      if (lane == holder) choice[i] = out;
     }
+    // Neighbouring picks, the one past the last among them (an infinite one is never sure).
+    const int next = __shfl_down(pick, 1);
+    const float here = unordered(pick), there = unordered(next);
+    const float apart = unsure + kUnsureOf * __builtin_fmaxf(__builtin_fabsf(here), __builtin_fabsf(there));
+    sure = ballot(lane < p.top && next != INT_MIN && !(here - there > apart)) == 0;
+    if (pick != INT_MIN) id = (holder_of >> p.lane_bits) * p.size + (holder_of & (lanes - 1)) + (pick & kSlots) * lanes;
+  }
+
+  // ---- 64 bits: the picked scores, or the whole choice ----
+  const auto exact_score = [&](float l) {  // (softmax: times the sum)
+    return p.sigmoid ? 1.0 / (1.0 + exp(-static_cast<double>(l))) : exp(static_cast<double>(l) - static_cast<double>(maximum));
+  };
+  double sum = 1.0;
+  if (!p.sigmoid && (!sure || !p.renormalize)) {
+    sum = 0.0;
+#pragma unroll
+    for (int i = 0; i < kIter; ++i)
+      if (logit[i] > kOut) sum += exact_score(logit[i]);
+    sum = wave_sum(sum);
+  }
+  if (!sure) id = choose_exactly<kIter>(p, lane, group, first, lanes, logit, bias, exact_score, sum);
+  double picked = 0.0;
+  if (lane < p.top && id >= 0) {
+    float l = load_logit(p.scores, p.kind, row * p.row_stride + id);
+    picked = exact_score(l < FLT_MAX ? l : FLT_MAX) / sum;
   }
   if (p.renormalize) {
-    const double sum = wave_sum(picked);
-    picked = sum > 0.0 ? picked / sum : 0.0;
+    double total = picked;
+    for (int offset = 1; offset < p.top; offset *= 2) total += __shfl_xor(total, offset);
+    picked = total > 0.0 ? picked / total : 0.0;
   }
   if (lane >= p.top) return;
   p.ids[row * p.top + lane] = id >= 0 && p.map != nullptr ? p.map[id] : id;
@@ -172,9 +375,8 @@ __global__ void __launch_bounds__(kChoiceWaves *kWave) expert_topk_kernel(Choice
 
 template <int kIter>
 void launch_choice(const ChoiceParams &p, hipStream_t stream) {
-  const size_t lds = p.groups > 1 ? sizeof(double) * kChoiceWaves * p.experts : 0;
   const dim3 grid(static_cast<uint32_t>(ceil_div<int64_t>(p.rows, kChoiceWaves)));
-  hipLaunchKernelGGL(expert_topk_kernel<kIter>, grid, dim3(kChoiceWaves * kWave), lds, stream, p);
+  hipLaunchKernelGGL(expert_topk_kernel<kIter>, grid, dim3(kChoiceWaves * kWave), 0, stream, p);
 }
 
 }  // namespace
@@ -228,12 +430,18 @@ extern "C" int32_t uniserve_expert_topk(const uniserve_expert_topk_call *call, v
     p.renormalize = call->renormalize != 0;
     p.factor = call->factor;
     const hipStream_t s = static_cast<hipStream_t>(stream);
-    const int needed = ceil_div(p.experts, kWave);
+    // Groups that all stay limit nothing.
+    if (p.top_groups == p.groups) p.groups = p.top_groups = 1;
+    p.size = p.experts / p.groups;
+    p.lane_bits = 6;
+    while ((kWave >> p.lane_bits) < p.groups) --p.lane_bits;
+    const int needed = ceil_div(p.size, 1 << p.lane_bits);
     if (needed <= 1) launch_choice<1>(p, s);
     else if (needed <= 2) launch_choice<2>(p, s);
     else if (needed <= 4) launch_choice<4>(p, s);
     else if (needed <= 8) launch_choice<8>(p, s);
-    else launch_choice<16>(p, s);
+    else if (needed <= 16) launch_choice<16>(p, s);
+    else launch_choice<32>(p, s);
     return launched(call, "expert_topk");
   });
 }
