@@ -52,9 +52,11 @@ def _stream(device=None):
     return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
 
 
-#: The handle of a device's current stream, without the Stream object that ``current_stream`` builds around it
-#: (0.1 us a call, not 1.9): the small operators' calls cost the host more than the device.
+# The small operators' calls cost the host more than the device, so they take the current stream's handle and the
+# current device's number without the objects that ``torch.cuda`` builds around them (0.1 us each, not 1.9 and 0.25),
+# compare devices by number (-1: the host) and read shapes and strides whole.
 _raw_stream = torch._C._cuda_getCurrentRawStream
+_current_device = torch._C._cuda_getDevice
 
 
 def _ptr(tensor):
@@ -88,28 +90,34 @@ def topk_softmax(scores, top, renormalize=True, scale=None, mapping=None, live=N
     return ids, weights
 
 
-def _enter(entry, call, device, name):
-    """Calls ``entry`` on the device's current stream, with that device current."""
-    index = device.index
-    if index == torch.cuda.current_device():
+def _enter(entry, call, index, name):
+    """Calls ``entry`` on the current stream of device ``index``, with that device current."""
+    if index == _current_device():
         status = entry(call, _raw_stream(index))
     else:
-        with torch.cuda.device(device):
+        with torch.cuda.device(index):
             status = entry(call, _raw_stream(index))
     if status != 0:
         _check(status, call, name)
 
 
-def _matrix(tensor, rows, columns, name, what):
-    """Refuses a tensor that is no [rows, columns] matrix of contiguous rows."""
-    if tensor.shape != (rows, columns) or (tensor.stride(1) != 1 and columns > 1):
-        raise ValueError(f"{name}: {what} is [{rows}, {columns}], its rows contiguous: got {tuple(tensor.shape)}, "
-                         f"strides {tensor.stride()}")
+def _matrix(tensor, rows, columns, index, name, what):
+    """The row stride of a [rows, columns] matrix of contiguous rows on device ``index``; refuses any other."""
+    if tensor.shape == (rows, columns) and tensor.get_device() == index:
+        stride, step = tensor.stride()
+        if step == 1 or columns <= 1:
+            return stride
+    raise ValueError(f"{name}: {what} is [{rows}, {columns}], its rows contiguous, on device {index}: got "
+                     f"{tuple(tensor.shape)}, strides {tensor.stride()}, on {tensor.device}")
 
 
-def _vector(tensor, count, dtypes, device, name, what):
-    if tensor.shape != (count,) or tensor.dtype not in dtypes or tensor.device != device or not tensor.is_contiguous():
-        raise ValueError(f"{name}: {what} is [{count}] of {' or '.join(str(d) for d in dtypes)} on {device}, contiguous")
+def _vector(tensor, count, dtypes, index, name, what):
+    """The address of a contiguous vector of one of ``dtypes``, or None for None."""
+    if tensor is None:
+        return None
+    if tensor.shape != (count,) or tensor.dtype not in dtypes or tensor.get_device() != index or not tensor.is_contiguous():
+        raise ValueError(f"{name}: {what} is [{count}] of {' or '.join(str(d) for d in dtypes)} on device {index}, contiguous")
+    return tensor.data_ptr()
 
 
 def expert_topk(scores, top, scoring="sigmoid", bias=None, groups=1, top_groups=1, group_top=2, renormalize=True,
@@ -125,69 +133,67 @@ def expert_topk(scores, top, scoring="sigmoid", bias=None, groups=1, top_groups=
 
     A logit (or a bias) of -inf or NaN takes its expert out; where too few are left, ids are -1 with
     weight 0, which ``moe_sort`` skips. ``mapping``, ``live`` and ``load`` are ``topk_softmax``'s."""
-    if scores.dim() != 2 or scores.dtype not in _ELEMENT or not scores.is_cuda:
+    element, index = _ELEMENT.get(scores.dtype), scores.get_device()
+    if scores.dim() != 2 or element is None or index < 0:
         raise ValueError("expert_topk: the scores are [tokens, experts] of f32, bf16 or f16 on a GPU")
     if scoring not in SCORING:
         raise ValueError(f"expert_topk: scoring is one of {sorted(SCORING)}, got {scoring!r}")
     tokens, experts = scores.shape
-    device = scores.device
-    _matrix(scores, tokens, experts, "expert_topk", "scores")
-    if bias is not None:
-        _vector(bias, experts, (torch.float32,), device, "expert_topk", "bias")
-    if mapping is not None:
-        _vector(mapping, experts, (torch.int32,), device, "expert_topk", "mapping")
-    if load is not None:
-        _vector(load, experts, (torch.int64,), device, "expert_topk", "load")
-    if live is not None and (live.numel() != 1 or live.dtype not in (torch.int32, torch.uint32) or live.device != device):
+    stride = _matrix(scores, tokens, experts, index, "expert_topk", "scores")
+    if live is not None and (live.numel() != 1 or live.dtype not in (torch.int32, torch.uint32) or live.get_device() != index):
         raise ValueError("expert_topk: live is one int32 on the scores' device")
-    ids = torch.empty((tokens, max(top, 0)), dtype=torch.int32, device=device)
-    weights = torch.empty((tokens, max(top, 0)), dtype=torch.float32, device=device)
-    call = ExpertTopkCall(scores.data_ptr(), _ptr(bias), _ptr(mapping), _ptr(live), _ptr(load), ids.data_ptr(),
-                          weights.data_ptr(), scores.stride(0), tokens, experts, top, groups, top_groups, group_top,
-                          _ELEMENT[scores.dtype], SCORING[scoring], 1 if renormalize else 0, factor)
-    _enter(library().uniserve_expert_topk, call, device, "expert_topk")
+    shape, device = (tokens, top if top > 0 else 0), scores.device
+    ids = torch.empty(shape, dtype=torch.int32, device=device)
+    weights = torch.empty(shape, dtype=torch.float32, device=device)
+    call = ExpertTopkCall(scores.data_ptr(), _vector(bias, experts, (torch.float32,), index, "expert_topk", "bias"),
+                          _vector(mapping, experts, (torch.int32,), index, "expert_topk", "mapping"), _ptr(live),
+                          _vector(load, experts, (torch.int64,), index, "expert_topk", "load"), ids.data_ptr(),
+                          weights.data_ptr(), stride, tokens, experts, top, groups, top_groups, group_top, element,
+                          SCORING[scoring], 1 if renormalize else 0, factor)
+    _enter(library().uniserve_expert_topk, call, index, "expert_topk")
     return ids, weights
 
 
 def _product(entry, name, x, weight, columns, bias, activation, gate, residual, out, out_dtype):
-    if x.dim() != 2 or x.dtype not in _PRODUCT or not x.is_cuda:
+    dtype, index = x.dtype, x.get_device()
+    element = _ELEMENT.get(dtype)
+    if x.dim() != 2 or dtype not in _PRODUCT or index < 0:
         raise ValueError(f"{name}: the input is [tokens, width] of bf16 or f16 on a GPU")
-    if weight.dtype != x.dtype or weight.device != x.device:
-        raise ValueError(f"{name}: the weight is the input's type, on its device")
+    if weight.dtype != dtype:
+        raise ValueError(f"{name}: the weight is the input's type")
     if activation not in LINEAR_ACTIVATION:
         raise ValueError(f"{name}: activation is one of silu, gelu_tanh or none, got {activation!r}")
     tokens, width = x.shape
-    device = x.device
-    _matrix(x, tokens, width, name, "the input")
-    _matrix(weight, weight.shape[0], width, name, "the weight")
+    x_stride = _matrix(x, tokens, width, index, name, "the input")
+    weight_stride = _matrix(weight, weight.shape[0], width, index, name, "the weight")
     if out is None:
-        out_dtype = x.dtype if out_dtype is None else out_dtype
-        if out_dtype not in _ELEMENT:
+        if out_dtype is None or out_dtype == dtype:
+            out_dtype, out_element, out = dtype, element, x.new_empty((tokens, columns))
+        elif out_dtype in _ELEMENT:
+            out_element, out = _ELEMENT[out_dtype], x.new_empty((tokens, columns), dtype=out_dtype)
+        else:
             raise ValueError(f"{name}: the output is the input's type or f32")
-        out = x.new_empty((tokens, columns), dtype=out_dtype)
+        out_stride = columns
     else:
         out_dtype = out.dtype if out_dtype is None else out_dtype
-        if out.dtype != out_dtype or out_dtype not in _ELEMENT or out.device != device:
-            raise ValueError(f"{name}: the output is the input's type or f32 (as out_dtype says), on {device}")
-        _matrix(out, tokens, columns, name, "the output")
-    element = _ELEMENT[x.dtype]
-    bias_element, gate_stride, residual_stride = element, 0, 0
+        if out.dtype != out_dtype or out_dtype not in _ELEMENT:
+            raise ValueError(f"{name}: the output is the input's type or f32, as out_dtype says")
+        out_element, out_stride = _ELEMENT[out_dtype], _matrix(out, tokens, columns, index, name, "the output")
+    bias_at, bias_element, gate_at, gate_stride, residual_at, residual_stride = None, element, None, 0, None, 0
     if bias is not None:
-        _vector(bias, weight.shape[0], (x.dtype, torch.float32), device, name, "the bias")
-        bias_element = _ELEMENT[bias.dtype]
+        bias_at, bias_element = _vector(bias, weight.shape[0], (dtype, torch.float32), index, name, "the bias"), _ELEMENT[bias.dtype]
     if gate is not None:
-        if gate.shape != (tokens, 1) or gate.dtype != x.dtype or gate.device != device:
-            raise ValueError(f"{name}: the gate is one logit per row, [tokens, 1] of the input's type on its device")
-        gate_stride = gate.stride(0)
+        if gate.dtype != dtype:
+            raise ValueError(f"{name}: the gate is one logit per row of the input's type")
+        gate_at, gate_stride = gate.data_ptr(), _matrix(gate, tokens, 1, index, name, "the gate")
     if residual is not None:
-        if residual.dtype != out_dtype or residual.device != device:
-            raise ValueError(f"{name}: the residual is of the output's type, on its device")
-        _matrix(residual, tokens, columns, name, "the residual")
-        residual_stride = residual.stride(0)
-    call = LinearCall(x.data_ptr(), weight.data_ptr(), _ptr(bias), _ptr(gate), _ptr(residual), out.data_ptr(), tokens,
-                      columns, width, x.stride(0), weight.stride(0), gate_stride, residual_stride, out.stride(0),
-                      element, bias_element, _ELEMENT[out_dtype], LINEAR_ACTIVATION[activation])
-    _enter(entry, call, device, name)
+        if residual.dtype != out_dtype:
+            raise ValueError(f"{name}: the residual is of the output's type")
+        residual_at, residual_stride = residual.data_ptr(), _matrix(residual, tokens, columns, index, name, "the residual")
+    call = LinearCall(x.data_ptr(), weight.data_ptr(), bias_at, gate_at, residual_at, out.data_ptr(), tokens, columns,
+                      width, x_stride, weight_stride, gate_stride, residual_stride, out_stride, element, bias_element,
+                      out_element, LINEAR_ACTIVATION[activation])
+    _enter(entry, call, index, name)
     return out
 
 
