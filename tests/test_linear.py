@@ -15,7 +15,7 @@ import numpy as np
 import pytest
 import torch
 
-from gpu_helpers import announce
+from gpu_helpers import announce, kernels_of
 from uniserve_moe import abi, ops
 
 U = 2.0**-24
@@ -202,6 +202,52 @@ def test_gated_linear(device, m, n, k, dtype, activation):
     assert_near(ops.gated_linear(x, w, activation=activation), reference(x, w, None, activation, gated=True))
     bias = normal((2 * n,), 5, 0.5, dtype if n % 2 else F32)
     assert_near(ops.gated_linear(x, w, bias=bias, activation=activation), reference(x, w, bias, activation, gated=True), "bias")
+
+
+#: Calls that the choice gives to each kernel: tokens and weight rows of a tile, wavefronts over them, stages
+#: of the ring, teams. K ends inside a stage, short of the ring, and leaves teams without a stage.
+KERNELS = [
+    (False, "256,256,2,4,2,1", 1025, 8200, 520), (True, "256,256,2,4,2,1", 513, 8200, 136),
+    (False, "128,128,2,2,2,1", 513, 8200, 72), (True, "128,128,2,2,2,1", 257, 8200, 72),
+    (False, "128,128,2,4,3,1", 513, 4104, 72), (True, "128,128,2,4,3,1", 200, 4104, 200),
+    (False, "128,64,2,2,3,1", 400, 8200, 72), (True, "128,64,2,2,3,1", 130, 8200, 72),
+    (False, "128,64,4,2,4,1", 200, 4104, 72), (True, "128,64,4,2,4,1", 100, 4104, 72),
+    (False, "64,64,2,2,4,1", 5, 8200, 200), (True, "64,64,2,2,4,1", 5, 8200, 72),
+    (False, "64,32,1,1,3,4", 33, 4104, 520), (True, "64,32,1,1,3,4", 130, 1000, 520),
+    (False, "32,32,1,1,4,4", 5, 40, 72), (True, "32,32,1,1,4,4", 17, 40, 200), (False, "32,32,1,1,4,4", 40, 136, 8),
+    (False, "16,16,1,1,4,8", 17, 130, 1032), (False, "16,16,1,1,4,8", 5, 17, 2056),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("gated, shape, m, n, k", KERNELS)
+def test_each_tile_kernel(device, gated, shape, m, n, k):
+    announce("linear kernel", shape, gated, m, n, k)
+    x, w, out = normal((m, k), 1), normal((n * (2 if gated else 1), k), 2, 0.05), normal((m, n), 3)
+    gate, residual = normal((m, 1), 4), normal((m, n), 5)
+
+    def call():
+        if gated:
+            return ops.gated_linear(x, w, out=out)
+        return ops.linear(x, w, gate=gate, residual=residual, out=out)
+
+    mangled = "TileShapeI" + "".join(f"Li{d}E" for d in shape.split(","))
+    names = kernels_of(call)
+    assert len(names) == 1 and mangled in names[0], names
+    call()
+    assert_near(out, reference(x, w, None, "silu", gated=True) if gated else reference(x, w, gate=gate, residual=residual))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("k", [8, 56, 64, 72, 128, 192, 256, 264, 512, 576, 2048, 2056])
+def test_short_and_ragged_walks(device, gated, k):
+    """Every count of stages around the rings' and the teams', whole and ragged."""
+    announce("linear walks", gated, k)
+    for m, n in ((20, 48), (150, 200)):
+        x, w = normal((m, k), k), normal((n * (2 if gated else 1), k), k + 1, 0.05)
+        got = ops.gated_linear(x, w) if gated else ops.linear(x, w)
+        assert_near(got, reference(x, w, None, "silu", gated=True) if gated else reference(x, w), f"{m} x {n}")
 
 
 @pytest.mark.gpu

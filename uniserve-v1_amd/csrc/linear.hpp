@@ -26,6 +26,10 @@ struct LinearParams {
   int32_t out_of_8;      ///< out (and residual) rows start at 16-byte aligned addresses
 };
 
+/// Launches a call that was found servable.
+void launch_bf16(const LinearParams &p, bool gated, hipStream_t stream);
+void launch_f16(const LinearParams &p, bool gated, hipStream_t stream);
+
 struct Bf16 {
   static __device__ __forceinline__ float low(uint32_t pair) { return __uint_as_float(pair << 16); }
   static __device__ __forceinline__ float high(uint32_t pair) { return __uint_as_float(pair & 0xffff0000u); }
