@@ -57,18 +57,17 @@ __device__ __forceinline__ float load_logit(const void *data, int kind, int64_t 
 }
 
 /// The maximum over the wavefront, as a scalar: DPP shifts carry it to lane 15 of each 16-lane row, broadcasts
-/// from row to row to lane 63.
+/// from row to row to lane 63. (In place and in one piece: written with the DPP builtin, every step costs a copy
+/// too. A DPP read of a register comes two wait states after its write.)
 __device__ __forceinline__ int wave_max(int x) {
-  auto step = [&](auto control) {
-    const int other = __builtin_amdgcn_update_dpp(INT_MIN, x, decltype(control)::value, 0xf, 0xf, false);
-    x = x < other ? other : x;
-  };
-  step(std::integral_constant<int, 0x111>{});  // row_shr 1, 2, 4, 8
-  step(std::integral_constant<int, 0x112>{});
-  step(std::integral_constant<int, 0x114>{});
-  step(std::integral_constant<int, 0x118>{});
-  step(std::integral_constant<int, 0x142>{});  // row_bcast15, row_bcast31
-  step(std::integral_constant<int, 0x143>{});
+  asm("s_nop 1\n\t"
+      "v_max_i32_dpp %0, %0, %0 row_shr:1 row_mask:0xf bank_mask:0xf\n\ts_nop 1\n\t"
+      "v_max_i32_dpp %0, %0, %0 row_shr:2 row_mask:0xf bank_mask:0xf\n\ts_nop 1\n\t"
+      "v_max_i32_dpp %0, %0, %0 row_shr:4 row_mask:0xf bank_mask:0xf\n\ts_nop 1\n\t"
+      "v_max_i32_dpp %0, %0, %0 row_shr:8 row_mask:0xf bank_mask:0xf\n\ts_nop 1\n\t"
+      "v_max_i32_dpp %0, %0, %0 row_bcast:15 row_mask:0xf bank_mask:0xf\n\ts_nop 1\n\t"
+      "v_max_i32_dpp %0, %0, %0 row_bcast:31 row_mask:0xf bank_mask:0xf"
+      : "+v"(x));
   return __builtin_amdgcn_readlane(x, 63);
 }
 
@@ -118,36 +117,28 @@ __device__ __forceinline__ void merge_best(F &best, F &second, F other, F other_
   second = second < low ? low : second;
 }
 
-/// Each lane's group's rank from the lane's choices: the group's best, plus its second where there is one and
-/// `group_top` is 2. `lanes`: P.
-template <int kIter, class F>
-__device__ __forceinline__ F group_rank(const F (&choice)[kIter], int lanes, int group_top) {
-  const F out = -static_cast<F>(__builtin_inff());
-  F best = out, second = out;
-#pragma unroll
-  for (int i = 0; i < kIter; ++i) merge_best(best, second, choice[i], out);
-  if constexpr (sizeof(F) == 4) {
-    // Quads, then the other quad of eight and the other eight of sixteen (all of a half hold the same by then).
-    auto step = [&](auto control) {
-      constexpr int kControl = decltype(control)::value;
-      merge_best(best, second, __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(best), kControl, 0xf, 0xf, false)),
-                 __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(second), kControl, 0xf, 0xf, false)));
-    };
-    if (lanes > 1) step(std::integral_constant<int, 0xb1>{});   // quad_perm [1, 0, 3, 2]
-    if (lanes > 2) step(std::integral_constant<int, 0x4e>{});   // quad_perm [2, 3, 0, 1]
-    if (lanes > 4) step(std::integral_constant<int, 0x141>{});  // row_half_mirror
-    if (lanes > 8) step(std::integral_constant<int, 0x140>{});  // row_mirror
-    for (int offset = 16; offset < lanes; offset *= 2) {
-      const F other = __shfl_xor(best, offset), other_second = __shfl_xor(second, offset);
-      merge_best(best, second, other, other_second);
-    }
-  } else {
-    for (int offset = 1; offset < lanes; offset *= 2) {
-      const F other = __shfl_xor(best, offset), other_second = __shfl_xor(second, offset);
-      merge_best(best, second, other, other_second);
-    }
+/// Each lane's group's two best choices, from the lanes' own best two. `lanes`: P.
+__device__ __forceinline__ void group_best(int &best, int &second, int lanes) {
+  // Quads, then the other quad of eight and the other eight of sixteen (all of a half hold the same by then).
+  auto step = [&](auto control) {
+    constexpr int kControl = decltype(control)::value;
+    merge_best(best, second, __builtin_amdgcn_mov_dpp(best, kControl, 0xf, 0xf, false),
+               __builtin_amdgcn_mov_dpp(second, kControl, 0xf, 0xf, false));
+  };
+  if (lanes > 1) step(std::integral_constant<int, 0xb1>{});   // quad_perm [1, 0, 3, 2]
+  if (lanes > 2) step(std::integral_constant<int, 0x4e>{});   // quad_perm [2, 3, 0, 1]
+  if (lanes > 4) step(std::integral_constant<int, 0x141>{});  // row_half_mirror
+  if (lanes > 8) step(std::integral_constant<int, 0x140>{});  // row_mirror
+  for (int offset = 16; offset < lanes; offset *= 2) {
+    const int other = __shfl_xor(best, offset), other_second = __shfl_xor(second, offset);
+    merge_best(best, second, other, other_second);
   }
-  return group_top == 2 && second > out ? best + second : best;
+}
+__device__ __forceinline__ void group_best(double &best, double &second, int lanes) {
+  for (int offset = 1; offset < lanes; offset *= 2) {
+    const double other = __shfl_xor(best, offset), other_second = __shfl_xor(second, offset);
+    merge_best(best, second, other, other_second);
+  }
 }
 
 /// The lane's keys in descending order (Batcher's odd-even merge sort, kIter a power of two).
@@ -177,9 +168,13 @@ __device__ __forceinline__ int choose_exactly(const ChoiceParams &p, int lane, i
   double choice[kIter];
 #pragma unroll
   for (int i = 0; i < kIter; ++i)
-    choice[i] = logit[i] > -__builtin_inff() ? exact_score(logit[i]) / sum + static_cast<double>(bias[i]) : out;
+    choice[i] = logit[i] > -__builtin_inff() ? (p.sigmoid ? exact_score(logit[i]) : exact_score(logit[i]) / sum) + static_cast<double>(bias[i]) : out;
   if (p.groups > 1) {
-    const double rank = group_rank(choice, lanes, p.group_top);
+    double rank = out, second = out;
+#pragma unroll
+    for (int i = 0; i < kIter; ++i) merge_best(rank, second, choice[i], out);
+    group_best(rank, second, lanes);
+    if (p.group_top == 2 && second > out) rank += second;
     int ahead = 0;
     for (int g = 0; g < p.groups; ++g) {
       const double other = __shfl(rank, g << p.lane_bits);
@@ -253,7 +248,7 @@ __global__ void __launch_bounds__(kChoiceWaves *kWave) expert_topk_kernel(Choice
   float maximum = kOut;
 #pragma unroll
   for (int i = 0; i < kIter; ++i) {
-    const bool candidate = first + i * lanes < past && logit[i] > kOut && bias[i] > kOut;
+    const bool candidate = (first + i * lanes < past) & (logit[i] > kOut) & (bias[i] > kOut);
     logit[i] = candidate ? (logit[i] < FLT_MAX ? logit[i] : FLT_MAX) : kOut;
     maximum = maximum < logit[i] ? logit[i] : maximum;
   }
@@ -267,33 +262,44 @@ __global__ void __launch_bounds__(kChoiceWaves *kWave) expert_topk_kernel(Choice
   // this are ordered as in 64 bits.
   constexpr int kSlotBits = kIter <= 1 ? 0 : kIter <= 2 ? 1 : kIter <= 4 ? 2 : kIter <= 8 ? 3 : kIter <= 16 ? 4 : 5;
   constexpr int kSlots = (1 << kSlotBits) - 1;
-  float key[kIter];
+  constexpr float kUnsureOf = (8.0f + 8.0f * kSlots) * 0x1p-24f;  // of a choice's own size
+  float score[kIter];
   float unsure;  // how far apart two scores have to be
   if (p.sigmoid) {
 #pragma unroll
-    for (int i = 0; i < kIter; ++i)
-      key[i] = logit[i] > kOut ? __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.4426950408889634f * logit[i])) : kOut;
+    for (int i = 0; i < kIter; ++i) score[i] = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.4426950408889634f * logit[i]));
     unsure = 0x1p-20f;
   } else {
     maximum = wave_max(maximum);
     float sum = 0.0f;
 #pragma unroll
     for (int i = 0; i < kIter; ++i) {
-      key[i] = logit[i] > kOut ? __builtin_amdgcn_exp2f(1.4426950408889634f * (logit[i] - maximum)) : kOut;
-      sum += logit[i] > kOut ? key[i] : 0.0f;
+      score[i] = logit[i] > kOut ? __builtin_amdgcn_exp2f(1.4426950408889634f * (logit[i] - maximum)) : 0.0f;
+      sum += score[i];
     }
     const float scale = 1.0f / wave_sum(sum);
 #pragma unroll
-    for (int i = 0; i < kIter; ++i) key[i] *= scale;  // (-inf stays: the scale is positive, or the row is empty)
+    for (int i = 0; i < kIter; ++i) score[i] *= scale;
     unsure = 2.0f * (kIter + 12) * 0x1p-24f * scale;
   }
+  // The lane's choices as ordered integers; no candidate: below kLowest, the lowest finite float, also with a
+  // slot in the low bits.
+  constexpr int kLowest = INT_MIN + 0x800000;
+  int order[kIter];
 #pragma unroll
-  for (int i = 0; i < kIter; ++i) key[i] = logit[i] > kOut ? key[i] + bias[i] : kOut;
-  constexpr float kUnsureOf = (8.0f + 8.0f * kSlots) * 0x1p-24f;  // of a choice's own size
+  for (int i = 0; i < kIter; ++i) {
+    const float choice = score[i] + bias[i];
+    order[i] = ordered(logit[i] > kOut ? choice : kOut);
+  }
 
   bool sure = true;
   if (p.groups > 1) {
-    const float rank = group_rank(key, lanes, p.group_top);
+    int best = INT_MIN, second = INT_MIN;
+#pragma unroll
+    for (int i = 0; i < kIter; ++i) merge_best(best, second, order[i], INT_MIN);
+    group_best(best, second, lanes);
+    float rank = best < kLowest ? kOut : unordered(best);
+    if (p.group_top == 2) rank += second < kLowest ? 0.0f : unordered(second);
     const float size = __builtin_fabsf(rank);
     const float margin = 2.0f * unsure + 0x1p-20f * wave_max(size < __builtin_inff() ? size : 0.0f);
     // Lane (g, q) compares group g with the groups q, q + P, ..; the ballots hold the P lanes' answers of a group
@@ -304,29 +310,26 @@ __global__ void __launch_bounds__(kChoiceWaves *kWave) expert_topk_kernel(Choice
     for (int g = 0; g < p.groups; g += lanes) {
       const int with = g + (lane & (lanes - 1));
       const float other = __shfl(rank, (with << p.lane_bits) & (kWave - 1));
-      ahead += __popcll(ballot(with < p.groups && other > above) & mine);
-      near += __popcll(ballot(with < p.groups && other >= below) & mine);
+      ahead += __popcll(ballot((with < p.groups) & (other > above)) & mine);
+      near += __popcll(ballot((with < p.groups) & (other >= below)) & mine);
     }
     const bool out = ahead >= p.top_groups;
-    sure = ballot(rank > kOut && !out && near >= p.top_groups) == 0;
-    if (out) {
+    sure = ballot((rank > kOut) & !out & (near >= p.top_groups)) == 0;
 #pragma unroll
-      for (int i = 0; i < kIter; ++i) key[i] = kOut;
-    }
+    for (int i = 0; i < kIter; ++i) order[i] = out ? INT_MIN : order[i];
   }
 
   int id = -1;
   if (sure) {
-    // The lane's choices as ordered integers, the slot in the low bits, in descending order; a round's offer is
-    // the lane's first, and only the lane whose offer won moves on. Lane j keeps pick j and its lane.
-    int order[kIter];
+    // The slot in the low bits, the lane's in descending order; a round's offer is the lane's first, and only the
+    // lane whose offer won moves on. Lane j keeps pick j and its lane.
 #pragma unroll
-    for (int i = 0; i < kIter; ++i) order[i] = key[i] > kOut ? (ordered(key[i]) & ~kSlots) | i : INT_MIN;
+    for (int i = 0; i < kIter; ++i) order[i] = (order[i] & ~kSlots) | i;
     sort_descending(order);
     int pick = INT_MIN, holder_of = 0;
     for (int j = 0; j <= p.top; ++j) {
       const int best = wave_max(order[0]);
-      if (best == INT_MIN) break;
+      if (best < kLowest) break;
       const int holder = __builtin_ctzll(ballot(order[0] == best));
       pick = lane == j ? best : pick;
       holder_of = lane == j ? holder : holder_of;
@@ -340,15 +343,15 @@ __global__ void __launch_bounds__(kChoiceWaves *kWave) expert_topk_kernel(Choice
     const int next = __shfl_down(pick, 1);
     const float here = unordered(pick), there = unordered(next);
     const float apart = unsure + kUnsureOf * __builtin_fmaxf(__builtin_fabsf(here), __builtin_fabsf(there));
-    sure = ballot(lane < p.top && next != INT_MIN && !(here - there > apart)) == 0;
-    if (pick != INT_MIN) id = (holder_of >> p.lane_bits) * p.size + (holder_of & (lanes - 1)) + (pick & kSlots) * lanes;
+    sure = ballot((lane < p.top) & (next >= kLowest) & !(here - there > apart)) == 0;
+    if (pick >= kLowest) id = (holder_of >> p.lane_bits) * p.size + (holder_of & (lanes - 1)) + (pick & kSlots) * lanes;
   }
 
   // ---- 64 bits: the picked scores, or the whole choice ----
   const auto exact_score = [&](float l) {  // (softmax: times the sum)
     return p.sigmoid ? 1.0 / (1.0 + exp(-static_cast<double>(l))) : exp(static_cast<double>(l) - static_cast<double>(maximum));
   };
-  double sum = 1.0;
+  double sum = 1.0;  // of the softmax, where it is wanted
   if (!p.sigmoid && (!sure || !p.renormalize)) {
     sum = 0.0;
 #pragma unroll
@@ -360,7 +363,8 @@ __global__ void __launch_bounds__(kChoiceWaves *kWave) expert_topk_kernel(Choice
   double picked = 0.0;
   if (lane < p.top && id >= 0) {
     float l = load_logit(p.scores, p.kind, row * p.row_stride + id);
-    picked = exact_score(l < FLT_MAX ? l : FLT_MAX) / sum;
+    picked = exact_score(l < FLT_MAX ? l : FLT_MAX);
+    if (!p.sigmoid) picked /= sum;
   }
   if (p.renormalize) {
     double total = picked;

@@ -142,9 +142,8 @@ def expert_topk(scores, top, scoring="sigmoid", bias=None, groups=1, top_groups=
     stride = _matrix(scores, tokens, experts, index, "expert_topk", "scores")
     if live is not None and (live.numel() != 1 or live.dtype not in (torch.int32, torch.uint32) or live.get_device() != index):
         raise ValueError("expert_topk: live is one int32 on the scores' device")
-    shape, device = (tokens, top if top > 0 else 0), scores.device
-    ids = torch.empty(shape, dtype=torch.int32, device=device)
-    weights = torch.empty(shape, dtype=torch.float32, device=device)
+    ids = torch.empty(tokens, top if top > 0 else 0, dtype=torch.int32, device=scores.device)
+    weights = torch.empty_like(ids, dtype=torch.float32)
     call = ExpertTopkCall(scores.data_ptr(), _vector(bias, experts, (torch.float32,), index, "expert_topk", "bias"),
                           _vector(mapping, experts, (torch.int32,), index, "expert_topk", "mapping"), _ptr(live),
                           _vector(load, experts, (torch.int64,), index, "expert_topk", "load"), ids.data_ptr(),
@@ -168,9 +167,9 @@ def _product(entry, name, x, weight, columns, bias, activation, gate, residual, 
     weight_stride = _matrix(weight, weight.shape[0], width, index, name, "the weight")
     if out is None:
         if out_dtype is None or out_dtype == dtype:
-            out_dtype, out_element, out = dtype, element, x.new_empty((tokens, columns))
+            out_dtype, out_element, out = dtype, element, x.new_empty(tokens, columns)
         elif out_dtype in _ELEMENT:
-            out_element, out = _ELEMENT[out_dtype], x.new_empty((tokens, columns), dtype=out_dtype)
+            out_element, out = _ELEMENT[out_dtype], x.new_empty(tokens, columns, dtype=out_dtype)
         else:
             raise ValueError(f"{name}: the output is the input's type or f32")
         out_stride = columns
