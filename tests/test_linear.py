@@ -207,12 +207,14 @@ def test_gated_linear(device, m, n, k, dtype, activation):
 #: Calls that the choice gives to each kernel: tokens and weight rows of a tile, wavefronts over them, stages
 #: of the ring, teams. K ends inside a stage, short of the ring, and leaves teams without a stage.
 KERNELS = [
-    (False, "256,256,2,4,2,1", 1025, 8200, 520), (True, "256,256,2,4,2,1", 513, 8200, 136),
+    (False, "256,256,2,4,2,1", 4000, 4088, 136), (True, "256,256,2,4,2,1", 700, 8200, 136),
     (False, "128,128,2,2,2,1", 513, 8200, 72), (True, "128,128,2,2,2,1", 257, 8200, 72),
     (False, "128,128,2,4,3,1", 513, 4104, 72), (True, "128,128,2,4,3,1", 200, 4104, 200),
+    (False, "96,128,2,2,4,1", 200, 8200, 520), (True, "96,128,2,2,4,1", 1025, 1000, 520),
     (False, "128,64,2,2,3,1", 400, 8200, 72), (True, "128,64,2,2,3,1", 130, 8200, 72),
     (False, "128,64,4,2,4,1", 200, 4104, 72), (True, "128,64,4,2,4,1", 100, 4104, 72),
     (False, "64,64,2,2,4,1", 5, 8200, 200), (True, "64,64,2,2,4,1", 5, 8200, 72),
+    (False, "48,64,1,2,4,2", 17, 8200, 1032), (True, "48,64,1,2,4,2", 17, 4104, 1032),
     (False, "64,32,1,1,3,4", 33, 4104, 520), (True, "64,32,1,1,3,4", 130, 1000, 520),
     (False, "32,32,1,1,4,4", 5, 40, 72), (True, "32,32,1,1,4,4", 17, 40, 200), (False, "32,32,1,1,4,4", 40, 136, 8),
     (False, "16,16,1,1,4,8", 17, 130, 1032), (False, "16,16,1,1,4,8", 5, 17, 2056),

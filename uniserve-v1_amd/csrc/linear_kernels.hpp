@@ -174,12 +174,14 @@ __global__ void __launch_bounds__(kThreads) few_tokens_kernel(LinearParams p) {
 // ---- the choice -------------------------------------------------------------------------------------------
 
 using Tile256 = TileShape<256, 256, 2, 4, 2>;
-// Two workgroups a CU, or one of eight wavefronts (two a SIMD) with a deeper ring where the tiles are few.
+// Two workgroups a CU, or (Alone) one with a deeper ring, most of eight wavefronts, where the tiles are few.
 using Tile128 = TileShape<128, 128, 2, 2, 2>;
 using Tile128Alone = TileShape<128, 128, 2, 4, 3>;
+using Tile96x128Alone = TileShape<96, 128, 2, 2, 4>;
 using Tile128x64 = TileShape<128, 64, 2, 2, 3>;
 using Tile128x64Alone = TileShape<128, 64, 4, 2, 4>;
 using Tile64 = TileShape<64, 64, 2, 2, 4>;
+using Tile48x64Alone = TileShape<48, 64, 1, 2, 4, 2>;
 // Fewer tiles yet: a team is one wavefront with a ring of its own, and the teams share K out.
 using Tile64x32 = TileShape<64, 32, 1, 1, 3, 4>;
 using Tile32 = TileShape<32, 32, 1, 1, 4, 4>;
@@ -188,8 +190,8 @@ using Tile16 = TileShape<16, 16, 1, 1, 4, 8>;
 /// A shape's time in microseconds, fitted to 460 measured (m, n, k) from 8 x 64 x 256 to 8192 x 2048 x 4096,
 /// plain and gated: `first` for a launch and `stage` for each 64-element stage of K in each round of 256 tiles
 /// (CUs), `round` for each round after the first. Shapes of two workgroups a CU (`pair` > 0) take any
-/// fraction of a round, from `pair` on. The choice by it is within 0.5% of the best shape on average, 20%
-/// at most; without the two Alone shapes 2.8% and 34%.
+/// fraction of a round, from `pair` on. The choice by it is within 1% of the best shape on average, 17% at
+/// most; without the four Alone shapes 3.5% and 36%.
 struct Cost {
   double first, round, stage, pair;
 };
@@ -223,28 +225,32 @@ void launch(const LinearParams &p, hipStream_t stream) {
     return;
   }
   const double costs[] = {
-      cost_of<Tile256>(p, kGated, {9.5, 10.0, 1.1, 0.0}),
-      cost_of<Tile128>(p, kGated, {5.3, 2.4, 0.54, 1.4}),
-      cost_of<Tile128Alone>(p, kGated, {4.8, 4.4, 0.41, 0.0}),
-      cost_of<Tile128x64>(p, kGated, {4.25, 1.9, 0.287, 1.64}),
-      cost_of<Tile128x64Alone>(p, kGated, {4.05, 3.2, 0.265, 0.0}),
-      cost_of<Tile64>(p, kGated, {3.65, 1.4, 0.188, 1.68}),
+      cost_of<Tile256>(p, kGated, {10.3, 11.3, 1.165, 0.0}),
+      cost_of<Tile128>(p, kGated, {5.25, 2.5, 0.535, 1.39}),
+      cost_of<Tile128Alone>(p, kGated, {4.7, 4.65, 0.41, 0.0}),
+      cost_of<Tile96x128Alone>(p, kGated, {5.3, 5.0, 0.341, 0.0}),
+      cost_of<Tile128x64>(p, kGated, {4.2, 1.95, 0.289, 1.65}),
+      cost_of<Tile128x64Alone>(p, kGated, {4.0, 3.3, 0.268, 0.0}),
+      cost_of<Tile64>(p, kGated, {3.65, 1.4, 0.186, 1.68}),
+      cost_of<Tile48x64Alone>(p, kGated, {4.05, 3.0, 0.154, 0.0}),
       cost_of<Tile64x32>(p, kGated, {3.95, 2.7, 0.113, 0.0}),
       cost_of<Tile32>(p, kGated, {3.6, 2.5, 0.077, 0.0}),
       kGated ? 1e30 : cost_of<Tile16>(p, kGated, {4.0, 3.0, 0.034, 0.0}),
   };
   int best = 0;
-  for (int i = 1; i < 9; ++i)
+  for (int i = 1; i < 11; ++i)
     if (costs[i] < costs[best]) best = i;
   switch (best) {
     case 0: return launch_tiles<T, kGated, Tile256>(p, stream);
     case 1: return launch_tiles<T, kGated, Tile128>(p, stream);
     case 2: return launch_tiles<T, kGated, Tile128Alone>(p, stream);
-    case 3: return launch_tiles<T, kGated, Tile128x64>(p, stream);
-    case 4: return launch_tiles<T, kGated, Tile128x64Alone>(p, stream);
-    case 5: return launch_tiles<T, kGated, Tile64>(p, stream);
-    case 6: return launch_tiles<T, kGated, Tile64x32>(p, stream);
-    case 7: return launch_tiles<T, kGated, Tile32>(p, stream);
+    case 3: return launch_tiles<T, kGated, Tile96x128Alone>(p, stream);
+    case 4: return launch_tiles<T, kGated, Tile128x64>(p, stream);
+    case 5: return launch_tiles<T, kGated, Tile128x64Alone>(p, stream);
+    case 6: return launch_tiles<T, kGated, Tile64>(p, stream);
+    case 7: return launch_tiles<T, kGated, Tile48x64Alone>(p, stream);
+    case 8: return launch_tiles<T, kGated, Tile64x32>(p, stream);
+    case 9: return launch_tiles<T, kGated, Tile32>(p, stream);
     default:
       if constexpr (!kGated) return launch_tiles<T, kGated, Tile16>(p, stream);
   }
