@@ -242,6 +242,42 @@ def test_each_tile_kernel(device, gated, shape, m, n, k):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("shape, m, n, k", [
+    ("128,128,2,4,2,1", 2000, 3001, 123), ("128,128,2,4,2,1", 700, 5001, 507), ("64,64,2,2,2,1", 40, 3001, 123),
+    ("64,64,2,2,2,1", 17, 3001, 5), ("32,32,1,1,2,4", 40, 300, 1181), ("32,32,1,1,2,4", 8, 40, 2047),
+])
+def test_each_kernel_for_unaligned_rows(device, gated, shape, m, n, k):
+    announce("linear unaligned kernel", shape, gated, m, n, k)
+    x, w, out = normal((m, k), 1), normal((n * (2 if gated else 1), k), 2, 0.05), normal((m, n), 3)
+
+    def call():
+        return ops.gated_linear(x, w, out=out) if gated else ops.linear(x, w, out=out)
+
+    mangled = "TileShapeI" + "".join(f"Li{d}E" for d in shape.split(","))
+    names = kernels_of(call)
+    assert len(names) == 1 and mangled in names[0], names
+    call()
+    assert_near(out, reference(x, w, None, "silu", gated=True) if gated else reference(x, w))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("k", [1, 2, 3, 5, 7, 9, 15, 17, 31, 57, 63, 65, 127, 129, 191, 255, 257, 511, 515])
+def test_every_remainder_of_unaligned_rows(device, gated, k):
+    """The last elements of rows that end inside 16 bytes, in every kernel through registers; what lies past
+    the rows (NaN here) is neither read into a sum nor needed."""
+    announce("linear remainders", gated, k)
+    for m, n in ((3, 40), (20, 48), (150, 200), (600, 1100)):
+        x = torch.full((m, k + 3), float("nan"), dtype=BF16, device=device)
+        w = torch.full((n * (2 if gated else 1), k + 1), float("nan"), dtype=BF16, device=device)
+        x[:, :k], w[:, :k] = normal((m, k), k), normal((w.shape[0], k), k + 1, 0.05)
+        x, w = x[:, :k], w[:, :k]
+        got = ops.gated_linear(x, w) if gated else ops.linear(x, w)
+        assert_near(got, reference(x, w, None, "silu", gated=True) if gated else reference(x, w), f"{m} x {n}")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("gated", [False, True])
 @pytest.mark.parametrize("k", [8, 56, 64, 72, 128, 192, 256, 264, 512, 576, 2048, 2056])
 def test_short_and_ragged_walks(device, gated, k):
     """Every count of stages around the rings' and the teams', whole and ragged."""

@@ -65,18 +65,29 @@ __device__ __forceinline__ float residual_at(const LinearParams &p, int64_t m, i
   return p.out_f32 ? static_cast<const float *>(p.residual)[at] : T::to_f32(static_cast<const uint16_t *>(p.residual)[at]);
 }
 
-/// Elements at .. at + 7 of a row of `width`, zeros past its end; one 16-byte load at any alignment where
-/// all eight lie in the row.
+/// Elements at .. at + 7 of a row of `width`, zeros past its end, by one 16-byte load at any alignment: where
+/// fewer than eight are left, the row's last eight, moved down.
 __device__ __forceinline__ u32x4 load8(const uint16_t *row, int64_t at, int64_t width) {
-  u32x4 v;
-  if (at + 8 <= width) {
-    __builtin_memcpy(&v, row + at, 16);
-    return v;
+  uint64_t v[2] = {0, 0};
+  if (width >= 8) {
+    const int64_t from = at + 8 <= width ? at : width - 8;
+    __builtin_memcpy(v, row + from, 16);
+    const int past = at - from < 8 ? static_cast<int>(at - from) : 8;  // elements before `at`
+    v[0] = past >= 4 ? v[1] : v[0];
+    v[1] = past >= 4 ? 0 : v[1];
+    const int bits = (past & 3) * 16;
+    v[0] = bits == 0 ? v[0] : (v[0] >> bits) | (v[1] << (64 - bits));
+    v[1] >>= bits;
+    v[0] = past == 8 ? 0 : v[0];
+  } else {
+#pragma unroll 1
+    for (int i = 0; i < 8; ++i) {
+      const uint64_t element = at + i < width ? row[at + i] : 0;
+      v[0] = (v[0] >> 16) | (v[1] << 48);
+      v[1] = (v[1] >> 16) | (element << 48);
+    }
   }
-  uint32_t e[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) e[i] = at + i < width ? row[at + i] : 0u;
-  return u32x4{e[0] | (e[1] << 16), e[2] | (e[3] << 16), e[4] | (e[5] << 16), e[6] | (e[7] << 16)};
+  return __builtin_bit_cast(u32x4, v);
 }
 
 /// The row's factor: sigmoid of its gate logit.

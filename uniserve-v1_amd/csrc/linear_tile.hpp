@@ -64,8 +64,9 @@ __device__ __forceinline__ void tile_of_block(int64_t m_tiles, int64_t n_tiles, 
   n_tile = within / rows;
 }
 
-/// Needs rows as p.by_dma says: whole 16-byte pieces, a tile's rows within 32-bit byte offsets.
-template <class T, bool kGated, class S>
+/// kDma: rows as p.by_dma says, whole 16-byte pieces, a tile's rows within 32-bit byte offsets. Else any rows:
+/// the stages come through registers, by 16-byte loads at any alignment, zeros past the rows' ends.
+template <class T, bool kGated, bool kDma, class S>
 __global__ void __launch_bounds__(S::kThreads) tile_kernel(LinearParams p) {
   using prefill::dma16;
   using prefill::lds_address;
@@ -92,7 +93,9 @@ __global__ void __launch_bounds__(S::kThreads) tile_kernel(LinearParams p) {
   // LDS rows are the wavefronts' in turn, gated: each wavefront's up rows and then its gate rows. Row r
   // keeps its chunk c at c ^ (r / 2) % 8: a lane reads the chunk that its place holds. ----
   const char *base[S::kLoads];
-  uint32_t offset[S::kLoads];
+  uint32_t offset[S::kLoads];           // kDma
+  const uint16_t *row_at[S::kLoads];    // else: the lane's row
+  u32x4 held[S::kLoads];                // and its chunk of the next stage
   const char *x_base = reinterpret_cast<const char *>(p.x + m0 * p.x_stride);
   const char *w_base = reinterpret_cast<const char *>(p.w + n0 * p.w_stride);
   auto chunk_of = [&](int i) { return (lane & 7) ^ ((lane >> 4) & 3) ^ (4 * ((wave + S::kWaves * i) & 1)); };
@@ -113,6 +116,7 @@ __global__ void __launch_bounds__(S::kThreads) tile_kernel(LinearParams p) {
       base[i] = second ? w_base + p.n * p.w_stride * 2 : w_base;
       at = (column < cols_left ? column : cols_left - 1) * p.w_stride;
     }
+    row_at[i] = reinterpret_cast<const uint16_t *>(base[i]) + at;
     base[i] += team * kStageBytes;
     offset[i] = static_cast<uint32_t>(at * 2) + chunk_of(i) * 16;
   }
@@ -122,7 +126,7 @@ __global__ void __launch_bounds__(S::kThreads) tile_kernel(LinearParams p) {
   const int stages = (all_stages + S::kSplit - 1) / S::kSplit;
   const int last_stage = (stages - 1) * S::kSplit + team;
   const int row_chunks = static_cast<int>(p.k / 8);
-  const int last_chunks = last_stage >= all_stages ? 0 : (row_chunks - last_stage * 8 < 8 ? row_chunks - last_stage * 8 : 8);
+  const int last_chunks = !kDma ? 8 : last_stage >= all_stages ? 0 : (row_chunks - last_stage * 8 < 8 ? row_chunks - last_stage * 8 : 8);
   const uint32_t ring_lds = __builtin_amdgcn_readfirstlane(lds_address(&ring[0][wave * 64]));
   int issued = 0;           // stages of the walk issued so far
   uint32_t to = ring_lds;   // where the next one goes
@@ -161,6 +165,22 @@ __global__ void __launch_bounds__(S::kThreads) tile_kernel(LinearParams p) {
     const u32x4 *rows = ring[buffer];
     if (b < NB) wf[half][b] = rows[tile_slot(w_row, half * 4 + g) + b * 128];
     else xf[half][b - NB] = rows[tile_slot(x_row, half * 4 + g) + (b - NB) * 128];
+  };
+  // Through registers: `fetch` loads the walk's next stage, `put` writes the one held to `buffer`.
+  auto fetch = [&]() {
+    const int64_t k = (static_cast<int64_t>(issued) * S::kSplit + team) * kStageK;
+    ++issued;
+    if (k + kStageK <= p.k) {
+#pragma unroll
+      for (int i = 0; i < S::kLoads; ++i) __builtin_memcpy(&held[i], row_at[i] + k + chunk_of(i) * 8, 16);
+    } else {
+#pragma unroll
+      for (int i = 0; i < S::kLoads; ++i) held[i] = load8(row_at[i], k + chunk_of(i) * 8, p.k);
+    }
+  };
+  auto put = [&](int buffer) {
+#pragma unroll
+    for (int i = 0; i < S::kLoads; ++i) ring[buffer][(wave + S::kWaves * i) * 64 + lane] = held[i];
   };
   constexpr int kReadsPer = (NB + MB + NB - 1) / NB;
   constexpr int kIssuesPer = (S::kLoads + NB - 1) / NB;
@@ -207,22 +227,33 @@ __global__ void __launch_bounds__(S::kThreads) tile_kernel(LinearParams p) {
   constexpr std::true_type yes{};
   constexpr std::false_type no{};
 
-  // At most the kStages - 2 stages behind the awaited one are outstanding.
-  constexpr int kBehind = (S::kStages - 2) * S::kLoads;
-  static_assert(kBehind + S::kLoads < 64, "vmcnt holds 6 bits");
-#pragma unroll
-  for (int s = 0; s < S::kStages; ++s) {
-    begin_stage();
-#pragma unroll
-    for (int i = 0; i < S::kLoads; ++i) issue(i);
-    end_stage();
-  }
   // The other wavefronts' loads and reads (a wavefront alone waits for its own).
   auto meet = [&]() {
     if constexpr (S::kWaves > 1) __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
   };
-  prefill::wait_loads_but<kBehind + S::kLoads>();
+  // By DMA at most the kStages - 2 stages behind the awaited one are outstanding.
+  constexpr int kBehind = (S::kStages - 2) * S::kLoads;
+  static_assert(kBehind + S::kLoads < 64, "vmcnt holds 6 bits");
+  constexpr int kWaitLds = 0xc07f;  // lgkmcnt 0, nothing else
+#pragma unroll
+  for (int s = 0; s < S::kStages; ++s) {
+    if constexpr (kDma) {
+      begin_stage();
+#pragma unroll
+      for (int i = 0; i < S::kLoads; ++i) issue(i);
+      end_stage();
+    } else {
+      fetch();
+      put(s);
+    }
+  }
+  if constexpr (kDma) {
+    prefill::wait_loads_but<kBehind + S::kLoads>();
+  } else {
+    fetch();
+    __builtin_amdgcn_s_waitcnt(kWaitLds);
+  }
   meet();
 #pragma unroll
   for (int b = 0; b < NB + MB; ++b) read(0, 0, b);
@@ -230,26 +261,31 @@ __global__ void __launch_bounds__(S::kThreads) tile_kernel(LinearParams p) {
   auto step = [&]() {
     __builtin_amdgcn_sched_barrier(0);
     multiply(first_half, yes, no, buffer);
-    // The stage is in registers, its reads done (lgkmcnt 0), and the next one in LDS.
-    __builtin_amdgcn_s_waitcnt(0x0070 | (kBehind & 15) | ((kBehind >> 4) << 14));
+    // The stage is in registers, its reads done (lgkmcnt 0), and the next one in LDS (DMA: vmcnt; else written
+    // half a stage or more ago).
+    __builtin_amdgcn_s_waitcnt(kDma ? 0x0070 | (kBehind & 15) | ((kBehind >> 4) << 14) : kWaitLds);
     meet();
+    if constexpr (!kDma) {
+      put(buffer);
+      fetch();
+    }
     buffer = buffer + 1 == S::kStages ? 0 : buffer + 1;
   };
   int k = 0;
   for (; k + S::kStages < stages - 1; ++k) {  // the next loads are not the walk's last
     step();
-    multiply(second_half, yes, yes, buffer);
+    multiply(second_half, yes, std::bool_constant<kDma>{}, buffer);
   }
   for (; k < stages - 1; ++k) {
     step();
-    begin_stage();
-    multiply(second_half, yes, yes, buffer);
+    if constexpr (kDma) begin_stage();
+    multiply(second_half, yes, std::bool_constant<kDma>{}, buffer);
   }
   if (last_chunks < 8) mask(first_half);
   multiply(first_half, yes, no, buffer);
   if (last_chunks < 8) mask(second_half);
   multiply(second_half, no, no, 0);
-  prefill::wait_all_loads();
+  if constexpr (kDma) prefill::wait_all_loads();
 
   // ---- the epilogue: each wavefront passes its sums through its own part of the ring (no longer read by
   // anyone), kPassMB token blocks at a time, so that a lane then holds eight consecutive columns of a
@@ -315,9 +351,9 @@ int64_t tiles_of(const LinearParams &p, bool gated) {
   return ceil_div<int64_t>(p.m, S::kBM) * ceil_div<int64_t>(p.n, gated ? S::kBN / 2 : S::kBN);
 }
 
-template <class T, bool kGated, class S>
+template <class T, bool kGated, bool kDma, class S>
 void launch_tiles(const LinearParams &p, hipStream_t stream) {
-  hipLaunchKernelGGL((tile_kernel<T, kGated, S>), dim3(static_cast<uint32_t>(tiles_of<S>(p, kGated))), dim3(S::kThreads), 0,
+  hipLaunchKernelGGL((tile_kernel<T, kGated, kDma, S>), dim3(static_cast<uint32_t>(tiles_of<S>(p, kGated))), dim3(S::kThreads), 0,
                      stream, p);
 }
 
