@@ -244,6 +244,26 @@ def test_choices_closer_than_fp32(device):
 
 
 @pytest.mark.gpu
+def test_group_ranks_past_fp32(device):
+    """Two finite choices may add up past FP32's range; a group's two may cancel to far less than their rounding."""
+    announce("expert_topk group ranks")
+    g = torch.Generator().manual_seed(5)
+    logits = logits_of(64, 16, torch.float32, 7)
+    for sign in (-1.0, 1.0):
+        bias = sign * (1.8e38 + 1.5e38 * torch.rand(16, generator=g))
+        for top_groups in (1, 2):
+            options = dict(groups=4, top_groups=top_groups)
+            got = ops.expert_topk(logits.to(device), 4, bias=bias.to(device), **options)
+            assert_choice(got, reference(logits.numpy(), 4, bias=bias.numpy(), **options), f"{sign} {top_groups}")
+    logits = logits_of(2000, 64, torch.float32, 8)
+    bias = 100.0 + 900.0 * torch.rand(32, generator=g)
+    bias = torch.stack([bias, -bias], 1).reshape(-1)
+    options = dict(groups=32, top_groups=8)
+    got = ops.expert_topk(logits.to(device), 8, bias=bias.to(device), **options)
+    assert_choice(got, reference(logits.numpy(), 8, bias=bias.numpy(), **options), "cancelled")
+
+
+@pytest.mark.gpu
 def test_small_scores_renormalise(device):
     """Sums far below FP32's epsilon, and picks whose scores are all zero (chosen by bias alone)."""
     announce("expert_topk small scores")

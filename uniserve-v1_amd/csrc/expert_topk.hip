@@ -298,9 +298,13 @@ __global__ void __launch_bounds__(kChoiceWaves *kWave) expert_topk_kernel(Choice
 #pragma unroll
     for (int i = 0; i < kIter; ++i) merge_best(best, second, order[i], INT_MIN);
     group_best(best, second, lanes);
-    float rank = best < kLowest ? kOut : unordered(best);
-    if (p.group_top == 2) rank += second < kLowest ? 0.0f : unordered(second);
-    const float size = __builtin_fabsf(rank);
+    // A rank's error goes by its two choices, which may cancel; a sum past the lowest finite float stays above the
+    // rank of a group without candidates, and near every other such sum.
+    const float first_of = best < kLowest ? kOut : unordered(best);
+    const float second_of = p.group_top < 2 || second < kLowest ? 0.0f : unordered(second);
+    float rank = first_of + second_of;
+    rank = best < kLowest || rank >= -FLT_MAX ? rank : -FLT_MAX;
+    const float size = __builtin_fmaxf(__builtin_fabsf(first_of), __builtin_fabsf(second_of));
     const float margin = 2.0f * unsure + 0x1p-20f * wave_max(size < __builtin_inff() ? size : 0.0f);
     // Lane (g, q) compares group g with the groups q, q + P, ..; the ballots hold the P lanes' answers of a group
     // side by side. `near` counts the groups that may lie ahead, its own among them.
