@@ -49,7 +49,7 @@ struct uniserve_expert_topk_call {
   int32_t *ids;          ///< [rows, top]
   float *weights;        ///< [rows, top]
   int64_t row_stride;
-  int64_t rows;
+  int64_t rows;          ///< at most 2^26 - 4, rows * top below 2^31
   int64_t experts;
   int64_t top;
   int64_t groups;        ///< 1: no groups
@@ -62,6 +62,6 @@ struct uniserve_expert_topk_call {
   char error[512];
 };
 
-/// Launches the choice on `stream`: nothing is allocated, no workspace is used and the call may be
+/// Launches the choice on `stream`. No output shares memory with an input or another output. Nothing is allocated, no workspace is used and the call may be
 /// captured. Returns 0, or nonzero with a message in `error`.
 UNISERVE_EXTERN_C int32_t uniserve_expert_topk(const struct uniserve_expert_topk_call *call, void *stream);

@@ -98,6 +98,7 @@ def filled_call():
     ({"top": 0}, "picks"), ({"top": 33}, "picks"), ({"top_groups": 1, "top": 9}, "kept groups"),
     ({"score_dtype": abi.DTYPE["f8e4m3"]}, "f32, bf16 or f16"), ({"scoring": 2}, "softmax or sigmoid"),
     ({"factor": float("nan")}, "finite"), ({"factor": float("inf")}, "finite"),
+    ({"rows": 1 << 26}, "rows in a call"), ({"row_stride": 1 << 60}, "too large"),
     ({"rows": -1}, "int32"), ({"rows": 1 << 29}, "int32"), ({"row_stride": 63}, "row stride"),
     ({"scores": None}, "needs scores"), ({"ids": None}, "needs scores"), ({"weights": None}, "needs scores"),
 ])

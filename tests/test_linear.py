@@ -144,6 +144,15 @@ def test_gated_linear_refusals(fields, says):
     assert says in call.error.decode()
 
 
+@pytest.mark.parametrize("gated, m, n", [(False, 64, (1 << 30) - 1), (False, 1 << 16, 1 << 20), (True, 64, 1 << 29), (True, 1 << 16, 1 << 19)])
+def test_refusals_of_more_tiles_than_a_launch_holds(gated, m, n):
+    call = filled_call(gated)
+    call.m, call.n, call.out_row_stride, call.out, call.weight = m, n, n, 1 << 40, 1 << 50
+    entry = abi.library().uniserve_gated_linear if gated else abi.library().uniserve_linear
+    assert entry(ctypes.byref(call), None) != 0
+    assert "too many tiles" in call.error.decode()
+
+
 def test_no_rows_launch_nothing():
     call = filled_call()
     call.m, call.input, call.out = 0, None, None
@@ -350,6 +359,26 @@ def test_arrays_past_4_gib(device, m):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("m", [1, 4])
+def test_more_columns_than_a_launch_has_wavefronts(device, gated, m):
+    announce("linear columns", gated, m)
+    n, k = (1 << 26) + 5, 8
+    x = normal((m, k), 1)
+    w = torch.empty(((2 if gated else 1) * n, k), dtype=BF16, device=device)
+    for first in range(0, w.shape[0], 1 << 24):
+        part = w[first:first + (1 << 24)]
+        part.copy_(normal(part.shape, first))
+    got = ops.gated_linear(x, w) if gated else ops.linear(x, w)
+    for first in (0, (1 << 25) - 100, n - 200):
+        rows = w[first:first + 200]
+        if gated:
+            rows = torch.cat([rows, w[n + first:n + first + 200]])
+        want = reference(x, rows, None, "silu", gated=True) if gated else reference(x, rows)
+        assert_near(got[:, first:first + 200], want, f"from {first}")
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("m, n, k", [(1, 64, 128), (64, 256, 512), (300, 320, 256)])
 def test_infinities_and_nans_stay_in_their_rows(device, m, n, k):
     """A row's NaN or infinity reaches that row's outputs and no other's; a weight row's its column."""
@@ -364,6 +393,54 @@ def test_infinities_and_nans_stay_in_their_rows(device, m, n, k):
     if rows:
         assert not torch.isfinite(got[rows][:, n - 1]).any()
         assert ((got[rows][:, :n - 1] - want[rows][:, :n - 1]).abs() <= tolerance[rows][:, :n - 1]).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m, n, k", [(2, 40, 72), (20, 72, 200), (90, 136, 328), (600, 264, 136), (70, 40, 75)])
+def test_what_lies_beside_the_rows_is_not_multiplied(device, m, n, k):
+    """Inputs are slices of buffers of NaN: before and behind each row, and rows above and below."""
+    announce("linear beside", m, n, k)
+    x, w = normal((m, k), 1), normal((2 * n, k), 2, 0.05)
+
+    def inside(source):
+        rows, columns = source.shape
+        buffer = torch.full((rows + 300, columns + 72), float("nan"), dtype=BF16, device=device)
+        return buffer[20:20 + rows, 8:8 + columns].copy_(source)
+
+    x_in, w_in = inside(x), inside(w)
+    assert_near(ops.linear(x_in, w_in), reference(x, w))
+    assert_near(ops.gated_linear(x_in, w_in), reference(x, w, None, "silu", gated=True), "gated")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m", [1, 64, 300])
+@pytest.mark.parametrize("dtype, low, high", [(F16, 2.0**-24, 2.0**14), (BF16, 2.0**-133, 2.0**60)])
+def test_subnormal_inputs_count(device, m, dtype, low, high):
+    announce("linear subnormal", m, dtype)
+    x = torch.randint(-100, 101, (m, 128), generator=torch.Generator().manual_seed(1)).double().mul(low).to(dtype).to(device)
+    w = normal((48, 128), 2, high, dtype=dtype) if dtype == BF16 else normal((48, 128), 2, 1.0, dtype=dtype) * high
+    w = w.clamp(-2 * high, 2 * high)
+    assert (x != 0).any()
+    assert_near(ops.linear(x, w, out_dtype=F32), reference(x, w, out_dtype=F32))
+    assert_near(ops.linear(w, x, out_dtype=F32), reference(w, x, out_dtype=F32), "as the weight")
+
+
+@pytest.mark.gpu
+def test_calls_on_two_streams_at_once(device):
+    announce("linear two streams")
+    sides = [torch.cuda.Stream(), torch.cuda.Stream()]
+    inputs = [(normal((m, 1024), m), normal((1536, 1024), m + 1, 0.05)) for m in (700, 40)]
+    want = [(ops.linear(x, w), ops.gated_linear(x, w)) for x, w in inputs]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(4):
+        for i, side in enumerate(sides):
+            with torch.cuda.stream(side):
+                x, w = inputs[i]
+                got[i].append((ops.linear(x, w), ops.gated_linear(x, w)))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(a, b) for pair in got[i] for a, b in zip(pair, want[i]))
 
 
 @pytest.mark.gpu

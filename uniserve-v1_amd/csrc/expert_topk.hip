@@ -413,8 +413,12 @@ extern "C" int32_t uniserve_expert_topk(const uniserve_expert_topk_call *call, v
     if (!std::isfinite(call->factor)) return UNISERVE_REFUSE(call, "expert_topk needs a finite factor");
     if (call->rows < 0 || call->rows > 0x7fffffffLL / call->top)
       return UNISERVE_REFUSE(call, "expert_topk's routes do not fit int32 indexes");
+    constexpr int64_t kMostRows = ((int64_t{1} << 32) / (kChoiceWaves * kWave) - 1) * kChoiceWaves;  // a launch's axis holds
+    if (call->rows > kMostRows) return UNISERVE_REFUSE(call, "expert_topk serves %lld rows in a call", static_cast<long long>(kMostRows));
     if (call->rows > 1 && call->row_stride < call->experts)
       return UNISERVE_REFUSE(call, "expert_topk's row stride is shorter than its rows");
+    if (call->rows > 1 && call->row_stride > (int64_t{1} << 40) / call->rows)
+      return UNISERVE_REFUSE(call, "expert_topk's scores are too large");
     if (call->rows == 0) return 0;
     if (call->scores == nullptr || call->ids == nullptr || call->weights == nullptr)
       return UNISERVE_REFUSE(call, "expert_topk needs scores, ids and weights");

@@ -32,7 +32,7 @@ bool aligned_to(const void *pointer, uintptr_t bytes) { return reinterpret_cast<
 
 /// Extents whose product of rows and stride stays far below 2^63 bytes.
 constexpr int64_t kMostElements = int64_t{1} << 40;
-/// 64 x 64 tiles of 256 threads whose threads an axis of a launch holds.
+/// 64 x 64 tiles of 256 threads whose threads an axis of a launch holds (shapes that need more are not chosen).
 constexpr int64_t kMostTiles = (int64_t{1} << 32) / 256 - 1;
 
 int32_t run(const uniserve_linear_call *call, void *stream, bool gated, const char *name) {
@@ -104,7 +104,7 @@ int32_t run(const uniserve_linear_call *call, void *stream, bool gated, const ch
   p.out_of_8 = out_stride * out_bytes % 16 == 0 && aligned_to(p.out, 16) &&
                (p.residual == nullptr || (residual_stride * out_bytes % 16 == 0 && aligned_to(p.residual, 16)));
   const hipStream_t s = static_cast<hipStream_t>(stream);
-  if (ceil_div<int64_t>(m, 64) * ceil_div<int64_t>(n, 64) > kMostTiles)
+  if (ceil_div<int64_t>(m, 64) * ceil_div<int64_t>(n, gated ? 32 : 64) > kMostTiles)
     return UNISERVE_REFUSE(call, "%s's output has too many tiles", name);
   if (call->dtype == UNISERVE_DTYPE_F16) launch_f16(p, gated, s);
   else launch_bf16(p, gated, s);

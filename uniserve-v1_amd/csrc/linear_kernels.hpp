@@ -137,9 +137,11 @@ template <class T, bool kGated>
 void launch(const LinearParams &p, hipStream_t stream) {
   // Up to four tokens: 1 x 2048 x 5632 6.6 us (the best tile shape 7.3), gated 1 x 5632 x 2048 9.0 (10.2), 4 x
   // 2048 x 5632 8.2 (9.1); with eight tokens 13.2 (9.3).
-  if (p.m == 1) return launch_few<T, kGated, 1>(p, stream);
-  if (p.m == 2) return launch_few<T, kGated, 2>(p, stream);
-  if (p.m <= 4) return launch_few<T, kGated, 4>(p, stream);
+  if (p.m <= 4 && p.n <= (int64_t{1} << 26) - 4) {  // a launch's axis holds fewer than 2^32 threads, a column takes 64
+    if (p.m == 1) return launch_few<T, kGated, 1>(p, stream);
+    if (p.m == 2) return launch_few<T, kGated, 2>(p, stream);
+    return launch_few<T, kGated, 4>(p, stream);
+  }
   if (!p.by_dma) {
     // Fitted as above to 273 sizes with odd k: within 0.5% of the best on average, 13% at most. 8192 x 2048 x 5631:
     // 350 us, where rows of 5632 take 150; 64 x 2048 x 4095: 17.5, and 8.5.
