@@ -245,6 +245,27 @@ def test_choices_closer_than_fp32(device):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("experts", [40, 64, 65, 256, 1000])
+@pytest.mark.parametrize("distinct", [1, 2, 5, 40])
+@pytest.mark.parametrize("options", [dict(), dict(scoring="softmax", renormalize=False), dict(top_groups=2)])
+def test_few_distinct_logits(device, experts, distinct, options):
+    """Ties within the picks, across their end and of more experts than a wavefront has lanes."""
+    if "top_groups" in options:
+        options = dict(options, groups=5 if experts % 5 == 0 else 4)
+    announce("expert_topk few distinct", experts, distinct, options)
+    g = torch.Generator().manual_seed(experts + distinct)
+    values = torch.randn(distinct, generator=g)
+    # Neighbours a few FP32 steps apart, too: the sigmoid's or the softmax's rounding decides in FP32.
+    values[distinct // 2:] = 0.5 + torch.arange(distinct - distinct // 2) * 2.0**-23
+    logits = values[torch.randint(0, distinct, (60, experts), generator=g)]
+    for bias in (None, torch.tensor([0.0, 0.25])[torch.randint(0, 2, (experts,), generator=g)]):
+        for top in (1, 8, 16):
+            got = ops.expert_topk(logits.to(device), top, bias=None if bias is None else bias.to(device), **options)
+            want = reference(logits.numpy(), top, bias=None if bias is None else bias.numpy(), **options)
+            assert_choice(got, want, f"top {top}")
+
+
+@pytest.mark.gpu
 def test_group_ranks_past_fp32(device):
     """Two finite choices may add up past FP32's range; a group's two may cancel to far less than their rounding."""
     announce("expert_topk group ranks")

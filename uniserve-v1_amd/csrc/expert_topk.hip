@@ -10,10 +10,17 @@
 // The choice is defined in 64 bits: two choices a few 1e-9 apart are common among hundreds of experts over
 // thousands of rows, and an FP32 sigmoid plus bias orders such a pair by its rounding. Doubles everywhere
 // cost 22.9 us at 8192 x 256 (8 groups, top 8), most of it in their lane exchanges. So a row is first chosen
-// from in FP32, whose error is bounded, one pick further than asked; where every two neighbouring picks (and
-// the groups at the edge of the kept ones) are further apart than twice that error, the doubles would choose
-// the same, and only the picked scores are evaluated in 64 bits. Other rows (one in a few hundred with FP32
-// logits; exact ties, so every other with bf16 logits and no bias) choose again from doubles.
+// from in FP32, whose error is bounded, until the next pick is further below pick `top` than twice that error:
+// no expert after it can be among the top. The scores of these candidates (mostly `top`) are evaluated in 64
+// bits, which the weights want anyway, and where two neighbours are closer than that the candidates are put in
+// order by them. The whole choice is made again from doubles only where FP32 cannot tell the groups at the
+// edge of the kept ones apart, or more than 64 candidates lie together.
+//
+// Bound by vector instructions, some 570 a row at 256 experts in 8 groups (180 in the picks' rounds, 150 in the
+// doubles); the reads would take 2 us at 8192 rows. 8192 x 256, 8 groups, top 8: f32 logits and a bias 10.4 us,
+// bf16 without one (ties in every other row) 14.4; 64 rows 4.7 and 7.0. With the whole choice from doubles in
+// every row with a close pair: 13.1, 24.2, 4.8 and 10.9 us. Two rows a wavefront, 32 lanes each: 14.6 us at 8192
+// rows (half the wavefronts to hide the rounds' latency), 45 against 56 at 65536.
 #include "common.hpp"
 #include "uniserve_expert_topk.h"
 
@@ -280,7 +287,7 @@ __global__ void __launch_bounds__(kChoiceWaves *kWave) expert_topk_kernel(Choice
     const float scale = 1.0f / wave_sum(sum);
 #pragma unroll
     for (int i = 0; i < kIter; ++i) score[i] *= scale;
-    unsure = 2.0f * (kIter + 12) * 0x1p-24f * scale;
+    unsure = 2.0f * (kIter + 12) * 0x1p-24f * __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(scale)));
   }
   // The lane's choices as ordered integers; no candidate: below kLowest, the lowest finite float, also with a
   // slot in the low bits.
@@ -323,53 +330,88 @@ __global__ void __launch_bounds__(kChoiceWaves *kWave) expert_topk_kernel(Choice
     for (int i = 0; i < kIter; ++i) order[i] = out ? INT_MIN : order[i];
   }
 
+  // Whether two choices of these sizes are ordered in 64 bits as here (an infinite one and its neighbours: no).
+  const auto apart = [&](float here, float there) {
+    return here - there > unsure + kUnsureOf * __builtin_fmaxf(__builtin_fabsf(here), __builtin_fabsf(there));
+  };
   int id = -1;
+  int count = p.top;  // candidates, lane by lane
+  bool ordered_here = false;
   if (sure) {
     // The slot in the low bits, the lane's in descending order; a round's offer is the lane's first, and only the
-    // lane whose offer won moves on. Lane j keeps pick j and its lane.
+    // lane whose offer won moves on. Lane j keeps pick j and its lane. The first pick clearly below pick top - 1
+    // ends the rounds: no other can be among the top.
 #pragma unroll
     for (int i = 0; i < kIter; ++i) order[i] = (order[i] & ~kSlots) | i;
     sort_descending(order);
     int pick = INT_MIN, holder_of = 0;
-    for (int j = 0; j <= p.top; ++j) {
-      const int best = wave_max(order[0]);
-      if (best < kLowest) break;
+    const auto take = [&](int best) {
       const int holder = __builtin_ctzll(ballot(order[0] == best));
-      pick = lane == j ? best : pick;
-      holder_of = lane == j ? holder : holder_of;
+      pick = lane == count ? best : pick;
+      holder_of = lane == count ? holder : holder_of;
       if (lane == holder) {
 #pragma unroll
         for (int i = 0; i + 1 < kIter; ++i) order[i] = order[i + 1];
         order[kIter - 1] = INT_MIN;
       }
+    };
+    int best = wave_max(order[0]), last = best;
+    for (count = 0; count < p.top && best >= kLowest; ++count) {
+      take(best);
+      last = best;
+      best = wave_max(order[0]);
     }
-    // Neighbouring picks, the one past the last among them (an infinite one is never sure).
-    const int next = __shfl_down(pick, 1);
-    const float here = unordered(pick), there = unordered(next);
-    const float apart = unsure + kUnsureOf * __builtin_fmaxf(__builtin_fabsf(here), __builtin_fabsf(there));
-    sure = ballot((lane < p.top) & (next >= kLowest) & !(here - there > apart)) == 0;
+    while (!(sure = best < kLowest || apart(unordered(last), unordered(best))) && count < kWave) {
+      take(best);
+      ++count;
+      best = wave_max(order[0]);
+    }
     if (pick >= kLowest) id = (holder_of >> p.lane_bits) * p.size + (holder_of & (lanes - 1)) + (pick & kSlots) * lanes;
+    const int next = __shfl_down(pick, 1);
+    ordered_here = ballot((lane + 1 < count) & !apart(unordered(pick), unordered(next))) == 0;
   }
 
-  // ---- 64 bits: the picked scores, or the whole choice ----
+  // ---- 64 bits: the candidates' scores and, where FP32 does not tell, their order, or the whole choice ----
   const auto exact_score = [&](float l) {  // (softmax: times the sum)
     return p.sigmoid ? 1.0 / (1.0 + exp(-static_cast<double>(l))) : exp(static_cast<double>(l) - static_cast<double>(maximum));
   };
   double sum = 1.0;  // of the softmax, where it is wanted
-  if (!p.sigmoid && (!sure || !p.renormalize)) {
+  if (!p.sigmoid && (!sure || !ordered_here || !p.renormalize)) {
     sum = 0.0;
 #pragma unroll
     for (int i = 0; i < kIter; ++i)
       if (logit[i] > kOut) sum += exact_score(logit[i]);
     sum = wave_sum(sum);
   }
-  if (!sure) id = choose_exactly<kIter>(p, lane, group, first, lanes, logit, bias, exact_score, sum);
+  if (!sure) {
+    id = choose_exactly<kIter>(p, lane, group, first, lanes, logit, bias, exact_score, sum);
+    count = p.top;
+  }
   double picked = 0.0;
-  if (lane < p.top && id >= 0) {
-    float l = load_logit(p.scores, p.kind, row * p.row_stride + id);
+  if (lane < count && id >= 0) {
+    const float l = load_logit(p.scores, p.kind, row * p.row_stride + id);
     picked = exact_score(l < FLT_MAX ? l : FLT_MAX);
     if (!p.sigmoid) picked /= sum;
   }
+  if (sure && !ordered_here) {
+    // Lane j's place among the candidates (lanes past them keep theirs), where it sends what it holds.
+    const double choice = picked + (p.bias != nullptr && id >= 0 ? static_cast<double>(p.bias[id]) : 0.0);
+    const uint64_t bits = __builtin_bit_cast(uint64_t, choice);
+    int place = lane < count ? 0 : lane;
+    for (int j = 0; j < count; ++j) {
+      const uint32_t low = __builtin_amdgcn_readlane(static_cast<int>(bits), j);
+      const uint32_t high = __builtin_amdgcn_readlane(static_cast<int>(bits >> 32), j);
+      const double other = __builtin_bit_cast(double, static_cast<uint64_t>(high) << 32 | low);
+      const int other_id = __builtin_amdgcn_readlane(id, j);
+      place += lane < count && (other > choice || (other == choice && other_id < id));
+    }
+    const uint64_t held = __builtin_bit_cast(uint64_t, picked);
+    id = __builtin_amdgcn_ds_permute(place * 4, id);
+    const uint32_t low = __builtin_amdgcn_ds_permute(place * 4, static_cast<int>(held));
+    const uint32_t high = __builtin_amdgcn_ds_permute(place * 4, static_cast<int>(held >> 32));
+    picked = __builtin_bit_cast(double, static_cast<uint64_t>(high) << 32 | low);
+  }
+  if (lane >= p.top) picked = 0.0;
   if (p.renormalize) {
     double total = picked;
     for (int offset = 1; offset < p.top; offset *= 2) total += __shfl_xor(total, offset);
