@@ -63,6 +63,36 @@ def test_block(device, tokens):
     assert_bf16_bar(bf16_values(out), expected.numpy(), f"{tokens} tokens")
 
 
+def test_block_captured(device):
+    """The whole block in a graph, replayed with other tokens, against the eager block: the same bits."""
+    announce("MoE block captured")
+    hidden, experts, top, intermediate, shared, tokens = 256, 16, 4, 128, 192, 45
+    p = {
+        "router": normal_bf16((experts, hidden), 1, 0.05), "up_gate": normal_bf16((experts, 2 * intermediate, hidden), 2, 0.02),
+        "down": normal_bf16((experts, hidden, intermediate), 3, 0.02), "shared_up_gate": normal_bf16((2 * shared, hidden), 4, 0.02),
+        "shared_down": normal_bf16((hidden, shared), 5, 0.02), "shared_gate": normal_bf16((1, hidden), 6, 0.02),
+    }
+    options = dict(groups=4, top_groups=2, bias=test_expert_topk.bias_of(experts, 8).to(device))
+    x = normal_bf16((tokens, hidden), 7)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(side):
+        block(x, p, top, options)
+        side.synchronize()
+        with torch.cuda.graph(graph, stream=side):
+            captured = block(x, p, top, options)
+    torch.cuda.current_stream().wait_stream(side)
+    for seed in (8, 9, 10):
+        x.copy_(normal_bf16((tokens, hidden), seed))
+        graph.replay()
+        torch.cuda.synchronize()
+        replayed = [t.clone() for t in captured]
+        for got, want in zip(replayed, block(x, p, top, options)):
+            assert torch.equal(got, want), seed
+        torch.cuda.synchronize()
+
+
 def test_masked_tokens_get_the_shared_expert_alone(device):
     """Padding rows whose logits are all -inf route nowhere: ids -1, weight 0, no routed sum."""
     announce("MoE block masked tokens")
