@@ -77,6 +77,17 @@ __device__ __forceinline__ void tile_of_block(int64_t m_tiles, int64_t n_tiles, 
   n_tile = within / rows;
 }
 
+/// Waits until at most `stages` stages of kLoads loads are outstanding (kMost or more: until kMost are).
+template <int kMost, int kLoads>
+__device__ __forceinline__ void wait_stages_but(int stages) {
+  if constexpr (kMost == 0) {
+    prefill::wait_loads_but<0>();
+  } else {
+    if (stages >= kMost) prefill::wait_loads_but<kMost * kLoads>();
+    else wait_stages_but<kMost - 1, kLoads>(stages);
+  }
+}
+
 /// kDma: rows as p.by_dma says, whole 16-byte pieces, a tile's rows within 32-bit byte offsets. Else any rows:
 /// the stages come through registers, by 16-byte loads at any alignment, zeros past the rows' ends.
 template <class T, bool kGated, bool kDma, class S>
@@ -141,13 +152,10 @@ __global__ void __launch_bounds__(S::kThreads) tile_kernel(LinearParams p) {
   const int row_chunks = static_cast<int>(p.k / 8);
   const int last_chunks = !kDma ? 8 : last_stage >= all_stages ? 0 : (row_chunks - last_stage * 8 < 8 ? row_chunks - last_stage * 8 : 8);
   const uint32_t ring_lds = __builtin_amdgcn_readfirstlane(lds_address(&ring[0][wave * 64]));
-  int issued = 0;           // stages of the walk issued so far
   uint32_t to = ring_lds;   // where the next one goes
-  // The next stage's loads: `begin_stage` (before the walk's last stage and those past it), each load,
-  // `end_stage`. Loads past the last stage read it again,
-  // into buffers nobody reads, so that every wait counts alike.
+  // The next stage's loads: `begin_stage` (before the walk's last stage), each load, `end_stage`.
   auto begin_stage = [&]() {
-    if (issued != stages - 1 || last_chunks == 8) return;
+    if (last_chunks == 8) return;
     // Chunks past the row's end: the row's first chunk of the stage is read instead (multiplied as zeros).
 #pragma unroll
     for (int i = 0; i < S::kLoads; ++i) {
@@ -157,10 +165,8 @@ __global__ void __launch_bounds__(S::kThreads) tile_kernel(LinearParams p) {
   };
   auto issue = [&](int i) { dma16(base[i], offset[i], to + i * S::kWaves * 1024); };
   auto end_stage = [&]() {
-    const int step = issued < stages - 1 ? S::kSplit * kStageBytes : 0;
 #pragma unroll
-    for (int i = 0; i < S::kLoads; ++i) base[i] += step;
-    ++issued;
+    for (int i = 0; i < S::kLoads; ++i) base[i] += S::kSplit * kStageBytes;
     to = to + S::kRows * kStageBytes == ring_lds + S::kLdsBytes ? ring_lds : to + S::kRows * kStageBytes;
   };
 
@@ -179,10 +185,12 @@ __global__ void __launch_bounds__(S::kThreads) tile_kernel(LinearParams p) {
     if (b < NB) wf[half][b] = rows[tile_slot(w_row, half * 4 + g) + b * 128];
     else xf[half][b - NB] = rows[tile_slot(x_row, half * 4 + g) + (b - NB) * 128];
   };
-  // Through registers: `fetch` loads the walk's next stage, `put` writes the one held to `buffer`.
+  // Through registers: `fetch` loads the walk's next stage, if there is one, `put` writes the one held to `buffer`.
+  int fetched = 0;
   auto fetch = [&]() {
-    const int64_t k = (static_cast<int64_t>(issued) * S::kSplit + team) * kStageK;
-    ++issued;
+    if (fetched == stages) return;
+    const int64_t k = (static_cast<int64_t>(fetched) * S::kSplit + team) * kStageK;
+    ++fetched;
     if (k + kStageK <= p.k) {
 #pragma unroll
       for (int i = 0; i < S::kLoads; ++i) __builtin_memcpy(&held[i], row_at[i] + k + chunk_of(i) * 8, 16);
@@ -245,24 +253,26 @@ __global__ void __launch_bounds__(S::kThreads) tile_kernel(LinearParams p) {
     if constexpr (S::kWaves > 1) __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
   };
-  // By DMA at most the kStages - 2 stages behind the awaited one are outstanding.
+  // Awaiting a stage by DMA, at most the kStages - 2 stages behind it are outstanding.
   constexpr int kBehind = (S::kStages - 2) * S::kLoads;
   static_assert(kBehind + S::kLoads < 64, "vmcnt holds 6 bits");
   constexpr int kWaitLds = 0xc07f;  // lgkmcnt 0, nothing else
 #pragma unroll
   for (int s = 0; s < S::kStages; ++s) {
     if constexpr (kDma) {
-      begin_stage();
+      if (s < stages) {
+        if (s == stages - 1) begin_stage();
 #pragma unroll
-      for (int i = 0; i < S::kLoads; ++i) issue(i);
-      end_stage();
+        for (int i = 0; i < S::kLoads; ++i) issue(i);
+        end_stage();
+      }
     } else {
       fetch();
       put(s);
     }
   }
   if constexpr (kDma) {
-    prefill::wait_loads_but<kBehind + S::kLoads>();
+    wait_stages_but<S::kStages - 1, S::kLoads>(stages - 1);
   } else {
     fetch();
     __builtin_amdgcn_s_waitcnt(kWaitLds);
@@ -271,12 +281,13 @@ __global__ void __launch_bounds__(S::kThreads) tile_kernel(LinearParams p) {
 #pragma unroll
   for (int b = 0; b < NB + MB; ++b) read(0, 0, b);
   int buffer = 0;
-  auto step = [&]() {
+  // A stage's first half; then it is in registers, its reads done (lgkmcnt 0), and the next one in LDS (DMA: vmcnt,
+  // `ends` where no loads follow; else written half a stage or more ago).
+  auto step = [&](auto ends, int left) {
     __builtin_amdgcn_sched_barrier(0);
     multiply(first_half, yes, no, buffer);
-    // The stage is in registers, its reads done (lgkmcnt 0), and the next one in LDS (DMA: vmcnt; else written
-    // half a stage or more ago).
-    __builtin_amdgcn_s_waitcnt(kDma ? 0x0070 | (kBehind & 15) | ((kBehind >> 4) << 14) : kWaitLds);
+    if constexpr (kDma && decltype(ends)::value) wait_stages_but<S::kStages - 2, S::kLoads>(left);
+    __builtin_amdgcn_s_waitcnt(kDma && !decltype(ends)::value ? 0x0070 | (kBehind & 15) | ((kBehind >> 4) << 14) : kWaitLds);
     meet();
     if constexpr (!kDma) {
       put(buffer);
@@ -285,20 +296,26 @@ __global__ void __launch_bounds__(S::kThreads) tile_kernel(LinearParams p) {
     buffer = buffer + 1 == S::kStages ? 0 : buffer + 1;
   };
   int k = 0;
-  for (; k + S::kStages < stages - 1; ++k) {  // the next loads are not the walk's last
-    step();
-    multiply(second_half, yes, std::bool_constant<kDma>{}, buffer);
+  if constexpr (kDma) {
+    for (; k + S::kStages < stages - 1; ++k) {  // the next loads are not the walk's last
+      step(no, 0);
+      multiply(second_half, yes, yes, buffer);
+    }
+    if (k + S::kStages == stages - 1) {
+      step(no, 0);
+      begin_stage();
+      multiply(second_half, yes, yes, buffer);
+      ++k;
+    }
   }
   for (; k < stages - 1; ++k) {
-    step();
-    if constexpr (kDma) begin_stage();
-    multiply(second_half, yes, std::bool_constant<kDma>{}, buffer);
+    step(yes, stages - 2 - k);
+    multiply(second_half, yes, no, buffer);
   }
   if (last_chunks < 8) mask(first_half);
   multiply(first_half, yes, no, buffer);
   if (last_chunks < 8) mask(second_half);
   multiply(second_half, no, no, 0);
-  if constexpr (kDma) prefill::wait_all_loads();
 
   // ---- the epilogue: each wavefront passes its sums through its own part of the ring (no longer read by
   // anyone), kPassMB token blocks at a time, so that a lane then holds eight consecutive columns of a
