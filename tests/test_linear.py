@@ -217,16 +217,16 @@ def test_gated_linear(device, m, n, k, dtype, activation):
 #: of the ring, teams. K ends inside a stage, short of the ring, and leaves teams without a stage.
 KERNELS = [
     (False, "256,256,2,4,2,1", 4000, 4088, 136), (True, "256,256,2,4,2,1", 700, 8200, 136),
-    (False, "128,128,2,2,2,1", 513, 8200, 72), (True, "128,128,2,2,2,1", 257, 8200, 72),
-    (False, "128,128,2,4,3,1", 513, 4104, 72), (True, "128,128,2,4,3,1", 200, 4104, 200),
-    (False, "96,128,2,2,4,1", 200, 8200, 520), (True, "96,128,2,2,4,1", 1025, 1000, 520),
-    (False, "128,64,2,2,3,1", 400, 8200, 72), (True, "128,64,2,2,3,1", 130, 8200, 72),
-    (False, "128,64,4,2,4,1", 200, 4104, 72), (True, "128,64,4,2,4,1", 100, 4104, 72),
-    (False, "64,64,2,2,4,1", 5, 8200, 200), (True, "64,64,2,2,4,1", 5, 8200, 72),
-    (False, "48,64,1,2,4,2", 17, 8200, 1032), (True, "48,64,1,2,4,2", 17, 4104, 1032),
-    (False, "64,32,1,1,3,4", 33, 4104, 520), (True, "64,32,1,1,3,4", 130, 1000, 520),
-    (False, "32,32,1,1,4,4", 5, 40, 72), (True, "32,32,1,1,4,4", 17, 40, 200), (False, "32,32,1,1,4,4", 40, 136, 8),
-    (False, "16,16,1,1,4,8", 17, 130, 1032), (False, "16,16,1,1,4,8", 5, 17, 2056),
+    (False, "128,128,2,2,2,1", 513, 8200, 72), (True, "128,128,2,2,2,1", 200, 8200, 72),
+    (False, "128,128,2,4,3,1", 513, 4104, 72), (True, "128,128,2,4,3,1", 257, 4104, 72),
+    (False, "96,128,2,2,4,1", 257, 8200, 520), (True, "96,128,2,2,4,1", 1025, 1000, 520),
+    (False, "128,64,4,2,4,1", 700, 2056, 72), (True, "128,64,4,2,4,1", 700, 1000, 136),
+    (False, "64,64,2,2,4,1", 100, 4104, 72), (True, "64,64,2,2,4,1", 5, 8200, 200),
+    (False, "48,64,1,2,4,2", 33, 8200, 520), (True, "48,64,1,2,4,2", 33, 4104, 520),
+    (False, "32,64,1,1,3,4", 5, 8200, 200), (True, "32,64,1,1,3,4", 5, 4104, 136),
+    (False, "32,32,1,1,4,4", 17, 4104, 72), (True, "32,32,1,1,4,4", 65, 1000, 72),
+    (False, "16,32,1,1,4,4", 17, 2056, 72), (True, "16,32,1,1,4,4", 5, 40, 136), (True, "16,32,1,1,4,4", 40, 136, 2056),
+    (False, "16,16,1,1,4,4", 17, 130, 1032), (False, "16,16,1,1,4,4", 5, 17, 2056), (False, "16,32,1,1,4,4", 40, 136, 8),
 ]
 
 
@@ -247,6 +247,23 @@ def test_each_tile_kernel(device, gated, shape, m, n, k):
     assert len(names) == 1 and mangled in names[0], names
     call()
     assert_near(out, reference(x, w, None, "silu", gated=True) if gated else reference(x, w, gate=gate, residual=residual))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("m", [1, 2])
+@pytest.mark.parametrize("k", [1, 7, 8, 505, 511, 512, 513, 1023, 1024, 1032, 1536, 1541, 2047, 2048, 2049, 3584, 4096, 4600])
+def test_one_and_two_tokens(device, gated, m, k):
+    """Every number of whole and partial chunks behind the walk's full steps."""
+    announce("linear few tokens", gated, m, k)
+    x, w, bias = normal((m, k), 1), normal((2 * 19, k), 2, 0.05), normal((38,), 3)
+    if gated:
+        call, want = (lambda: ops.gated_linear(x, w, bias=bias)), reference(x, w, bias, "silu", gated=True)
+    else:
+        call, want = (lambda: ops.linear(x, w, bias=bias)), reference(x, w, bias)
+    names = kernels_of(call)
+    assert len(names) == 1 and "few_tokens_kernel" in names[0], names
+    assert_near(call(), want)
 
 
 @pytest.mark.gpu
@@ -360,7 +377,7 @@ def test_arrays_past_4_gib(device, m):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("gated", [False, True])
-@pytest.mark.parametrize("m", [1, 4])
+@pytest.mark.parametrize("m", [1, 2, 4])
 def test_more_columns_than_a_launch_has_wavefronts(device, gated, m):
     announce("linear columns", gated, m)
     n, k = (1 << 26) + 5, 8

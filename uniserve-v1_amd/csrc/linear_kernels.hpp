@@ -2,7 +2,7 @@
 //
 // The dense products' kernels of one element type and the choice among them (linear_bf16.hip and
 // linear_f16.hip compile them): tiles (linear_tile.hpp), by DMA or, for rows that it cannot read, through
-// registers, and a kernel for up to four tokens.
+// registers, and a kernel for one or two tokens.
 #pragma once
 
 #include "linear.hpp"
@@ -15,13 +15,13 @@ namespace linear {
 
 constexpr int kFewThreads = 256;
 
-/// Up to kTokens tokens at any strides and alignments: a wavefront reads one weight row (gated: its gate row
+/// kTokens tokens or fewer at any strides and alignments: a wavefront reads one weight row (gated: its gate row
 /// too) in whole kilobytes, eight elements a lane, and its lanes' sums meet at the end. Bound by the weights: 1 x
-/// 2048 x 5632 (23 MB) 6.6 us, gated 1 x 5632 x 2048 (46 MB) 9.0 us, 5.1 TB/s, where a copy reaches 4.8.
+/// 2048 x 5632 (23 MB) 6.3 us, gated 1 x 5632 x 2048 (46 MB) 9.0 us, 5.1 TB/s, where a copy reaches 4.8. (The
+/// last chunks one by one, each after the one before: 7.5 us at K = 5632.)
 template <class T, bool kGated, int kTokens>
 __global__ void __launch_bounds__(kFewThreads) few_tokens_kernel(LinearParams p) {
   constexpr int kRows = kGated ? 2 : 1;
-  constexpr int kUnroll = 4;
   const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / kWave);
   const int lane = lane_id();
   const int64_t n = static_cast<int64_t>(blockIdx.x) * (kFewThreads / kWave) + wave;
@@ -43,35 +43,41 @@ __global__ void __launch_bounds__(kFewThreads) few_tokens_kernel(LinearParams p)
       into = __builtin_fmaf(T::high(x[i]), T::high(w[i]), into);
     }
   };
+  // `count` chunks of a kilobyte a row from `at` on, all their loads first.
   constexpr int64_t kChunk = kWave * 8;
   int64_t at = lane * 8;
-  for (; at - lane * 8 + kUnroll * kChunk <= p.k; at += kUnroll * kChunk) {
-    u32x4 x[kUnroll][kTokens], w[kUnroll][kRows];
+  auto chunks = [&](auto count_of, auto load) {
+    constexpr int kCount = decltype(count_of)::value;
+    u32x4 x[kCount][kTokens], w[kCount][kRows];
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
+    for (int u = 0; u < kCount; ++u) {
 #pragma unroll
-      for (int r = 0; r < kRows; ++r) __builtin_memcpy(&w[u][r], row[r] + at + u * kChunk, 16);
+      for (int r = 0; r < kRows; ++r) w[u][r] = load(row[r], at + u * kChunk);
 #pragma unroll
-      for (int t = 0; t < kTokens; ++t) __builtin_memcpy(&x[u][t], token[t] + at + u * kChunk, 16);
+      for (int t = 0; t < kTokens; ++t) x[u][t] = load(token[t], at + u * kChunk);
     }
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u)
+    for (int u = 0; u < kCount; ++u)
 #pragma unroll
       for (int r = 0; r < kRows; ++r)
 #pragma unroll
         for (int t = 0; t < kTokens; ++t) add(x[u][t], w[u][r], sum[r][t]);
+    at += kCount * kChunk;
+  };
+  const auto inside = [](const uint16_t *from, int64_t i) {
+    u32x4 v;
+    __builtin_memcpy(&v, from + i, 16);
+    return v;
+  };
+  const auto at_end = [&](const uint16_t *from, int64_t i) { return load8(from, i, p.k); };
+  int64_t left = p.k;
+  for (; left >= 4 * kChunk; left -= 4 * kChunk) chunks(std::integral_constant<int, 4>{}, inside);
+  if (left >= 2 * kChunk) {
+    chunks(std::integral_constant<int, 2>{}, inside);
+    left -= 2 * kChunk;
   }
-  for (; at < p.k; at += kChunk) {
-    u32x4 w[kRows];
-#pragma unroll
-    for (int r = 0; r < kRows; ++r) w[r] = load8(row[r], at, p.k);
-#pragma unroll
-    for (int t = 0; t < kTokens; ++t) {
-      const u32x4 x = load8(token[t], at, p.k);
-#pragma unroll
-      for (int r = 0; r < kRows; ++r) add(x, w[r], sum[r][t]);
-    }
-  }
+  if (left > kChunk) chunks(std::integral_constant<int, 2>{}, at_end);
+  else if (left > 0) chunks(std::integral_constant<int, 1>{}, at_end);
 #pragma unroll
   for (int offset = kWave / 2; offset > 0; offset /= 2)
 #pragma unroll
@@ -91,40 +97,46 @@ __global__ void __launch_bounds__(kFewThreads) few_tokens_kernel(LinearParams p)
 // ---- the choice -------------------------------------------------------------------------------------------
 
 using Tile256 = TileShape<256, 256, 2, 4, 2>;
-// Two workgroups a CU, or (Alone) one with a deeper ring, most of eight wavefronts, where the tiles are few.
+// Two workgroups a CU, or (Alone) one with a deeper ring, where the tiles are few.
 using Tile128 = TileShape<128, 128, 2, 2, 2>;
 using Tile128Alone = TileShape<128, 128, 2, 4, 3>;
 using Tile96x128Alone = TileShape<96, 128, 2, 2, 4>;
-using Tile128x64 = TileShape<128, 64, 2, 2, 3>;
 using Tile128x64Alone = TileShape<128, 64, 4, 2, 4>;
 using Tile64 = TileShape<64, 64, 2, 2, 4>;
 using Tile48x64Alone = TileShape<48, 64, 1, 2, 4, 2>;
 // Fewer tiles yet: a team is one wavefront with a ring of its own, and the teams share K out.
-using Tile64x32 = TileShape<64, 32, 1, 1, 3, 4>;
-using Tile32 = TileShape<32, 32, 1, 1, 4, 4>;
-using Tile16 = TileShape<16, 16, 1, 1, 4, 8>;
+using Tile32x64Alone = TileShape<32, 64, 1, 1, 3, 4>;
+using Tile32Alone = TileShape<32, 32, 1, 1, 4, 4>;
+using Tile16x32Alone = TileShape<16, 32, 1, 1, 4, 4>;
+using Tile16 = TileShape<16, 16, 1, 1, 4, 4>;
 
 // Through registers, for rows that the DMA cannot read.
 using Any128 = TileShape<128, 128, 2, 4, 2>;
 using Any64 = TileShape<64, 64, 2, 2, 2>;
 using Any32 = TileShape<32, 32, 1, 1, 2, 4>;
 
-/// A shape's time in microseconds, fitted to 460 measured (m, n, k) from 8 x 64 x 256 to 8192 x 2048 x 4096,
-/// plain and gated: `first` for a launch and `stage` for each 64-element stage of K in each round of 256 tiles
-/// (CUs), `round` for each round after the first. Shapes of two workgroups a CU (`pair` > 0) take any
-/// fraction of a round, from `pair` on. The choice by it is within 1% of the best shape on average, 17% at
-/// most; without the four Alone shapes 3.5% and 36%.
+/// A shape's time in microseconds, fitted to 650 measured (m, n, k) from 5 x 64 x 256 to 8192 x 6144 x 4096, plain
+/// and gated: `first` for a launch, `round` for each round of 256 tiles (CUs) after the first, `stage` for each
+/// 64-element stage of K in each round. Shapes of two workgroups a CU (`shared` > 0) take any fraction of a round
+/// and `shared` a stage and round once CUs are shared, where less than `least` rounds take as long as that many.
+/// The choice by it is within 0.6% of the best shape on average, 19% at most; without one of the shapes up to 2.2%
+/// and 39% (Tile64), without the four that one wavefront a team multiplies 2.6% and 25% more.
 struct Cost {
-  double first, round, stage, pair;
+  double first, round, stage, shared, least;
 };
 
 template <class S>
 double cost_of(const LinearParams &p, bool gated, const Cost &c) {
-  const double tiles = static_cast<double>(tiles_of<S>(p, gated));
-  if (tiles * S::kThreads >= 4294967296.0) return 1e30;  // more threads than a launch's axis holds
-  double rounds = tiles <= 256.0 ? 1.0 : tiles / 256.0;
-  if (tiles > 256.0) rounds = c.pair == 0.0 ? static_cast<double>(ceil_div<int64_t>(tiles_of<S>(p, gated), 256)) : (rounds < c.pair ? c.pair : rounds);
-  return c.first + c.round * (rounds - 1.0) + c.stage * static_cast<double>(ceil_div<int64_t>(p.k, kStageK)) * rounds;
+  const int64_t tiles = tiles_of<S>(p, gated);
+  if (static_cast<double>(tiles) * S::kThreads >= 4294967296.0) return 1e30;  // more threads than a launch's axis holds
+  const double stages = static_cast<double>(ceil_div<int64_t>(p.k, kStageK));
+  if (tiles <= 256) return c.first + c.stage * stages;
+  if (c.shared == 0.0) {
+    const double rounds = static_cast<double>(ceil_div<int64_t>(tiles, 256));
+    return c.first + c.round * (rounds - 1.0) + c.stage * stages * rounds;
+  }
+  const double rounds = static_cast<double>(tiles) / 256.0;
+  return c.first + c.round * (rounds - 1.0) + c.shared * stages * (rounds < c.least ? c.least : rounds);
 }
 
 template <class T, bool kGated, int kTokens>
@@ -136,34 +148,33 @@ void launch_few(const LinearParams &p, hipStream_t stream) {
 
 template <class T, bool kGated>
 void launch(const LinearParams &p, hipStream_t stream) {
-  // Up to four tokens: 1 x 2048 x 5632 6.6 us (the best tile shape 7.3), gated 1 x 5632 x 2048 9.0 (10.2), 4 x
-  // 2048 x 5632 8.2 (9.1); with eight tokens 13.2 (9.3).
-  if (p.m <= 4 && p.n <= (int64_t{1} << 26) - 4) {  // a launch's axis holds fewer than 2^32 threads, a column takes 64
+  // One or two tokens: 1 x 2048 x 5632 6.3 us (the best tile shape 6.8), gated 1 x 5632 x 2048 9.0 (10.1), 2 x 512 x
+  // 2048 3.1 (4.2); four by the same kernel 4 x 2048 x 5632 8.1 (6.9), 4 x 4096 x 2048 6.1 (5.9).
+  if (p.m <= 2 && p.n <= (int64_t{1} << 26) - 4) {  // a launch's axis holds fewer than 2^32 threads, a column takes 64
     if (p.m == 1) return launch_few<T, kGated, 1>(p, stream);
-    if (p.m == 2) return launch_few<T, kGated, 2>(p, stream);
-    return launch_few<T, kGated, 4>(p, stream);
+    return launch_few<T, kGated, 2>(p, stream);
   }
   if (!p.by_dma) {
     // Fitted as above to 273 sizes with odd k: within 0.5% of the best on average, 13% at most. 8192 x 2048 x 5631:
     // 350 us, where rows of 5632 take 150; 64 x 2048 x 4095: 17.5, and 8.5.
-    const double wide = cost_of<Any128>(p, kGated, {8.7, 10.0, 0.76, 0.0}), mid = cost_of<Any64>(p, kGated, {6.1, 2.2, 0.44, 1.68}),
-                 small = cost_of<Any32>(p, kGated, {6.9, 1.8, 0.17, 0.0});
+    const double wide = cost_of<Any128>(p, kGated, {8.7, 10.0, 0.76}), mid = cost_of<Any64>(p, kGated, {6.1, 2.2, 0.44, 0.44, 1.68}),
+                 small = cost_of<Any32>(p, kGated, {6.9, 1.8, 0.17});
     if (wide <= mid && wide <= small) return launch_tiles<T, kGated, false, Any128>(p, stream);
     if (mid <= small) return launch_tiles<T, kGated, false, Any64>(p, stream);
     return launch_tiles<T, kGated, false, Any32>(p, stream);
   }
   const double costs[] = {
-      cost_of<Tile256>(p, kGated, {10.3, 11.3, 1.165, 0.0}),
-      cost_of<Tile128>(p, kGated, {5.25, 2.5, 0.535, 1.39}),
-      cost_of<Tile128Alone>(p, kGated, {4.7, 4.65, 0.41, 0.0}),
-      cost_of<Tile96x128Alone>(p, kGated, {5.3, 5.0, 0.341, 0.0}),
-      cost_of<Tile128x64>(p, kGated, {4.2, 1.95, 0.289, 1.65}),
-      cost_of<Tile128x64Alone>(p, kGated, {4.0, 3.3, 0.268, 0.0}),
-      cost_of<Tile64>(p, kGated, {3.65, 1.4, 0.186, 1.68}),
-      cost_of<Tile48x64Alone>(p, kGated, {4.05, 3.0, 0.154, 0.0}),
-      cost_of<Tile64x32>(p, kGated, {3.95, 2.7, 0.113, 0.0}),
-      cost_of<Tile32>(p, kGated, {3.6, 2.5, 0.077, 0.0}),
-      kGated ? 1e30 : cost_of<Tile16>(p, kGated, {4.0, 3.0, 0.034, 0.0}),
+      cost_of<Tile256>(p, kGated, {9.9, 11.7, 1.211}),
+      cost_of<Tile128>(p, kGated, {4.65, 2.68, 0.603, 0.448, 1.82}),
+      cost_of<Tile128Alone>(p, kGated, {4.76, 4.21, 0.428}),
+      cost_of<Tile96x128Alone>(p, kGated, {5.16, 4.57, 0.344}),
+      cost_of<Tile128x64Alone>(p, kGated, {4.26, 3.24, 0.272}),
+      cost_of<Tile64>(p, kGated, {3.8, 1.16, 0.19, 0.176, 1.8}),
+      cost_of<Tile48x64Alone>(p, kGated, {3.94, 2.6, 0.154}),
+      cost_of<Tile32x64Alone>(p, kGated, {3.66, 2.44, 0.118}),
+      cost_of<Tile32Alone>(p, kGated, {3.46, 2.21, 0.081}),
+      cost_of<Tile16x32Alone>(p, kGated, {3.35, 2.2, 0.059}),
+      kGated ? 1e30 : cost_of<Tile16>(p, kGated, {3.4, 0.85, 0.032, 0.038, 1.91}),
   };
   int best = 0;
   for (int i = 1; i < 11; ++i)
@@ -173,12 +184,12 @@ void launch(const LinearParams &p, hipStream_t stream) {
     case 1: return launch_tiles<T, kGated, true, Tile128>(p, stream);
     case 2: return launch_tiles<T, kGated, true, Tile128Alone>(p, stream);
     case 3: return launch_tiles<T, kGated, true, Tile96x128Alone>(p, stream);
-    case 4: return launch_tiles<T, kGated, true, Tile128x64>(p, stream);
-    case 5: return launch_tiles<T, kGated, true, Tile128x64Alone>(p, stream);
-    case 6: return launch_tiles<T, kGated, true, Tile64>(p, stream);
-    case 7: return launch_tiles<T, kGated, true, Tile48x64Alone>(p, stream);
-    case 8: return launch_tiles<T, kGated, true, Tile64x32>(p, stream);
-    case 9: return launch_tiles<T, kGated, true, Tile32>(p, stream);
+    case 4: return launch_tiles<T, kGated, true, Tile128x64Alone>(p, stream);
+    case 5: return launch_tiles<T, kGated, true, Tile64>(p, stream);
+    case 6: return launch_tiles<T, kGated, true, Tile48x64Alone>(p, stream);
+    case 7: return launch_tiles<T, kGated, true, Tile32x64Alone>(p, stream);
+    case 8: return launch_tiles<T, kGated, true, Tile32Alone>(p, stream);
+    case 9: return launch_tiles<T, kGated, true, Tile16x32Alone>(p, stream);
     default:
       if constexpr (!kGated) return launch_tiles<T, kGated, true, Tile16>(p, stream);
   }
