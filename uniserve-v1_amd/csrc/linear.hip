@@ -101,8 +101,6 @@ int32_t run(const uniserve_linear_call *call, void *stream, bool gated, const ch
   constexpr int64_t kMostStride = int64_t{1} << 22;
   p.by_dma = k % 8 == 0 && x_stride % 8 == 0 && w_stride % 8 == 0 && aligned_to(p.x, 16) && aligned_to(p.w, 16) &&
              x_stride <= kMostStride && w_stride <= kMostStride;
-  p.out_of_8 = out_stride * out_bytes % 16 == 0 && aligned_to(p.out, 16) &&
-               (p.residual == nullptr || (residual_stride * out_bytes % 16 == 0 && aligned_to(p.residual, 16)));
   const hipStream_t s = static_cast<hipStream_t>(stream);
   if (ceil_div<int64_t>(m, 64) * ceil_div<int64_t>(n, gated ? 32 : 64) > kMostTiles)
     return UNISERVE_REFUSE(call, "%s's output has too many tiles", name);

@@ -23,7 +23,6 @@ struct LinearParams {
   int32_t out_f32;
   int32_t activation;
   int32_t by_dma;        ///< input and weight rows suit the tile kernels' loads
-  int32_t out_of_8;      ///< out (and residual) rows start at 16-byte aligned addresses
 };
 
 /// Launches a call that was found servable.
@@ -104,15 +103,28 @@ template <class T, bool kGated>
 struct Columns8 {
   float bias[kGated ? 16 : 8];
   int count;
-  bool vectors;  ///< all eight columns, at 16-byte aligned addresses
+  bool vectors;  ///< all eight columns: 16-byte accesses, at any alignment
 
   __device__ __forceinline__ Columns8(const LinearParams &p, int64_t n) {
     count = p.n - n < 8 ? (p.n > n ? static_cast<int>(p.n - n) : 0) : 8;
-    vectors = p.out_of_8 && count == 8;
+    vectors = count == 8;
+    constexpr int kBiases = kGated ? 16 : 8;
+    // Columns past the last repeat it, so that all loads go out together.
+    int64_t at[kBiases];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      bias[i] = p.bias != nullptr && i < count ? bias_at<T>(p, n + i) : 0.0f;
-      if constexpr (kGated) bias[8 + i] = p.bias != nullptr && i < count ? bias_at<T>(p, p.n + n + i) : 0.0f;
+    for (int i = 0; i < kBiases; ++i) at[i] = (n + i % 8 < p.n ? n + i % 8 : p.n - 1) + (i < 8 ? 0 : p.n);
+    if (p.bias == nullptr) {
+#pragma unroll
+      for (int i = 0; i < kBiases; ++i) bias[i] = 0.0f;
+    } else if (p.bias_f32) {
+#pragma unroll
+      for (int i = 0; i < kBiases; ++i) bias[i] = static_cast<const float *>(p.bias)[at[i]];
+    } else {
+      uint16_t bits[kBiases];
+#pragma unroll
+      for (int i = 0; i < kBiases; ++i) bits[i] = static_cast<const uint16_t *>(p.bias)[at[i]];
+#pragma unroll
+      for (int i = 0; i < kBiases; ++i) bias[i] = T::to_f32(bits[i]);
     }
   }
 
@@ -125,18 +137,33 @@ struct Columns8 {
   template <int kRows>
   __device__ __forceinline__ void load(const LinearParams &p, const int64_t (&m)[kRows], int64_t n, Extras<kRows> &e) const {
     if constexpr (kGated) return;
-    if (p.residual != nullptr && vectors) {
+    if (p.residual != nullptr) {
+      const int64_t last = p.n - 1;  // repeated past the last column, whose lanes read element by element
       if (p.out_f32) {
 #pragma unroll
         for (int i = 0; i < kRows; ++i) {
-          const u32x4 *from = reinterpret_cast<const u32x4 *>(static_cast<const float *>(p.residual) + m[i] * p.residual_stride + n);
-          e.residual[i][0] = from[0];
-          e.residual[i][1] = from[1];
+          const float *from = static_cast<const float *>(p.residual) + m[i] * p.residual_stride;
+          if (vectors) {
+            __builtin_memcpy(&e.residual[i][0], from + n, 16);
+            __builtin_memcpy(&e.residual[i][1], from + n + 4, 16);
+          } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) e.residual[i][j / 4][j % 4] = __float_as_uint(from[n + j < last ? n + j : last]);
+          }
         }
       } else {
 #pragma unroll
-        for (int i = 0; i < kRows; ++i)
-          e.residual[i][0] = *reinterpret_cast<const u32x4 *>(static_cast<const uint16_t *>(p.residual) + m[i] * p.residual_stride + n);
+        for (int i = 0; i < kRows; ++i) {
+          const uint16_t *from = static_cast<const uint16_t *>(p.residual) + m[i] * p.residual_stride;
+          if (vectors) {
+            __builtin_memcpy(&e.residual[i][0], from + n, 16);
+          } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              e.residual[i][0][j] = static_cast<uint32_t>(from[n + 2 * j < last ? n + 2 * j : last]) |
+                                    static_cast<uint32_t>(from[n + 2 * j + 1 < last ? n + 2 * j + 1 : last]) << 16;
+          }
+        }
       }
     }
     if (p.gate != nullptr) {
@@ -164,11 +191,7 @@ struct Columns8 {
         for (int i = 0; i < 8; ++i) v[i] *= factor;
       }
       if (p.residual != nullptr) {
-        if (!vectors) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-            if (i < count) v[i] += residual_at<T>(p, m, n + i);
-        } else if (p.out_f32) {
+        if (p.out_f32) {
 #pragma unroll
           for (int i = 0; i < 8; ++i) v[i] += __uint_as_float(residual[i / 4][i % 4]);
         } else {
@@ -180,8 +203,7 @@ struct Columns8 {
     if (p.out_f32) {
       float *out = static_cast<float *>(p.out) + m * p.out_stride + n;
       if (vectors) {
-        *reinterpret_cast<floatx4 *>(out) = floatx4{v[0], v[1], v[2], v[3]};
-        *reinterpret_cast<floatx4 *>(out + 4) = floatx4{v[4], v[5], v[6], v[7]};
+        __builtin_memcpy(out, v, 32);
       } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i)
@@ -190,8 +212,8 @@ struct Columns8 {
     } else {
       uint16_t *out = static_cast<uint16_t *>(p.out) + m * p.out_stride + n;
       if (vectors) {
-        *reinterpret_cast<u32x4 *>(out) =
-            u32x4{T::pack2(v[0], v[1]), T::pack2(v[2], v[3]), T::pack2(v[4], v[5]), T::pack2(v[6], v[7])};
+        const u32x4 packed{T::pack2(v[0], v[1]), T::pack2(v[2], v[3]), T::pack2(v[4], v[5]), T::pack2(v[6], v[7])};
+        __builtin_memcpy(out, &packed, 16);
       } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i)
