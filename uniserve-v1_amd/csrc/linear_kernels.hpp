@@ -15,7 +15,7 @@ namespace linear {
 
 constexpr int kFewThreads = 256;
 
-/// kTokens tokens or fewer at any strides and alignments: a wavefront reads one weight row (gated: its gate row
+/// kTokens tokens at any strides and alignments: a wavefront reads one weight row (gated: its gate row
 /// too) in whole kilobytes, eight elements a lane, and its lanes' sums meet at the end. Bound by the weights: 1 x
 /// 2048 x 5632 (23 MB) 6.3 us, gated 1 x 5632 x 2048 (46 MB) 9.0 us, 5.1 TB/s, where a copy reaches 4.8. (The
 /// last chunks one by one, each after the one before: 7.5 us at K = 5632.)
@@ -30,7 +30,7 @@ __global__ void __launch_bounds__(kFewThreads) few_tokens_kernel(LinearParams p)
 #pragma unroll
   for (int r = 0; r < kRows; ++r) row[r] = p.w + (n + r * p.n) * p.w_stride;
 #pragma unroll
-  for (int t = 0; t < kTokens; ++t) token[t] = p.x + (t < p.m ? t : p.m - 1) * p.x_stride;
+  for (int t = 0; t < kTokens; ++t) token[t] = p.x + t * p.x_stride;
   float sum[kRows][kTokens];
 #pragma unroll
   for (int r = 0; r < kRows; ++r)
@@ -91,7 +91,7 @@ __global__ void __launch_bounds__(kFewThreads) few_tokens_kernel(LinearParams p)
     v = lane == t ? sum[0][t] : v;
     g = lane == t ? sum[kRows - 1][t] : g;
   }
-  if (lane < kTokens && lane < p.m) finish1<T, kGated>(p, lane, n, v, g);
+  if (lane < kTokens) finish1<T, kGated>(p, lane, n, v, g);
 }
 
 // ---- the choice -------------------------------------------------------------------------------------------
@@ -156,7 +156,7 @@ void launch(const LinearParams &p, hipStream_t stream) {
   }
   if (!p.by_dma) {
     // Fitted as above to 273 sizes with odd k: within 0.5% of the best on average, 13% at most. 8192 x 2048 x 5631:
-    // 350 us, where rows of 5632 take 150; 64 x 2048 x 4095: 17.5, and 8.5.
+    // 313 us, where rows of 5632 take 150; 64 x 2048 x 4095: 14.7, and 7.5.
     const double wide = cost_of<Any128>(p, kGated, {8.7, 10.0, 0.76}), mid = cost_of<Any64>(p, kGated, {6.1, 2.2, 0.44, 0.44, 1.68}),
                  small = cost_of<Any32>(p, kGated, {6.9, 1.8, 0.17});
     if (wide <= mid && wide <= small) return launch_tiles<T, kGated, false, Any128>(p, stream);

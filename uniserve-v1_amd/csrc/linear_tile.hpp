@@ -18,11 +18,11 @@
 // 5632 (150 us, 1.26 PFLOP/s, a single round of tiles whose ends nothing overlaps) and 0.71 in gated 8192 x 5632
 // x 4096 (580 us, 1.30 PFLOP/s); random operands draw the clock down, zeros take 111 us where those take 135 to
 // 150. Of the 111 the barriers cost 10, the operand reads 5, the loads 6 (each taken out of a copy). Tried there
-// without gain: arrival counters in LDS for the barrier, all reads of a half stage at its start, four wavefronts
-// of 128 x 128. Smaller products: what a CU can load, 115 to 135 GB/s from L2 and 60 to 70 from beyond, so the
-// shape with the fewest rows per CU that still gives every CU a tile (gated 200 x 1408 x 4096: 220 tiles of 48 x
-// 64, 0.9 MB each, 14.4 us). By registers and 128-byte rows the loads are no faster, in operand layout (16 rows
-// of 64 bytes) 38 GB/s.
+// without gain: arrival counters in LDS for the barrier, all reads of a half stage at its start, its loads over
+// two halves, 32 x 32 x 16 MFMAs, four wavefronts of 128 x 128. Smaller products: what a CU can load, 115 to 135
+// GB/s from L2 and 60 to 70 from beyond, so the shape with the fewest rows per CU that still gives every CU a tile
+// (gated 200 x 1408 x 4096: 220 tiles of 48 x 64, 0.9 MB each, 14.0 us). By registers and 128-byte rows the loads
+// are no faster, in operand layout (16 rows of 64 bytes) 38 GB/s.
 #pragma once
 
 #include <type_traits>
