@@ -119,8 +119,8 @@ using Any32 = TileShape<32, 32, 1, 1, 2, 4>;
 /// and gated: `first` for a launch, `round` for each round of 256 tiles (CUs) after the first, `stage` for each
 /// 64-element stage of K in each round. Shapes of two workgroups a CU (`shared` > 0) take any fraction of a round
 /// and `shared` a stage and round once CUs are shared, where less than `least` rounds take as long as that many.
-/// The choice by it is within 0.6% of the best shape on average, 19% at most; without one of the shapes up to 2.2%
-/// and 39% (Tile64), without the four that one wavefront a team multiplies 2.6% and 25% more.
+/// The choice by it is within 0.6% of the best shape on average, 19% at most; without one of the shapes up to 2.3%
+/// and 39% (Tile64), with 128 x 64 and 64 x 32 in place of Tile32x64Alone and Tile16x32Alone 2.6% and 25%.
 struct Cost {
   double first, round, stage, shared, least;
 };
