@@ -217,16 +217,19 @@ def test_gated_linear(device, m, n, k, dtype, activation):
 #: of the ring, teams. K ends inside a stage, short of the ring, and leaves teams without a stage.
 KERNELS = [
     (False, "256,256,2,4,2,1", 4000, 4088, 136), (True, "256,256,2,4,2,1", 700, 8200, 136),
-    (False, "128,128,2,2,2,1", 513, 8200, 72), (True, "128,128,2,2,2,1", 200, 8200, 72),
-    (False, "128,128,2,4,3,1", 513, 4104, 72), (True, "128,128,2,4,3,1", 257, 4104, 72),
-    (False, "96,128,2,2,4,1", 257, 8200, 520), (True, "96,128,2,2,4,1", 1025, 1000, 520),
-    (False, "128,64,4,2,4,1", 700, 2056, 72), (True, "128,64,4,2,4,1", 700, 1000, 136),
+    (False, "192,256,2,4,2,1", 1025, 8200, 72), (True, "192,256,2,4,2,1", 400, 8200, 72),
+    (False, "128,256,2,4,3,1", 700, 8200, 72), (True, "128,256,2,4,3,1", 257, 8200, 72),
+    (False, "192,128,4,2,3,1", 400, 8200, 72), (True, "192,128,4,2,3,1", 130, 8200, 136),
+    (False, "128,128,2,2,2,1", 1400, 8200, 72), (True, "128,128,2,2,2,1", 1025, 8200, 72),
+    (False, "128,128,2,4,3,1", 513, 4104, 72), (True, "128,128,2,4,3,1", 200, 4104, 72),
+    (False, "96,128,2,2,4,1", 200, 8200, 520), (True, "96,128,2,2,4,1", 1025, 1000, 520),
+    (False, "128,64,4,2,4,1", 200, 4104, 72), (True, "128,64,4,2,4,1", 100, 4104, 72),
     (False, "64,64,2,2,4,1", 100, 4104, 72), (True, "64,64,2,2,4,1", 5, 8200, 200),
     (False, "48,64,1,2,4,2", 33, 8200, 520), (True, "48,64,1,2,4,2", 33, 4104, 520),
     (False, "32,64,1,1,3,4", 5, 8200, 200), (True, "32,64,1,1,3,4", 5, 4104, 136),
     (False, "32,32,1,1,4,4", 17, 4104, 72), (True, "32,32,1,1,4,4", 65, 1000, 72),
     (False, "16,32,1,1,4,4", 17, 2056, 72), (True, "16,32,1,1,4,4", 5, 40, 136), (True, "16,32,1,1,4,4", 40, 136, 2056),
-    (False, "16,16,1,1,4,4", 17, 130, 1032), (False, "16,16,1,1,4,4", 5, 17, 2056), (False, "16,32,1,1,4,4", 40, 136, 8),
+    (False, "16,16,1,1,4,4", 40, 136, 8), (False, "16,16,1,1,4,4", 17, 130, 1032), (False, "16,16,1,1,4,4", 5, 17, 2056),
 ]
 
 
@@ -269,8 +272,11 @@ def test_one_and_two_tokens(device, gated, m, k):
 @pytest.mark.gpu
 @pytest.mark.parametrize("gated", [False, True])
 @pytest.mark.parametrize("shape, m, n, k", [
-    ("128,128,2,4,2,1", 2000, 3001, 123), ("128,128,2,4,2,1", 700, 5001, 507), ("64,64,2,2,2,1", 40, 3001, 123),
-    ("64,64,2,2,2,1", 17, 3001, 5), ("32,32,1,1,2,4", 40, 300, 1181), ("32,32,1,1,2,4", 8, 40, 2047),
+    ("128,128,2,4,2,1", 1100, 3001, 507), ("128,128,2,4,2,1", 700, 5001, 507),
+    ("96,128,2,2,2,1", 1100, 5001, 123), ("96,128,2,2,2,1", 2000, 3001, 123),
+    ("64,64,2,2,2,1", 65, 5001, 5), ("64,64,2,2,2,1", 130, 3001, 5),
+    ("32,32,1,1,2,4", 17, 5001, 2047), ("32,32,1,1,2,4", 130, 1001, 2047),
+    ("16,32,1,1,2,4", 40, 300, 1181), ("16,32,1,1,2,4", 8, 40, 2047),
 ])
 def test_each_kernel_for_unaligned_rows(device, gated, shape, m, n, k):
     announce("linear unaligned kernel", shape, gated, m, n, k)

@@ -97,6 +97,9 @@ __global__ void __launch_bounds__(kFewThreads) few_tokens_kernel(LinearParams p)
 // ---- the choice -------------------------------------------------------------------------------------------
 
 using Tile256 = TileShape<256, 256, 2, 4, 2>;
+using Tile192x256 = TileShape<192, 256, 2, 4, 2>;
+using Tile128x256 = TileShape<128, 256, 2, 4, 3>;
+using Tile192x128 = TileShape<192, 128, 4, 2, 3>;
 // Two workgroups a CU, or (Alone) one with a deeper ring, where the tiles are few.
 using Tile128 = TileShape<128, 128, 2, 2, 2>;
 using Tile128Alone = TileShape<128, 128, 2, 4, 3>;
@@ -112,15 +115,17 @@ using Tile16 = TileShape<16, 16, 1, 1, 4, 4>;
 
 // Through registers, for rows that the DMA cannot read.
 using Any128 = TileShape<128, 128, 2, 4, 2>;
+using Any96x128 = TileShape<96, 128, 2, 2, 2>;
 using Any64 = TileShape<64, 64, 2, 2, 2>;
 using Any32 = TileShape<32, 32, 1, 1, 2, 4>;
+using Any16x32 = TileShape<16, 32, 1, 1, 2, 4>;
 
-/// A shape's time in microseconds, fitted to 650 measured (m, n, k) from 5 x 64 x 256 to 8192 x 6144 x 4096, plain
+/// A shape's time in microseconds, fitted to 1060 measured (m, n, k) from 3 x 64 x 256 to 8192 x 11264 x 5632, plain
 /// and gated: `first` for a launch, `round` for each round of 256 tiles (CUs) after the first, `stage` for each
-/// 64-element stage of K in each round. Shapes of two workgroups a CU (`shared` > 0) take any fraction of a round
-/// and `shared` a stage and round once CUs are shared, where less than `least` rounds take as long as that many.
-/// The choice by it is within 0.6% of the best shape on average, 19% at most; without one of the shapes up to 2.3%
-/// and 39% (Tile64), with 128 x 64 and 64 x 32 in place of Tile32x64Alone and Tile16x32Alone 2.6% and 25%.
+/// 64-element stage of K in each round. Of shapes of two workgroups a CU (`shared` > 0) 512 tiles take 2 `shared` a
+/// stage; of the tiles past whole 512s up to 256 take `stage`, more `least` times `shared`. The choice by it is
+/// within 0.5% of the best shape on average, 20% at most; without the 192 x 256, 128 x 256 and 192 x 128 tiles 2.8%
+/// and 38%, without one other shape up to 2.1% and 51% (Tile128Alone).
 struct Cost {
   double first, round, stage, shared, least;
 };
@@ -129,14 +134,21 @@ template <class S>
 double cost_of(const LinearParams &p, bool gated, const Cost &c) {
   const int64_t tiles = tiles_of<S>(p, gated);
   if (static_cast<double>(tiles) * S::kThreads >= 4294967296.0) return 1e30;  // more threads than a launch's axis holds
-  const double stages = static_cast<double>(ceil_div<int64_t>(p.k, kStageK));
-  if (tiles <= 256) return c.first + c.stage * stages;
-  if (c.shared == 0.0) {
-    const double rounds = static_cast<double>(ceil_div<int64_t>(tiles, 256));
-    return c.first + c.round * (rounds - 1.0) + c.stage * stages * rounds;
+  const double rounds = static_cast<double>(ceil_div<int64_t>(tiles, 256)), stages = static_cast<double>(ceil_div<int64_t>(p.k, kStageK));
+  double per_stage = c.stage * rounds;
+  if (c.shared > 0.0) {
+    const int64_t rest = tiles % 512;
+    per_stage = 2.0 * c.shared * static_cast<double>(tiles / 512) + (rest == 0 ? 0.0 : rest <= 256 ? c.stage : c.least * c.shared);
   }
-  const double rounds = static_cast<double>(tiles) / 256.0;
-  return c.first + c.round * (rounds - 1.0) + c.shared * stages * (rounds < c.least ? c.least : rounds);
+  return c.first + c.round * (rounds - 1.0) + per_stage * stages;
+}
+
+template <int kShapes>
+int cheapest(const double (&costs)[kShapes]) {
+  int best = 0;
+  for (int i = 1; i < kShapes; ++i)
+    if (costs[i] < costs[best]) best = i;
+  return best;
 }
 
 template <class T, bool kGated, int kTokens>
@@ -155,41 +167,53 @@ void launch(const LinearParams &p, hipStream_t stream) {
     return launch_few<T, kGated, 2>(p, stream);
   }
   if (!p.by_dma) {
-    // Fitted as above to 273 sizes with odd k: within 0.5% of the best on average, 13% at most. 8192 x 2048 x 5631:
-    // 313 us, where rows of 5632 take 150; 64 x 2048 x 4095: 14.7, and 7.5.
-    const double wide = cost_of<Any128>(p, kGated, {8.7, 10.0, 0.76}), mid = cost_of<Any64>(p, kGated, {6.1, 2.2, 0.44, 0.44, 1.68}),
-                 small = cost_of<Any32>(p, kGated, {6.9, 1.8, 0.17});
-    if (wide <= mid && wide <= small) return launch_tiles<T, kGated, false, Any128>(p, stream);
-    if (mid <= small) return launch_tiles<T, kGated, false, Any64>(p, stream);
-    return launch_tiles<T, kGated, false, Any32>(p, stream);
+    // Fitted as above to 415 sizes with odd k: within 1.4% of the best on average, 17% at most; without Any96x128 and
+    // Any16x32 8.6% and 35%. 8192 x 2048 x 5631: 306 us, where rows of 5632 take 150; 64 x 2048 x 4095: 12.2, and 7.5.
+    const double costs[] = {
+        cost_of<Any128>(p, kGated, {6.12, 4.81, 0.727}),
+        cost_of<Any96x128>(p, kGated, {6.95, 1.77, 0.667}),
+        cost_of<Any64>(p, kGated, {4.33, 0.812, 0.473, 0.294, 2.11}),
+        cost_of<Any32>(p, kGated, {4.4, 0.734, 0.173}),
+        cost_of<Any16x32>(p, kGated, {4.09, 0.383, 0.124}),
+    };
+    switch (cheapest(costs)) {
+      case 0: return launch_tiles<T, kGated, false, Any128>(p, stream);
+      case 1: return launch_tiles<T, kGated, false, Any96x128>(p, stream);
+      case 2: return launch_tiles<T, kGated, false, Any64>(p, stream);
+      case 3: return launch_tiles<T, kGated, false, Any32>(p, stream);
+      default: return launch_tiles<T, kGated, false, Any16x32>(p, stream);
+    }
   }
   const double costs[] = {
-      cost_of<Tile256>(p, kGated, {9.9, 11.7, 1.211}),
-      cost_of<Tile128>(p, kGated, {4.65, 2.68, 0.603, 0.448, 1.82}),
-      cost_of<Tile128Alone>(p, kGated, {4.76, 4.21, 0.428}),
-      cost_of<Tile96x128Alone>(p, kGated, {5.16, 4.57, 0.344}),
-      cost_of<Tile128x64Alone>(p, kGated, {4.26, 3.24, 0.272}),
-      cost_of<Tile64>(p, kGated, {3.8, 1.16, 0.19, 0.176, 1.8}),
-      cost_of<Tile48x64Alone>(p, kGated, {3.94, 2.6, 0.154}),
-      cost_of<Tile32x64Alone>(p, kGated, {3.66, 2.44, 0.118}),
-      cost_of<Tile32Alone>(p, kGated, {3.46, 2.21, 0.081}),
-      cost_of<Tile16x32Alone>(p, kGated, {3.35, 2.2, 0.059}),
-      kGated ? 1e30 : cost_of<Tile16>(p, kGated, {3.4, 0.85, 0.032, 0.038, 1.91}),
+      cost_of<Tile256>(p, kGated, {10.3, 9.4, 1.311}),
+      cost_of<Tile192x256>(p, kGated, {7.87, 7.8, 1.045}),
+      cost_of<Tile128x256>(p, kGated, {6.39, 5.74, 0.763}),
+      cost_of<Tile192x128>(p, kGated, {5.21, 4.98, 0.599}),
+      cost_of<Tile128>(p, kGated, {4.46, 2.07, 0.611, 0.436, 1.75}),
+      cost_of<Tile128Alone>(p, kGated, {4.5, 3.91, 0.434}),
+      cost_of<Tile96x128Alone>(p, kGated, {4.87, 3.98, 0.356}),
+      cost_of<Tile128x64Alone>(p, kGated, {4.06, 2.87, 0.28}),
+      cost_of<Tile64>(p, kGated, {3.67, 0.957, 0.184, 0.168, 1.9}),
+      cost_of<Tile48x64Alone>(p, kGated, {3.81, 2.54, 0.151}),
+      cost_of<Tile32x64Alone>(p, kGated, {3.51, 2.44, 0.118}),
+      cost_of<Tile32Alone>(p, kGated, {3.33, 2.17, 0.08}),
+      cost_of<Tile16x32Alone>(p, kGated, {3.22, 2.09, 0.06}),
+      kGated ? 1e30 : cost_of<Tile16>(p, kGated, {3.22, 0.707, 0.034, 0.038, 1.78}),
   };
-  int best = 0;
-  for (int i = 1; i < 11; ++i)
-    if (costs[i] < costs[best]) best = i;
-  switch (best) {
+  switch (cheapest(costs)) {
     case 0: return launch_tiles<T, kGated, true, Tile256>(p, stream);
-    case 1: return launch_tiles<T, kGated, true, Tile128>(p, stream);
-    case 2: return launch_tiles<T, kGated, true, Tile128Alone>(p, stream);
-    case 3: return launch_tiles<T, kGated, true, Tile96x128Alone>(p, stream);
-    case 4: return launch_tiles<T, kGated, true, Tile128x64Alone>(p, stream);
-    case 5: return launch_tiles<T, kGated, true, Tile64>(p, stream);
-    case 6: return launch_tiles<T, kGated, true, Tile48x64Alone>(p, stream);
-    case 7: return launch_tiles<T, kGated, true, Tile32x64Alone>(p, stream);
-    case 8: return launch_tiles<T, kGated, true, Tile32Alone>(p, stream);
-    case 9: return launch_tiles<T, kGated, true, Tile16x32Alone>(p, stream);
+    case 1: return launch_tiles<T, kGated, true, Tile192x256>(p, stream);
+    case 2: return launch_tiles<T, kGated, true, Tile128x256>(p, stream);
+    case 3: return launch_tiles<T, kGated, true, Tile192x128>(p, stream);
+    case 4: return launch_tiles<T, kGated, true, Tile128>(p, stream);
+    case 5: return launch_tiles<T, kGated, true, Tile128Alone>(p, stream);
+    case 6: return launch_tiles<T, kGated, true, Tile96x128Alone>(p, stream);
+    case 7: return launch_tiles<T, kGated, true, Tile128x64Alone>(p, stream);
+    case 8: return launch_tiles<T, kGated, true, Tile64>(p, stream);
+    case 9: return launch_tiles<T, kGated, true, Tile48x64Alone>(p, stream);
+    case 10: return launch_tiles<T, kGated, true, Tile32x64Alone>(p, stream);
+    case 11: return launch_tiles<T, kGated, true, Tile32Alone>(p, stream);
+    case 12: return launch_tiles<T, kGated, true, Tile16x32Alone>(p, stream);
     default:
       if constexpr (!kGated) return launch_tiles<T, kGated, true, Tile16>(p, stream);
   }
