@@ -310,3 +310,27 @@ def test_a_missing_library_fails_loudly(monkeypatch, tmp_path):
         abi.library()
     with pytest.raises(RuntimeError, match="is not built"):
         ops.quantize_mxfp8(torch.zeros((1, 128), dtype=torch.bfloat16))
+
+
+def test_the_operators_import_on_a_torch_without_gpu_support():
+    """Such a torch lacks the calls behind ``torch.cuda``: importing the operators does not need them, and a call of
+    theirs is refused for its host tensors."""
+    import os
+    import subprocess
+    import sys
+
+    lines = ["import torch",
+             "for name in ('_cuda_getCurrentRawStream', '_cuda_getDevice'):",
+             "    if hasattr(torch._C, name):",
+             "        delattr(torch._C, name)",
+             "from uniserve_moe import ops",
+             "for call in (lambda: ops.expert_topk(torch.zeros(2, 8), 2), lambda: ops.linear(*[torch.zeros(2, 8).bfloat16()] * 2)):",
+             "    try:",
+             "        call()",
+             "    except ValueError as error:",
+             "        print(error)"]
+    path = os.pathsep.join([str(ROOT / "uniserve-v1_amd"), *filter(None, [os.environ.get("PYTHONPATH")])])
+    ran = subprocess.run([sys.executable, "-c", "\n".join(lines)], capture_output=True, text=True,
+                         env={**os.environ, "PYTHONPATH": path})
+    assert ran.returncode == 0, ran.stderr
+    assert ran.stdout.count("on a GPU") == 2

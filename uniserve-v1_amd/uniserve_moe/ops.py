@@ -54,9 +54,10 @@ def _stream(device=None):
 
 # The small operators' calls cost the host more than the device, so they take the current stream's handle and the
 # current device's number without the objects that ``torch.cuda`` builds around them (0.1 us each, not 1.9 and 0.25),
-# compare devices by number (-1: the host) and read shapes and strides whole.
-_raw_stream = torch._C._cuda_getCurrentRawStream
-_current_device = torch._C._cuda_getDevice
+# compare devices by number (-1: the host) and read shapes and strides whole. A torch without GPU support lacks both
+# (and has no tensor that a call would reach them with).
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+_current_device = getattr(torch._C, "_cuda_getDevice", None)
 
 
 def _ptr(tensor):
