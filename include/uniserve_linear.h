@@ -15,10 +15,14 @@
 // one gate logit per row, in the inputs' type, gate_stride elements apart; residual [m, n] in the
 // output's type. The output is the inputs' type, or FP32 (uniserve_linear: a router's logits).
 //
-// Any strides, extents and alignments are served; rows of whole 16 bytes at 16-byte aligned addresses
-// take the fast kernels. The output may be the residual itself (same address and stride), in place;
-// an output that overlaps an input in any other way is refused. Nothing is allocated, no workspace is
-// used and the calls may be captured. Results do not depend on what else runs.
+// Any alignment and any k is served. Row strides are no shorter than the rows (the gate's may be 0: one
+// logit for all rows); those of absent arrays and single rows are not read. Refused are m or k of 2^31
+// and more, n of 2^30 and more, an array of more than 2^40 elements from its first row to its last, and
+// an output of more than 2^24 - 1 tiles of 64 x 64 (gated: 64 x 32). The fast kernels take rows of whole
+// 16 bytes (k, base addresses and row strides of the input and the weight) at row strides of up to 2^22
+// elements; other rows go through registers. The output may be the residual itself (same address and
+// stride), in place; an output that overlaps an input in any other way is refused. Nothing is allocated,
+// no workspace is used and the calls may be captured. Results do not depend on what else runs.
 
 #pragma once
 

@@ -144,6 +144,28 @@ def test_gated_linear_refusals(fields, says):
     assert says in call.error.decode()
 
 
+#: Strides of arrays that a call does not have, and of single rows.
+UNUSED = [
+    {"residual_row_stride": 1 << 60}, {"residual_row_stride": -5}, {"gate_stride": 1 << 60}, {"gate_stride": -5},
+    {"m": 1, "input_row_stride": 1 << 60}, {"m": 1, "input_row_stride": 0}, {"m": 1, "out_row_stride": 1 << 60},
+    {"m": 1, "out_row_stride": -1}, {"m": 1, "residual": 8 << 20, "residual_row_stride": 1 << 60},
+    {"m": 1, "gate": 9 << 20, "gate_stride": 1 << 60}, {"n": 1, "weight_row_stride": 1 << 60},
+]
+
+
+@pytest.mark.parametrize("gated, fields", [(False, fields) for fields in UNUSED] +
+                         [(True, fields) for fields in UNUSED if not {"n", "gate", "residual"} & set(fields)])
+def test_unused_strides_are_not_read(gated, fields):
+    """An absent array and a single row have no stride: the call comes to the check after the strides' (the output
+    is the input here)."""
+    call = filled_call(gated)
+    for name, value in {**fields, "out": 1 << 20}.items():
+        setattr(call, name, value)
+    entry = abi.library().uniserve_gated_linear if gated else abi.library().uniserve_linear
+    assert entry(ctypes.byref(call), None) != 0
+    assert "overlaps one of its inputs" in call.error.decode()
+
+
 @pytest.mark.parametrize("gated, m, n", [(False, 64, (1 << 30) - 1), (False, 1 << 16, 1 << 20), (True, 64, 1 << 29), (True, 1 << 16, 1 << 19)])
 def test_refusals_of_more_tiles_than_a_launch_holds(gated, m, n):
     call = filled_call(gated)
@@ -526,6 +548,25 @@ def test_no_rows(device):
     w = normal((32, 64), 1)
     assert ops.linear(torch.empty((0, 64), dtype=BF16, device=device), w).shape == (0, 32)
     assert ops.gated_linear(torch.empty((0, 64), dtype=BF16, device=device), w).shape == (0, 16)
+
+
+@pytest.mark.gpu
+def test_strides_that_a_call_does_not_use(device):
+    """The C entry with anything in the strides of absent arrays and of single rows."""
+    announce("linear unused strides")
+    x, w = normal((1, 256), 1), normal((48, 256), 2, 0.05)
+    gate, residual, out = normal((1, 1), 3), normal((1, 48), 4), torch.empty((1, 48), dtype=BF16, device=device)
+    call = filled_call()
+    call.input, call.weight, call.out = x.data_ptr(), w.data_ptr(), out.data_ptr()
+    call.m, call.n, call.k, call.weight_row_stride = 1, 48, 256, 256
+    call.input_row_stride = call.out_row_stride = call.residual_row_stride = call.gate_stride = 1 << 60
+    assert abi.library().uniserve_linear(ctypes.byref(call), None) == 0, call.error
+    torch.cuda.synchronize()
+    assert_near(out, reference(x, w))
+    call.gate, call.residual = gate.data_ptr(), residual.data_ptr()
+    assert abi.library().uniserve_linear(ctypes.byref(call), None) == 0, call.error
+    torch.cuda.synchronize()
+    assert_near(out, reference(x, w, gate=gate, residual=residual), "one row's gate and residual")
 
 
 @pytest.mark.gpu

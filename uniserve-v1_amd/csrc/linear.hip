@@ -60,16 +60,15 @@ int32_t run(const uniserve_linear_call *call, void *stream, bool gated, const ch
     return UNISERVE_REFUSE(call, "%s's gate stride is negative", name);
   if (m > INT32_MAX || n > INT32_MAX / 2 || k > INT32_MAX)
     return UNISERVE_REFUSE(call, "%s's extents do not fit int32", name);
-  const int64_t strides[] = {call->input_row_stride, call->out_row_stride, call->residual_row_stride, call->gate_stride};
-  for (const int64_t stride : strides)
-    if (stride > kMostElements / m) return UNISERVE_REFUSE(call, "%s's arrays are too large", name);
-  if (call->weight_row_stride > kMostElements / weight_rows) return UNISERVE_REFUSE(call, "%s's arrays are too large", name);
-  // A call of one row has no stride to go by.
+  // A single row has no stride to go by, an absent array neither.
   const int64_t x_stride = m > 1 ? call->input_row_stride : k;
   const int64_t w_stride = weight_rows > 1 ? call->weight_row_stride : k;
   const int64_t out_stride = m > 1 ? call->out_row_stride : n;
-  const int64_t residual_stride = m > 1 ? call->residual_row_stride : n;
-  const int64_t gate_stride = m > 1 ? call->gate_stride : 0;
+  const int64_t residual_stride = m > 1 && call->residual != nullptr ? call->residual_row_stride : n;
+  const int64_t gate_stride = m > 1 && call->gate != nullptr ? call->gate_stride : 0;
+  for (const int64_t stride : {x_stride, out_stride, residual_stride, gate_stride})
+    if (stride > kMostElements / m) return UNISERVE_REFUSE(call, "%s's arrays are too large", name);
+  if (w_stride > kMostElements / weight_rows) return UNISERVE_REFUSE(call, "%s's arrays are too large", name);
   const int64_t out_bytes = call->out_dtype == UNISERVE_DTYPE_F32 ? 4 : 2;
   const int64_t bias_bytes = call->bias_dtype == UNISERVE_DTYPE_F32 ? 4 : 2;
   const auto extent = [](const void *first, int64_t rows, int64_t columns, int64_t stride, int64_t bytes) {
