@@ -403,6 +403,56 @@ def test_arrays_past_4_gib(device, m):
     assert_near(ops.linear(x, w_far), reference(x, w_far), "far weight")
 
 
+#: The DMA kernels' largest row stride, in elements.
+FAR = 1 << 22
+
+
+def spread(source, stride):
+    """The rows `stride` elements apart."""
+    rows, columns = source.shape
+    far = torch.empty((rows - 1) * stride + columns, dtype=source.dtype, device=source.device)
+    return far.as_strided((rows, columns), (stride, 1)).copy_(source)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("stride, by_dma", [(FAR, True), (FAR + 8, False)])
+@pytest.mark.parametrize("far, m, n, k", [
+    ("input", 700, 136, 264), ("input", 700, 8200, 136), ("input", 1025, 8200, 72), ("input", 1100, 40, 136),
+    ("weight", 40, 700, 264), ("weight", 300, 700, 136), ("weight", 3000, 700, 136),
+])
+def test_tiles_past_4_gib(device, gated, stride, by_dma, far, m, n, k):
+    """Tiles of the input and the weight (gated: the gate rows, too) that start past 4 GiB, of up to 256 rows 8 MiB
+    apart, by the kernels of ordinary rows and, one step of the stride further, by those through registers."""
+    announce("linear far tiles", gated, stride, far, m, n, k)
+    x, w = normal((m, k), 1), normal((n * (2 if gated else 1), k), 2, 0.05)
+    x_far, w_far = (spread(x, stride), w) if far == "input" else (x, spread(w, stride))
+    out = torch.empty((m, n), dtype=BF16, device=device)
+
+    def call():
+        return ops.gated_linear(x_far, w_far, out=out) if gated else ops.linear(x_far, w_far, out=out)
+
+    names = kernels_of(call)
+    kernel = f"tile_kernelINS0_4Bf16ELb{int(gated)}ELb{int(by_dma)}E"
+    assert len(names) == 1 and kernel in names[0], names
+    call()
+    assert_near(out, reference(x, w, None, "silu", gated=True) if gated else reference(x, w))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m", [1, 2])
+def test_one_and_two_tokens_past_4_gib(device, m):
+    """Weight rows, and their gate rows, past 4 GiB; a second token's input, residual and output, too."""
+    announce("linear few tokens far", m)
+    n, k = 700, 264
+    x, w, residual = normal((m, k), 1), normal((2 * n, k), 2, 0.05), normal((m, n), 3)
+    w_far, stride = spread(w, FAR), (1 << 31) + 16
+    assert_near(ops.linear(x, w_far), reference(x, w), "far weight")
+    assert_near(ops.gated_linear(x, w_far), reference(x, w, None, "silu", gated=True), "far up and gate rows")
+    x_far, out = spread(x, stride), spread(residual, stride)
+    assert_near(ops.linear(x_far, w[:n], residual=out, out=out), reference(x, w[:n], residual=residual), "far rows")
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("gated", [False, True])
 @pytest.mark.parametrize("m", [1, 2, 4])
