@@ -175,6 +175,49 @@ def test_against_the_definition(device, experts, top, options, tokens, dtype):
     assert_choice(got, want)
 
 
+#: 32 experts a lane (the most that a kernel holds, with their own error bound and slots), and sigmoid groups ranked by
+#: their best expert.
+WIDE = [(1023, 16, dict(groups=3, top_groups=2)), (1017, 8, dict(groups=9, top_groups=4)),
+        (1010, 32, dict(groups=5, top_groups=1, group_top=1)), (1020, 5, dict(groups=17, top_groups=16, factor=2.5))]
+BEST = [(96, 6, dict(groups=8, top_groups=3, group_top=1)), (160, 8, dict(groups=5, top_groups=2, group_top=1)),
+        (60, 4, dict(groups=20, top_groups=7, group_top=1)), (12, 2, dict(groups=12, top_groups=3, group_top=1))]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("scoring", ["sigmoid", "softmax"])
+@pytest.mark.parametrize("experts, top, options", WIDE + BEST)
+def test_wide_groups_and_groups_by_their_best(device, scoring, experts, top, options):
+    announce("expert_topk wide", scoring, experts, top, options)
+    for seed, (dtype, biased, renormalize) in enumerate(((torch.float32, True, True), (torch.float32, False, False),
+                                                         (torch.bfloat16, True, False), (torch.float16, False, True))):
+        bias = bias_of(experts, seed) if biased else None
+        logits = logits_of(60, experts, dtype, experts + seed)
+        got = ops.expert_topk(logits.to(device), top, scoring=scoring, bias=None if bias is None else bias.to(device),
+                              renormalize=renormalize, **options)
+        want = reference(logits.double().numpy(), top, scoring=scoring, bias=None if bias is None else bias.double().numpy(),
+                         renormalize=renormalize, **options)
+        assert_choice(got, want, f"{dtype}, bias {biased}")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("scoring", ["sigmoid", "softmax"])
+@pytest.mark.parametrize("experts, options", [(64, {}), (256, {}), (512, {}), (1024, {}), (256, dict(groups=8, top_groups=3)),
+                                              (1023, dict(groups=3, top_groups=2)), (1017, dict(groups=9, top_groups=4))])
+def test_biases_that_bring_choices_together(device, scoring, experts, options):
+    """Biases that lift experts of unlike scores to one choice, but for the FP32 rounding of the bias: what orders
+    them lies far below an FP32 score's error, of the softmax's sum included. Few experts, and every one."""
+    announce("expert_topk lifted", scoring, experts, options)
+    g = torch.Generator().manual_seed(experts + 1)
+    base = torch.randn(experts, generator=g) * 2.0
+    exact = torch.softmax(base.double(), 0) if scoring == "softmax" else torch.sigmoid(base.double())
+    lifted = (1.0 - exact).float()
+    few = torch.rand(experts, generator=g) < 24 / experts
+    logits = base + torch.randint(-3, 4, (40, experts), generator=g) * 2.0**-22
+    for bias in (torch.where(few, lifted, -1.0), lifted):
+        got = ops.expert_topk(logits.to(device), 8, scoring=scoring, bias=bias.to(device), **options)
+        assert_choice(got, reference(logits.numpy(), 8, scoring=scoring, bias=bias.numpy(), **options))
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("scoring", ["sigmoid", "softmax"])
 @pytest.mark.parametrize("groups", [1, 4])
