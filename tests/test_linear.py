@@ -564,6 +564,23 @@ def test_results_repeat_and_rows_do_not_depend_on_the_batch_s_other_rows(device,
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("m, n, k", [(2, 704, 2048), (5, 40, 136), (33, 4104, 520), (100, 4104, 72), (200, 1408, 4096),
+                                     (777, 1408, 2048), (1100, 264, 515)])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_gated_results_repeat(device, m, n, k, dtype):
+    """Bit for bit, whatever ran before on the same compute units: teams that share K add their sums in one order."""
+    announce("gated_linear repeats", m, n, k, dtype)
+    x, w = normal((m, k), 1, dtype=dtype), normal((2 * n, k), 2, 0.05, dtype)
+    other = normal((1024, 1024), 3)
+    first = ops.gated_linear(x, w)
+    assert_near(first, reference(x, w, None, "silu", gated=True))
+    for _ in range(4):
+        ops.linear(other, other)
+        assert torch.equal(ops.gated_linear(x, w), first)
+        assert torch.equal(ops.gated_linear(x.clone(), w.clone()), first)
+
+
+@pytest.mark.gpu
 def test_captured_replays_and_other_streams(device):
     announce("linear graph")
     x, up_gate, down = normal((48, 256), 1), normal((384, 256), 2, 0.05), normal((256, 192), 3, 0.05)
