@@ -262,11 +262,15 @@ __global__ void __launch_bounds__(kChoiceWaves *kWave) expert_topk_kernel(Choice
 
   // ---- the choice in FP32 ----
   // A sigmoid here is off by less than 2^-22: in steps of 2^-24 the exponent's rounding gives 1.5 |l| s (1 - s)
-  // < 0.34, the exponential 0.5, 1 + e and the reciprocal 3. A softmax's probability is off by less than
-  // kIter + 12 steps of the row's largest: its sum adds kIter + 6 times, the exponent's rounding gives 2.5 x e^-x
-  // < 0.92, the exponential 2, the quotient and the product 2. The bias's addition rounds by half a step of the
-  // choice, and the slot in a key's low bits moves it by 2 kSlots. Two choices further apart than twice all
-  // this are ordered as in 64 bits.
+  // < 0.34, the exponential 0.5, 1 + e and the reciprocal 3. Two of them move against each other by twice that.
+  // Two softmax probabilities of a row move against each other by less than 2 (kIter + 12) steps of the row's
+  // largest. Each by its own errors: x below the maximum the exponent's rounding gives 2.5 x e^-x < 0.92, the
+  // exponential 2, the product 1. And all by one factor, which changes a difference once, not twice: the sum's
+  // kIter + 5 additions and the quotient's 1, the exponentials' 2, and 2.5 times the mean of x under the softmax,
+  // which is largest where all but the maximum lie equally deep: W((N - 1) / e) for N experts (Lambert's W), 2.3 for
+  // 64 and 4.5 for 1024. Together 23 steps of the 26 at kIter = 1, 59 of the 88 at 32. The bias's addition rounds by
+  // half a step of the choice, and the slot in a key's low bits moves it by 2 kSlots. Two choices further apart than
+  // all this are ordered as in 64 bits.
   constexpr int kSlotBits = kIter <= 1 ? 0 : kIter <= 2 ? 1 : kIter <= 4 ? 2 : kIter <= 8 ? 3 : kIter <= 16 ? 4 : 5;
   constexpr int kSlots = (1 << kSlotBits) - 1;
   constexpr float kUnsureOf = (8.0f + 8.0f * kSlots) * 0x1p-24f;  // of a choice's own size
