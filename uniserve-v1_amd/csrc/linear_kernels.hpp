@@ -17,8 +17,9 @@ constexpr int kFewThreads = 256;
 
 /// kTokens tokens at any strides and alignments: a wavefront reads one weight row (gated: its gate row
 /// too) in whole kilobytes, eight elements a lane, and its lanes' sums meet at the end. Bound by the weights: 1 x
-/// 2048 x 5632 (23 MB) 6.3 us, gated 1 x 5632 x 2048 (46 MB) 9.0 us, 5.1 TB/s, where a copy reaches 4.8. (The
-/// last chunks one by one, each after the one before: 7.5 us at K = 5632.)
+/// 2048 x 5632 (23 MB) 6.3 us, gated 1 x 5632 x 2048 (46 MB) 9.0 us, 5.1 TB/s, where a copy reaches 4.8; with weights
+/// that come from HBM 7.2 and 10.1 us, 3.2 and 4.6 TB/s. (The last chunks one by one, each after the one before: 7.5 us
+/// at K = 5632.)
 template <class T, bool kGated, int kTokens>
 __global__ void __launch_bounds__(kFewThreads) few_tokens_kernel(LinearParams p) {
   constexpr int kRows = kGated ? 2 : 1;
@@ -120,12 +121,13 @@ using Any64 = TileShape<64, 64, 2, 2, 2>;
 using Any32 = TileShape<32, 32, 1, 1, 2, 4>;
 using Any16x32 = TileShape<16, 32, 1, 1, 2, 4>;
 
-/// A shape's time in microseconds, fitted to 1060 measured (m, n, k) from 3 x 64 x 256 to 8192 x 11264 x 5632, plain
-/// and gated: `first` for a launch, `round` for each round of 256 tiles (CUs) after the first, `stage` for each
-/// 64-element stage of K in each round. Of shapes of two workgroups a CU (`shared` > 0) 512 tiles take 2 `shared` a
-/// stage; of the tiles past whole 512s up to 256 take `stage`, more `least` times `shared`. The choice by it is
-/// within 0.5% of the best shape on average, 20% at most; without the 192 x 256, 128 x 256 and 192 x 128 tiles 2.8%
-/// and 38%, without one other shape up to 2.1% and 51% (Tile128Alone).
+/// A shape's time in microseconds, fitted to 1056 measured sizes, plain and gated (m from 3 to 8192, n from 64 to
+/// 11264, k from 256 to 5632): `first` for a launch, `round` for each round of 256 tiles (CUs) after the first, `stage`
+/// for each 64-element stage of K in each round. Of shapes of two workgroups a CU (`shared` > 0) 512 tiles take 2
+/// `shared` a stage; of the tiles past whole 512s up to 256 take `stage`, more `least` times `shared`. The choice by it
+/// takes 0.5% longer than the best shape on average, 20% at most. Each shape is chosen at 19 (Tile48x64Alone) to 138
+/// (Tile16x32Alone) of these sizes; the choice without it takes 2% (Tile128x256) to 20% (Tile64) longer there on
+/// average, 14 to 42% at most. Without the 192 x 256, 128 x 256 and 192 x 128 tiles: 2.2% and 35% over all sizes.
 struct Cost {
   double first, round, stage, shared, least;
 };
@@ -167,8 +169,10 @@ void launch(const LinearParams &p, hipStream_t stream) {
     return launch_few<T, kGated, 2>(p, stream);
   }
   if (!p.by_dma) {
-    // Fitted as above to 415 sizes with odd k: within 1.4% of the best on average, 17% at most; without Any96x128 and
-    // Any16x32 8.6% and 35%. 8192 x 2048 x 5631: 306 us, where rows of 5632 take 150; 64 x 2048 x 4095: 12.2, and 7.5.
+    // Fitted as above to 415 sizes with odd k: 0.6% longer than the best on average, 17% at most; without Any96x128
+    // and Any16x32 8.0% and 34%. Each is chosen at 44 to 160 of them, where the choice without it takes 8 to 24% longer.
+    // 8192 x 2048 x 5631: 306 us, where rows of 5632 take 150; 64 x 2048 x 4095: 12.2, and 7.5. How much of that the
+    // loads cost, each over two pieces of a line, and how much the smaller tiles is not known.
     const double costs[] = {
         cost_of<Any128>(p, kGated, {6.12, 4.81, 0.727}),
         cost_of<Any96x128>(p, kGated, {6.95, 1.77, 0.667}),

@@ -19,7 +19,9 @@
 // x 4096 (580 us, 1.30 PFLOP/s); random operands draw the clock down, zeros take 111 us where those take 135 to
 // 150. Of the 111 the barriers cost 10, the operand reads 5, the loads 6 (each taken out of a copy). Tried there
 // without gain: arrival counters in LDS for the barrier, all reads of a half stage at its start, its loads over
-// two halves, 32 x 32 x 16 MFMAs, four wavefronts of 128 x 128. Smaller products: what a CU can load, 115 to 135
+// two halves, 32 x 32 x 16 MFMAs, four wavefronts of 128 x 128. The 256 x 256 kernels use all 256 registers and
+// spill 8 (gated 2): written before the walk and in its last stages, read back there and in the epilogue; the loops
+// over the stages access no scratch. Smaller products: what a CU can load, 115 to 135
 // GB/s from L2 and 60 to 70 from beyond, so the shape with the fewest rows per CU that still gives every CU a tile
 // (gated 200 x 1408 x 4096: 220 tiles of 48 x 64, 0.9 MB each, 14.0 us). By registers and 128-byte rows the loads
 // are no faster, in operand layout (16 rows of 64 bytes) 38 GB/s.
