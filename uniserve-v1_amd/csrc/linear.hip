@@ -2,36 +2,13 @@
 //
 // The dense products on gfx950 (include/uniserve_linear.h states the operators): the entries and their
 // refusals. The kernels and the choice among them are in linear_kernels.hpp.
+#include "extents.hpp"
 #include "linear.hpp"
 
 namespace uniserve {
 namespace linear {
 namespace {
 
-/// `rows` rows of `bytes` bytes, `stride` bytes apart.
-struct Extent {
-  const char *first;
-  int64_t rows, bytes, stride;
-};
-
-/// Whether two arrays share a byte. Rows of equal strides may interleave (two column ranges of one
-/// buffer); of different strides, arrays whose ranges meet count as sharing.
-bool overlap(const Extent &a, const Extent &b) {
-  if (a.first == nullptr || b.first == nullptr || a.rows == 0 || b.rows == 0) return false;
-  const uintptr_t a0 = reinterpret_cast<uintptr_t>(a.first), b0 = reinterpret_cast<uintptr_t>(b.first);
-  const uintptr_t a1 = a0 + static_cast<uintptr_t>((a.rows - 1) * a.stride + a.bytes);
-  const uintptr_t b1 = b0 + static_cast<uintptr_t>((b.rows - 1) * b.stride + b.bytes);
-  if (a1 <= b0 || b1 <= a0) return false;
-  if (a.stride != b.stride || a.rows == 1 || b.rows == 1) return true;
-  const int64_t apart = static_cast<int64_t>(b0 - a0) % a.stride;
-  const int64_t offset = apart < 0 ? apart + a.stride : apart;  // where b's rows start in a's
-  return !(offset >= a.bytes && offset + b.bytes <= a.stride);
-}
-
-bool aligned_to(const void *pointer, uintptr_t bytes) { return reinterpret_cast<uintptr_t>(pointer) % bytes == 0; }
-
-/// Extents whose product of rows and stride stays far below 2^63 bytes.
-constexpr int64_t kMostElements = int64_t{1} << 40;
 /// 64 x 64 tiles of 256 threads whose threads an axis of a launch holds (shapes that need more are not chosen).
 constexpr int64_t kMostTiles = (int64_t{1} << 32) / 256 - 1;
 
@@ -71,9 +48,6 @@ int32_t run(const uniserve_linear_call *call, void *stream, bool gated, const ch
   if (w_stride > kMostElements / weight_rows) return UNISERVE_REFUSE(call, "%s's arrays are too large", name);
   const int64_t out_bytes = call->out_dtype == UNISERVE_DTYPE_F32 ? 4 : 2;
   const int64_t bias_bytes = call->bias_dtype == UNISERVE_DTYPE_F32 ? 4 : 2;
-  const auto extent = [](const void *first, int64_t rows, int64_t columns, int64_t stride, int64_t bytes) {
-    return Extent{static_cast<const char *>(first), rows, columns * bytes, stride * bytes};
-  };
   const Extent out = extent(call->out, m, n, out_stride, out_bytes);
   if (overlap(out, extent(call->input, m, k, x_stride, 2)) || overlap(out, extent(call->weight, weight_rows, k, w_stride, 2)) ||
       overlap(out, extent(call->bias, 1, weight_rows, weight_rows, bias_bytes)) ||

@@ -15,6 +15,8 @@ ACTIVATION = {"silu": 0, "gelu_tanh": 1}
 ENTRY_SUFFIX = {"silu": "", "gelu_tanh": "_gelu_tanh"}
 # The dense products also go without (UNISERVE_ACTIVATION_NONE).
 LINEAR_ACTIVATION = {None: -1, **ACTIVATION}
+# add_norm's norms (uniserve_norm).
+NORM = {"rms": 0, "layer": 1}
 # expert_topk's scores (uniserve_scoring).
 SCORING = {"softmax": 0, "sigmoid": 1}
 
@@ -411,6 +413,39 @@ class LinearCall(ctypes.Structure):
     ]
 
 
+class AddNormCall(ctypes.Structure):
+    """``uniserve_add_norm_call``."""
+
+    _fields_ = [
+        ("input", _P),
+        ("residual", _P),
+        ("post", _P),
+        ("post_bias", _P),
+        ("gate", _P),
+        ("channels", _P),
+        ("weight", _P),
+        ("bias", _P),
+        ("total", _P),
+        ("out", _P),
+        ("rows", _I64),
+        ("width", _I64),
+        ("input_row_stride", _I64),
+        ("residual_row_stride", _I64),
+        ("total_row_stride", _I64),
+        ("out_row_stride", _I64),
+        ("gate_stride", _I64),
+        ("dtype", ctypes.c_int32),
+        ("total_dtype", ctypes.c_int32),
+        ("vector_dtype", ctypes.c_int32),
+        ("norm", ctypes.c_int32),
+        ("eps", ctypes.c_float),
+        ("offset", ctypes.c_float),
+        ("scale", ctypes.c_float),
+        ("residual_scale", ctypes.c_float),
+        ("error", _ERR),
+    ]
+
+
 def max_tiles(tokens, top, local_experts, tile=128):
     """``ops::moe::max_tiles`` (crates/ops/src/moe/mod.rs:63-70)."""
     expanded = tokens * top
@@ -460,6 +495,7 @@ _ENTRIES = {
     "uniserve_expert_topk": ExpertTopkCall,
     "uniserve_linear": LinearCall,
     "uniserve_gated_linear": LinearCall,
+    "uniserve_add_norm": AddNormCall,
 }
 
 

@@ -17,7 +17,9 @@ from .abi import (
     ENTRY_SUFFIX,
     LAYOUT_PERMUTED,
     LINEAR_ACTIVATION,
+    NORM,
     SCORING,
+    AddNormCall,
     ExpertTopkCall,
     GatherCall,
     GatherFp8Call,
@@ -239,6 +241,75 @@ def sigmoid_gated_add_(target, update, gate):
     if status != 0:
         raise RuntimeError(f"sigmoid_gated_add refused the call: {error.value.decode()}")
     return target
+
+
+def add_norm(x, weight, residual=None, post=None, gate=None, channels=None, scale=1.0, residual_scale=1.0, norm="rms",
+             bias=None, post_bias=None, offset=0.0, eps=1e-6, out=None, total=None):
+    """``(out, total)``: ``total = residual_scale * residual + scale * sigmoid(gate) * channels * b`` with ``b`` the
+    rows ``x`` ``[T, H]`` (f32, bf16 or f16) or, with ``post`` ``[H]``, their norm; ``out`` is the norm of ``total``
+    by ``weight`` ``[H]`` (None: the join alone).
+
+    ``norm`` is "rms", ``v / sqrt(mean(v^2) + eps) * (offset + weight)``, or "layer", of ``v`` less its mean and with
+    the biases ``bias`` and ``post_bias``, both of which may be absent. ``gate`` is one logit per row (``[T, 1]``),
+    ``channels`` a factor per column. ``residual`` and ``total`` are of ``x``'s type or f32, ``out`` of ``x``'s; the
+    vectors are all of ``x``'s type or all f32. FP32 within, one rounding into each output. Either output may be
+    given, also as ``x`` or ``residual`` itself, in place. With nothing to join, ``total`` is ``x`` unless it is given."""
+    dtype, index = x.dtype, x.get_device()
+    element = _ELEMENT.get(dtype)
+    if x.dim() != 2 or element is None or index < 0:
+        raise ValueError("add_norm: the rows are [tokens, width] of f32, bf16 or f16 on a GPU")
+    if norm not in NORM:
+        raise ValueError(f"add_norm: norm is rms or layer, got {norm!r}")
+    rows, width = x.shape
+    x_stride = _matrix(x, rows, width, index, "add_norm", "the input")
+    vector = None
+    for v in (weight, post, channels, bias, post_bias):
+        if v is not None:
+            vector = v.dtype if vector is None else vector
+            if v.dtype != vector or (vector != dtype and vector != torch.float32):
+                raise ValueError("add_norm: the vectors are all of the rows' type or all f32")
+    kinds = (vector,)
+    gate_at, gate_stride, residual_at, residual_stride, stream = None, 0, None, 0, dtype
+    if gate is not None:
+        if gate.dtype != dtype:
+            raise ValueError("add_norm: the gate is one logit per row of the rows' type")
+        gate_at, gate_stride = gate.data_ptr(), _matrix(gate, rows, 1, index, "add_norm", "the gate")
+    if residual is not None:
+        stream = residual.dtype
+        residual_at, residual_stride = residual.data_ptr(), _matrix(residual, rows, width, index, "add_norm", "the residual")
+    elif total is not None:
+        stream = total.dtype
+    if stream != dtype and stream != torch.float32:
+        raise ValueError("add_norm: the residual and the total are of the rows' type or f32")
+    returned = total
+    if total is not None:
+        if total.dtype != stream:
+            raise ValueError("add_norm: the total is of the residual's type")
+        total_stride = _matrix(total, rows, width, index, "add_norm", "the total")
+    elif residual is not None or post is not None or gate is not None or channels is not None or scale != 1.0:
+        returned = total = torch.empty(rows, width, dtype=stream, device=x.device)
+        total_stride = width
+    else:
+        returned, total_stride = x, 0
+    if weight is None:
+        if out is not None or bias is not None:
+            raise ValueError("add_norm: without a weight there is no out and no bias")
+        out_stride = 0
+    elif out is None:
+        out, out_stride = torch.empty(rows, width, dtype=dtype, device=x.device), width
+    else:
+        if out.dtype != dtype:
+            raise ValueError("add_norm: the output is of the rows' type")
+        out_stride = _matrix(out, rows, width, index, "add_norm", "the output")
+    call = AddNormCall(x.data_ptr(), residual_at, _vector(post, width, kinds, index, "add_norm", "post"),
+                       _vector(post_bias, width, kinds, index, "add_norm", "post_bias"), gate_at,
+                       _vector(channels, width, kinds, index, "add_norm", "channels"),
+                       _vector(weight, width, kinds, index, "add_norm", "the weight"),
+                       _vector(bias, width, kinds, index, "add_norm", "the bias"), _ptr(total), _ptr(out), rows, width,
+                       x_stride, residual_stride, total_stride, out_stride, gate_stride, element, _ELEMENT[stream],
+                       element if vector is None else _ELEMENT[vector], NORM[norm], eps, offset, scale, residual_scale)
+    _enter(library().uniserve_add_norm, call, index, "add_norm")
+    return out, returned
 
 
 def empty_maps(tokens, top, local_experts, device, fill=-7):
