@@ -27,7 +27,7 @@
 
 #include "uniserve_abi.h"
 
-#define UNISERVE_ADD_NORM_MAX_WIDTH 65536
+#define UNISERVE_ADD_NORM_MAX_WIDTH 32768
 
 enum uniserve_norm
 #ifdef __cplusplus

@@ -97,7 +97,7 @@ def filled_call():
 
 
 REFUSED = [
-    ({"rows": -1}, "positive"), ({"width": 0}, "positive"), ({"width": 65537}, "65536"),
+    ({"rows": -1}, "positive"), ({"width": 0}, "positive"), ({"width": 32769}, "32768"),
     ({"dtype": abi.DTYPE["i32"]}, "bf16, f16 or f32"), ({"total_dtype": abi.DTYPE["f16"]}, "residual and total"),
     ({"vector_dtype": abi.DTYPE["f16"]}, "vectors"), ({"norm": 2}, "rms or layer"),
     ({"bias": 9 << 20}, "no bias"), ({"post_bias": 9 << 20, "norm": 1}, "comes with post"),
@@ -155,7 +155,7 @@ def test_python_refusals():
 # ---- on the MI355X ----------------------------------------------------------------------------------
 
 #: One element to the longest row, with both ends of every shape's widths; rows beyond them by tens and thousands.
-WIDTHS = [1, 7, 8, 9, 64, 100, 511, 512, 513, 1000, 1024, 1031, 2048, 2056, 4095, 4096, 4104, 8192, 8200, 16384, 16392, 65528, 65535]
+WIDTHS = [1, 7, 8, 9, 64, 100, 511, 512, 513, 1000, 1024, 1031, 2048, 2056, 4095, 4096, 4104, 8192, 8200, 16384, 16392, 32760, 32767]
 
 
 def inputs(rows, width, dtype, stream=None, vector=None, seed=0):

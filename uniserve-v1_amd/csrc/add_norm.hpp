@@ -97,8 +97,8 @@ __device__ __forceinline__ float wave_sum(float v) {
 /// kTeam threads to a row, kChunks chunks of eight elements a thread: chunk c of a row is thread c % kTeam's.
 /// kWhole: rows of whole chunks.
 template <class X, class R, int kTeam, int kChunks, bool kWhole>
-__global__ void __launch_bounds__(kTeam < 256 ? 256 : kTeam) add_norm_kernel(AddNormParams p) {
-  constexpr int kTeams = kTeam < 256 ? 256 / kTeam : 1;  // of a workgroup
+__global__ void __launch_bounds__(kTeam < 128 ? 256 : kTeam) add_norm_kernel(AddNormParams p) {
+  constexpr int kTeams = kTeam < 128 ? 256 / kTeam : 1;  // of a workgroup: several are a wavefront each, without barriers
   constexpr int kWaves = kTeam / kWave;
   __shared__ float partial[2][kWaves > 1 ? kWaves : 1];
   const int t = static_cast<int>(threadIdx.x) % kTeam;
@@ -229,7 +229,7 @@ __global__ void __launch_bounds__(kTeam < 256 ? 256 : kTeam) add_norm_kernel(Add
 
 template <class X, class R, int kTeam, int kChunks>
 void launch_shape(const AddNormParams &p, hipStream_t stream) {
-  constexpr int kTeams = kTeam < 256 ? 256 / kTeam : 1;
+  constexpr int kTeams = kTeam < 128 ? 256 / kTeam : 1;
   constexpr int64_t kMostBlocks = int64_t{1} << 20;  // rows past them are the same blocks' next
   const int64_t blocks = ceil_div<int64_t>(p.rows, kTeams);
   const dim3 grid(static_cast<uint32_t>(blocks < kMostBlocks ? blocks : kMostBlocks)), threads(kTeam * kTeams);
@@ -237,20 +237,22 @@ void launch_shape(const AddNormParams &p, hipStream_t stream) {
   else hipLaunchKernelGGL((add_norm_kernel<X, R, kTeam, kChunks, false>), grid, threads, 0, stream, p);
 }
 
+/// One chunk a thread as far as a workgroup's threads go. 8192 x 4096 bf16 (268 MB), plain and with a norm after the
+/// block: 512 threads a row 40.8 and 46.4 us, 256 of two chunks 42.1 and 47.3, 128 of four 50.7 and 60.6, a
+/// wavefront a row 62 and 102 (its registers leave room for one wavefront a SIMD); 64 x 4096: 3.1 and 3.8, 3.5
+/// and 4.4, 4.4 and 5.8, 6.6 and 9.2. Bound by the bytes from some hundred rows on (8192 x 4096 at 6.6 TB/s, partly
+/// from the memory-side cache, where a copy of 4 GiB runs at 4.7), below by the launch and the row's chain of loads
+/// and sums (one row of 2048 2.6 us, 3.2 with both norms).
 template <class X, class R>
 void launch(const AddNormParams &p, hipStream_t stream) {
   const int32_t chunks = ceil_div(p.width, 8);
-  if (chunks <= 512 && p.rows >= 1024) {
-    if (chunks <= 64) return launch_shape<X, R, 64, 1>(p, stream);
-    if (chunks <= 128) return launch_shape<X, R, 64, 2>(p, stream);
-    if (chunks <= 256) return launch_shape<X, R, 64, 4>(p, stream);
-    return launch_shape<X, R, 64, 8>(p, stream);
-  }
+  if (chunks <= 64) return launch_shape<X, R, 64, 1>(p, stream);
+  if (chunks <= 128) return launch_shape<X, R, 128, 1>(p, stream);
   if (chunks <= 256) return launch_shape<X, R, 256, 1>(p, stream);
-  if (chunks <= 512) return launch_shape<X, R, 256, 2>(p, stream);
-  if (chunks <= 1024) return launch_shape<X, R, 256, 4>(p, stream);
-  if (chunks <= 2048) return launch_shape<X, R, 256, 8>(p, stream);
-  return launch_shape<X, R, 1024, 8>(p, stream);
+  if (chunks <= 512) return launch_shape<X, R, 512, 1>(p, stream);
+  if (chunks <= 1024) return launch_shape<X, R, 1024, 1>(p, stream);
+  if (chunks <= 2048) return launch_shape<X, R, 1024, 2>(p, stream);
+  return launch_shape<X, R, 1024, 4>(p, stream);
 }
 
 }  // namespace add_norm
