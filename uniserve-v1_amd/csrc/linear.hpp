@@ -25,9 +25,36 @@ struct LinearParams {
   int32_t by_dma;        ///< input and weight rows suit the tile kernels' loads
 };
 
+/// Where a row's rank values lie between the adapters' two products, group by group of at most 32 ranks (gated: the
+/// up half's groups, then the gate half's): `width` elements that hold the values rounded, as many their errors, and
+/// the group's factor (FP32, f16 only: the power of two that both were divided by), padded to 16 bytes.
+struct LowLayout {
+  int32_t width;   ///< ranks of a group: 8, 16 or 32
+  int32_t groups;  ///< of a half
+  __host__ __device__ explicit LowLayout(int64_t rank)
+      : width(rank <= 8 ? 8 : rank <= 16 ? 16 : 32), groups(static_cast<int32_t>((rank + width - 1) / width)) {}
+  __host__ __device__ int32_t group_bytes() const { return 4 * width + 16; }
+  __host__ __device__ int64_t row_bytes(int halves) const { return static_cast<int64_t>(halves) * groups * group_bytes(); }
+};
+
+/// A product whose rows have low-rank adapters.
+struct AdapterParams : LinearParams {
+  const uint16_t *down;    ///< [adapters, rank, k]; gated: [adapters, 2 rank, k]
+  const uint16_t *up;      ///< [adapters, n, rank]; gated: [adapters, 2 n, rank]
+  const int32_t *adapter;  ///< [m]
+  const float *scales;     ///< [adapters], or null
+  char *low;               ///< the workspace: each row's rank values
+  int64_t down_stride, down_row_stride, up_stride, up_row_stride;
+  int32_t adapters, rank;
+  int32_t down_whole;  ///< input and down rows are whole 16-byte pieces
+  int32_t up_whole;    ///< up rows are
+};
+
 /// Launches a call that was found servable.
 void launch_bf16(const LinearParams &p, bool gated, hipStream_t stream);
 void launch_f16(const LinearParams &p, bool gated, hipStream_t stream);
+void launch_adapters_bf16(const AdapterParams &p, bool gated, hipStream_t stream);
+void launch_adapters_f16(const AdapterParams &p, bool gated, hipStream_t stream);
 
 struct Bf16 {
   static __device__ __forceinline__ float low(uint32_t pair) { return __uint_as_float(pair << 16); }

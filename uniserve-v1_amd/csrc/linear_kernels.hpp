@@ -20,8 +20,8 @@ constexpr int kFewThreads = 256;
 /// 2048 x 5632 (23 MB) 6.3 us, gated 1 x 5632 x 2048 (46 MB) 9.0 us, 5.1 TB/s, where a copy reaches 4.8; with weights
 /// that come from HBM 7.2 and 10.1 us, 3.2 and 4.6 TB/s. (The last chunks one by one, each after the one before: 7.5 us
 /// at K = 5632.)
-template <class T, bool kGated, int kTokens>
-__global__ void __launch_bounds__(kFewThreads) few_tokens_kernel(LinearParams p) {
+template <class T, bool kGated, int kTokens, class P>
+__global__ void __launch_bounds__(kFewThreads) few_tokens_kernel(P p) {
   constexpr int kRows = kGated ? 2 : 1;
   const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / kWave);
   const int lane = lane_id();
@@ -37,6 +37,7 @@ __global__ void __launch_bounds__(kFewThreads) few_tokens_kernel(LinearParams p)
   for (int r = 0; r < kRows; ++r)
 #pragma unroll
     for (int t = 0; t < kTokens; ++t) sum[r][t] = 0.0f;
+  if constexpr (std::is_same<P, AdapterParams>::value) start_low_rank<T>(p, n, sum);
   auto add = [&](const u32x4 &x, const u32x4 &w, float &into) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -153,15 +154,15 @@ int cheapest(const double (&costs)[kShapes]) {
   return best;
 }
 
-template <class T, bool kGated, int kTokens>
-void launch_few(const LinearParams &p, hipStream_t stream) {
+template <class T, bool kGated, int kTokens, class P>
+void launch_few(const P &p, hipStream_t stream) {
   constexpr int kWaves = kFewThreads / kWave;
-  hipLaunchKernelGGL((few_tokens_kernel<T, kGated, kTokens>), dim3(static_cast<uint32_t>(ceil_div<int64_t>(p.n, kWaves))),
+  hipLaunchKernelGGL((few_tokens_kernel<T, kGated, kTokens, P>), dim3(static_cast<uint32_t>(ceil_div<int64_t>(p.n, kWaves))),
                      dim3(kFewThreads), 0, stream, p);
 }
 
-template <class T, bool kGated>
-void launch(const LinearParams &p, hipStream_t stream) {
+template <class T, bool kGated, class P>
+void launch(const P &p, hipStream_t stream) {
   // One or two tokens: 1 x 2048 x 5632 6.3 us (the best tile shape 6.8), gated 1 x 5632 x 2048 9.0 (10.1), 2 x 512 x
   // 2048 3.1 (4.2); four by the same kernel 4 x 2048 x 5632 8.1 (6.9), 4 x 4096 x 2048 6.1 (5.9).
   if (p.m <= 2 && p.n <= (int64_t{1} << 26) - 4) {  // a launch's axis holds fewer than 2^32 threads, a column takes 64

@@ -31,6 +31,7 @@
 
 #include "grouped_prefill.hpp"
 #include "linear.hpp"
+#include "linear_adapter.hpp"
 
 namespace uniserve {
 namespace linear {
@@ -92,8 +93,9 @@ __device__ __forceinline__ void wait_stages_but(int stages) {
 
 /// kDma: rows as p.by_dma says, whole 16-byte pieces, a tile's rows within 32-bit byte offsets. Else any rows:
 /// the stages come through registers, by 16-byte loads at any alignment, zeros past the rows' ends.
-template <class T, bool kGated, bool kDma, class S>
-__global__ void __launch_bounds__(S::kThreads) tile_kernel(LinearParams p) {
+/// P: LinearParams, or AdapterParams, whose rows' adapters are added to the sums behind the walk.
+template <class T, bool kGated, bool kDma, class S, class P>
+__global__ void __launch_bounds__(S::kThreads) tile_kernel(P p) {
   using prefill::dma16;
   using prefill::lds_address;
   __shared__ u32x4 rings[S::kSplit][S::kStages][S::kRows * 8];
@@ -318,6 +320,8 @@ __global__ void __launch_bounds__(S::kThreads) tile_kernel(LinearParams p) {
   multiply(first_half, yes, no, buffer);
   if (last_chunks < 8) mask(second_half);
   multiply(second_half, no, no, 0);
+  if constexpr (std::is_same<P, AdapterParams>::value)
+    add_low_rank<T, kGated>(p, acc, m0 + wave_m * MB * 16, n0 + wave_n * kWaveCols, team, S::kSplit);
 
   // ---- the epilogue: each wavefront passes its sums through its own part of the ring (no longer read by
   // anyone), kPassMB token blocks at a time, so that a lane then holds eight consecutive columns of a
@@ -383,9 +387,9 @@ int64_t tiles_of(const LinearParams &p, bool gated) {
   return ceil_div<int64_t>(p.m, S::kBM) * ceil_div<int64_t>(p.n, gated ? S::kBN / 2 : S::kBN);
 }
 
-template <class T, bool kGated, bool kDma, class S>
-void launch_tiles(const LinearParams &p, hipStream_t stream) {
-  hipLaunchKernelGGL((tile_kernel<T, kGated, kDma, S>), dim3(static_cast<uint32_t>(tiles_of<S>(p, kGated))), dim3(S::kThreads), 0,
+template <class T, bool kGated, bool kDma, class S, class P>
+void launch_tiles(const P &p, hipStream_t stream) {
+  hipLaunchKernelGGL((tile_kernel<T, kGated, kDma, S, P>), dim3(static_cast<uint32_t>(tiles_of<S>(p, kGated))), dim3(S::kThreads), 0,
                      stream, p);
 }
 

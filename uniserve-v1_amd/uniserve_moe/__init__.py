@@ -8,6 +8,7 @@ loudly when the shared object has not been built.
 """
 
 from .abi import (  # noqa: F401
+    AdapterLinearCall,
     AddNormCall,
     DTYPE,
     ExpertTopkCall,

@@ -446,6 +446,27 @@ class AddNormCall(ctypes.Structure):
     ]
 
 
+class AdapterLinearCall(ctypes.Structure):
+    """``uniserve_adapter_linear_call``; the product's fields are reached directly, too."""
+
+    _anonymous_ = ("product",)
+    _fields_ = [
+        ("product", LinearCall),
+        ("down", _P),
+        ("up", _P),
+        ("adapter", _P),
+        ("scales", _P),
+        ("workspace", _P),
+        ("workspace_bytes", _I64),
+        ("adapters", _I64),
+        ("rank", _I64),
+        ("down_stride", _I64),
+        ("down_row_stride", _I64),
+        ("up_stride", _I64),
+        ("up_row_stride", _I64),
+    ]
+
+
 def max_tiles(tokens, top, local_experts, tile=128):
     """``ops::moe::max_tiles`` (crates/ops/src/moe/mod.rs:63-70)."""
     expanded = tokens * top
@@ -496,6 +517,8 @@ _ENTRIES = {
     "uniserve_linear": LinearCall,
     "uniserve_gated_linear": LinearCall,
     "uniserve_add_norm": AddNormCall,
+    "uniserve_adapter_linear": AdapterLinearCall,
+    "uniserve_adapter_gated_linear": AdapterLinearCall,
 }
 
 
@@ -529,6 +552,8 @@ def library():
     lib.uniserve_moe_layer_step.restype = ctypes.c_int32
     lib.uniserve_moe_layer_views_of.argtypes = [_I64] * 6 + [ctypes.POINTER(LayerViews)]
     lib.uniserve_moe_layer_views_of.restype = ctypes.c_int32
+    lib.uniserve_adapter_workspace.argtypes = [_I64] * 2
+    lib.uniserve_adapter_workspace.restype = _I64
     lib.uniserve_moe_max_tiles.argtypes = [_I64] * 4
     lib.uniserve_moe_max_tiles.restype = _I64
     _LIBRARY = lib

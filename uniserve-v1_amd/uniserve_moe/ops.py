@@ -19,6 +19,7 @@ from .abi import (
     LINEAR_ACTIVATION,
     NORM,
     SCORING,
+    AdapterLinearCall,
     AddNormCall,
     ExpertTopkCall,
     GatherCall,
@@ -156,7 +157,8 @@ def expert_topk(scores, top, scoring="sigmoid", bias=None, groups=1, top_groups=
     return ids, weights
 
 
-def _product(entry, name, x, weight, columns, bias, activation, gate, residual, out, out_dtype):
+def _product_call(name, x, weight, columns, bias, activation, gate, residual, out, out_dtype):
+    """A dense product's call, its output and its device."""
     dtype, index = x.dtype, x.get_device()
     element = _ELEMENT.get(dtype)
     if x.dim() != 2 or dtype not in _PRODUCT or index < 0:
@@ -195,6 +197,11 @@ def _product(entry, name, x, weight, columns, bias, activation, gate, residual, 
     call = LinearCall(x.data_ptr(), weight.data_ptr(), bias_at, gate_at, residual_at, out.data_ptr(), tokens, columns,
                       width, x_stride, weight_stride, gate_stride, residual_stride, out_stride, element, bias_element,
                       out_element, LINEAR_ACTIVATION[activation])
+    return call, out, index
+
+
+def _product(entry, name, x, weight, columns, bias, activation, gate, residual, out, out_dtype):
+    call, out, index = _product_call(name, x, weight, columns, bias, activation, gate, residual, out, out_dtype)
     _enter(entry, call, index, name)
     return out
 
@@ -219,6 +226,69 @@ def gated_linear(x, up_gate, bias=None, activation="silu", out=None):
         raise ValueError("gated_linear: the weight is [2 I, width], the up rows and then the gate rows")
     return _product(library().uniserve_gated_linear, "gated_linear", x, up_gate, up_gate.shape[0] // 2, bias,
                     activation, None, None, out, None)
+
+
+def adapter_workspace(tokens, rank_rows):
+    """The bytes of ``workspace`` that ``tokens`` rows take with adapters of ``rank_rows`` rows each in ``down``."""
+    return library().uniserve_adapter_workspace(tokens, rank_rows)
+
+
+def _stack(tensor, rows, columns, dtype, index, name, what):
+    """The strides of an [adapters, rows, columns] stack with contiguous rows; refuses any other."""
+    if (tensor.dim() == 3 and tensor.shape[1] == rows and tensor.shape[2] == columns and tensor.dtype == dtype
+            and tensor.get_device() == index):
+        stride, row_stride, step = tensor.stride()
+        if step == 1 or columns <= 1:
+            return stride, row_stride
+    raise ValueError(f"{name}: {what} is [adapters, {rows}, {columns}] of {dtype}, its rows contiguous, on device {index}: "
+                     f"got {tuple(tensor.shape)} of {tensor.dtype}, strides {tensor.stride()}, on {tensor.device}")
+
+
+def _adapted(entry, name, x, weight, columns, halves, down, up, adapter, scales, bias, activation, gate, residual, out,
+             out_dtype, workspace):
+    product, out, index = _product_call(name, x, weight, columns, bias, activation, gate, residual, out, out_dtype)
+    if down.dim() != 3 or up.dim() != 3 or down.shape[0] != up.shape[0] or down.shape[1] != halves * up.shape[2]:
+        raise ValueError(f"{name}: down is [adapters, {'2 ' if halves == 2 else ''}rank, width], up [adapters, rows, rank]")
+    count, _, rank = up.shape
+    down_stride, down_row_stride = _stack(down, halves * rank, x.shape[1], x.dtype, index, name, "down")
+    up_stride, up_row_stride = _stack(up, halves * columns, rank, x.dtype, index, name, "up")
+    if workspace is None:
+        workspace = torch.empty(adapter_workspace(x.shape[0], halves * rank), dtype=torch.uint8, device=x.device)
+    elif workspace.get_device() != index or not workspace.is_contiguous():
+        raise ValueError(f"{name}: the workspace is contiguous, on device {index}")
+    call = AdapterLinearCall(product, down.data_ptr(), up.data_ptr(),
+                             _vector(adapter, x.shape[0], (torch.int32,), index, name, "adapter"),
+                             _vector(scales, count, (torch.float32,), index, name, "scales"), workspace.data_ptr(),
+                             workspace.numel() * workspace.element_size(), count, rank, down_stride, down_row_stride,
+                             up_stride, up_row_stride)
+    _enter(entry, call, index, name)
+    return out
+
+
+def adapter_linear(x, weight, down, up, adapter, scales=None, bias=None, activation=None, gate=None, residual=None,
+                   out=None, out_dtype=None, workspace=None):
+    """``linear`` with each row's own low-rank adapter beside the shared weight: with ``a = adapter[t]`` (int32
+    ``[T]``; outside the stack: none), ``x[t] @ weight.T + scales[a] * (x[t] @ down[a].T) @ up[a].T`` takes the
+    product's place. ``down`` is ``[A, R, K]`` and ``up`` ``[A, N, R]`` of ``x``'s type (adapters of smaller rank
+    padded with zeros), ``scales`` f32 ``[A]`` or None for ones.
+
+    ``workspace``: ``adapter_workspace(T, R)`` bytes, aligned as torch allocates, for one call at a time; None
+    allocates them."""
+    if weight.dim() != 2:
+        raise ValueError("adapter_linear: the weight is [rows, width]")
+    return _adapted(library().uniserve_adapter_linear, "adapter_linear", x, weight, weight.shape[0], 1, down, up, adapter,
+                    scales, bias, activation, gate, residual, out, out_dtype, workspace)
+
+
+def adapter_gated_linear(x, up_gate, down, up, adapter, scales=None, bias=None, activation="silu", out=None,
+                         workspace=None):
+    """``gated_linear`` with each row's own low-rank adapter, whose halves have factors of their own: ``down``
+    ``[A, 2 R, K]``, the up half's rows and then the gate half's, ``up`` ``[A, 2 I, R]`` likewise. The rest is
+    ``adapter_linear``'s; ``workspace`` takes ``adapter_workspace(T, 2 R)`` bytes."""
+    if up_gate.dim() != 2 or up_gate.shape[0] % 2 != 0:
+        raise ValueError("adapter_gated_linear: the weight is [2 I, width], the up rows and then the gate rows")
+    return _adapted(library().uniserve_adapter_gated_linear, "adapter_gated_linear", x, up_gate, up_gate.shape[0] // 2, 2,
+                    down, up, adapter, scales, bias, activation, None, None, out, None, workspace)
 
 
 _PRODUCT = (torch.bfloat16, torch.float16)
