@@ -23,7 +23,7 @@
 // `workspace` is uniserve_adapter_workspace(m, rank rows) bytes, 16-byte aligned, rank rows being the rows of
 // one adapter in down; its contents before the call do not matter and after it are of no use. Calls that may
 // overlap in time need one each. Two launches; nothing is allocated and the call may be captured. Refused
-// besides what the products refuse: 2^28 - 15 rows and more, a rank above UNISERVE_ADAPTER_MAX_RANK, stacks of more than 2^40
+// besides what the products refuse: more than 2^23 rows, a rank above UNISERVE_ADAPTER_MAX_RANK, stacks of more than 2^40
 // elements, an output that overlaps a stack, the indices, the scales or the workspace, and a workspace that
 // overlaps any input.
 

@@ -266,7 +266,7 @@ def test_each_tile_kernel(device, gated, shape, m, n, k, rank):
 
     mangled = "TileShapeI" + "".join(f"Li{d}E" for d in shape.split(","))
     names = kernels_of(run)
-    assert len(names) == 2 and "low_rank_kernel" in names[0] and mangled in names[1], names
+    assert len(names) == 2 and "RankParams" in names[0] and mangled in names[1], names
     for order in (each_other, runs):
         call["adapter"].copy_(order(m, 5))
         run()

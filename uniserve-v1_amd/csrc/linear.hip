@@ -13,6 +13,9 @@ namespace {
 /// 64 x 64 tiles of 256 threads whose threads an axis of a launch holds (shapes that need more are not chosen).
 constexpr int64_t kMostTiles = (int64_t{1} << 32) / 256 - 1;
 
+/// The largest row stride of 256 rows within the DMA's 32-bit byte offsets.
+constexpr int64_t kMostStride = int64_t{1} << 22;
+
 /// Whether a product can be served: 0, with its parameters in `p`, or a refusal. A call without rows (m = 0) has no
 /// parameters.
 int32_t check(const uniserve_linear_call *call, bool gated, const char *name, LinearParams &p) {
@@ -73,7 +76,6 @@ int32_t check(const uniserve_linear_call *call, bool gated, const char *name, Li
   p.out_f32 = call->out_dtype == UNISERVE_DTYPE_F32;
   p.activation = static_cast<int32_t>(call->activation);
   // The tile kernels' DMA reads whole 16 bytes at aligned addresses, a tile's rows within 32-bit offsets.
-  constexpr int64_t kMostStride = int64_t{1} << 22;
   p.by_dma = k % 8 == 0 && x_stride % 8 == 0 && w_stride % 8 == 0 && aligned_to(p.x, 16) && aligned_to(p.w, 16) &&
              x_stride <= kMostStride && w_stride <= kMostStride;
   if (ceil_div<int64_t>(m, 64) * ceil_div<int64_t>(n, gated ? 32 : 64) > kMostTiles)
@@ -81,8 +83,8 @@ int32_t check(const uniserve_linear_call *call, bool gated, const char *name, Li
   return 0;
 }
 
-/// Rows of the first factor's kernel, 16 threads each, that an axis of a launch holds.
-constexpr int64_t kMostAdapterRows = (int64_t{1} << 28) - 16;
+/// Rows whose tiles of 32 x 32 rank values, at the largest rank, an axis of a launch holds.
+constexpr int64_t kMostAdapterRows = int64_t{1} << 23;
 
 int32_t run(const uniserve_linear_call *call, void *stream, bool gated, const char *name) {
   LinearParams p{};
@@ -142,9 +144,11 @@ int32_t run_adapters(const uniserve_adapter_linear_call *adapters, void *stream,
   p.scales = adapters->scales;
   p.low = static_cast<char *>(adapters->workspace);
   p.adapters = static_cast<int32_t>(count), p.rank = static_cast<int32_t>(rank);
-  p.down_whole = p.k % 8 == 0 && p.x_stride % 8 == 0 && p.down_stride % 8 == 0 && p.down_row_stride % 8 == 0 &&
-                 aligned_to(p.x, 16) && aligned_to(p.down, 16);
-  p.up_whole = rank % 8 == 0 && p.up_stride % 8 == 0 && p.up_row_stride % 8 == 0 && aligned_to(p.up, 16);
+  p.down_by_dma = p.k % 8 == 0 && p.x_stride % 8 == 0 && p.down_stride % 8 == 0 && p.down_row_stride % 8 == 0 &&
+                  aligned_to(p.x, 16) && aligned_to(adapters->down, 16) && p.x_stride <= kMostStride &&
+                  down_rows * p.down_row_stride <= 256 * kMostStride;
+  p.up_whole = rank % 8 == 0 && p.up_stride % 8 == 0 && p.up_row_stride % 8 == 0 && aligned_to(adapters->up, 16) &&
+               p.up_row_stride <= kMostStride;
   const hipStream_t s = static_cast<hipStream_t>(stream);
   if (call->dtype == UNISERVE_DTYPE_F16) launch_adapters_f16(p, gated, s);
   else launch_adapters_bf16(p, gated, s);

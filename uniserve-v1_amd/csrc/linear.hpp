@@ -5,7 +5,7 @@
 #pragma once
 
 #include "common.hpp"
-#include "uniserve_linear.h"
+#include "uniserve_adapter_linear.h"
 
 namespace uniserve {
 namespace linear {
@@ -46,8 +46,19 @@ struct AdapterParams : LinearParams {
   char *low;               ///< the workspace: each row's rank values
   int64_t down_stride, down_row_stride, up_stride, up_row_stride;
   int32_t adapters, rank;
-  int32_t down_whole;  ///< input and down rows are whole 16-byte pieces
-  int32_t up_whole;    ///< up rows are
+  int32_t down_by_dma;  ///< input and down rows suit the tile kernels' loads
+  int32_t up_whole;     ///< up rows are whole 16-byte pieces, 256 of them within 32-bit byte offsets
+};
+
+/// The adapters' first factor as a product: columns are the rank values in their layout's order, n of them.
+struct RankParams : AdapterParams {
+  int32_t width, groups, halves;  ///< LowLayout
+  /// Column j's row of an adapter's first factor (past the rank: the last one; the value is dropped).
+  __device__ __forceinline__ int64_t down_row(int64_t j) const {
+    const int at = static_cast<int>(j < n ? j : n - 1);
+    const int group = at / width, half = group / groups, in_half = (group - half * groups) * width + at % width;
+    return half * rank + (in_half < rank ? in_half : rank - 1);
+  }
 };
 
 /// Launches a call that was found servable.

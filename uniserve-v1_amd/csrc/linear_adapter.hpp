@@ -26,202 +26,358 @@ __device__ __forceinline__ u32x4 load8_of(const uint16_t *row, int64_t at, int64
   else return load8(row, at, width);
 }
 
-// ---- the first factor -------------------------------------------------------------------------------------
+// ---- which adapters a tile names ---------------------------------------------------------------------------
 
-/// 16 rows by kBlocks blocks of 16 ranks a workgroup, whose kWaves wavefronts take the 64-element stages of K in
-/// turn and add their sums in LDS. blockIdx.y: the rank blocks; blockIdx.z: with gridDim.z > 1 the workgroups
-/// share out the adapters that the 16 rows name. kWide: groups of 32 ranks (LowLayout), two blocks each.
-template <class T, bool kWhole, bool kWide, int kWaves, int kBlocks>
-__global__ void __launch_bounds__(kWaves *kWave) low_rank_kernel(AdapterParams p, int halves) {
-  constexpr int kPerGroup = kWide ? 2 : 1;
-  static_assert(kBlocks % kPerGroup == 0, "whole groups");
-  __shared__ float sums[kWaves][kBlocks][16][16];  // of rank block, row, rank
-  const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / kWave);
-  const int lane = lane_id();
-  const int r16 = lane & 15, g = lane >> 4;
-  const int64_t m0 = static_cast<int64_t>(blockIdx.x) * 16;
-  const LowLayout layout(p.rank);
-  const int first_block = static_cast<int>(blockIdx.y) * kBlocks;
-  const int all_blocks = halves * layout.groups * kPerGroup;
-  const uint16_t *x = p.x + (m0 + r16 < p.m ? m0 + r16 : p.m - 1) * p.x_stride;
-  // The lane's row of each block in an adapter's factor (past the rank: the last one, its value is dropped).
-  int64_t row[kBlocks];
+/// The distinct adapters of a tile's rows, one after the other, found by every wavefront alike.
+struct NamedAdapters {
+  int id[4];              ///< of rows lane, 64 + lane, ..
+  uint64_t remaining[4];  ///< rows whose adapter has not come yet
+  uint64_t members[4];    ///< rows of the current one
+  int current = -1;
+  uint32_t turn = 0, share = 0, shares = 1;
+  int blocks;
+
+  /// (find takes the rows' adapters from LDS)
+  __device__ __forceinline__ explicit NamedAdapters(int rows) : blocks((rows + 63) / 64) {}
+  __device__ __forceinline__ void find(const int32_t *ids) {
 #pragma unroll
-  for (int q = 0; q < kBlocks; ++q) {
-    const int block = first_block + q < all_blocks ? first_block + q : all_blocks - 1;
-    const int half = block / (layout.groups * kPerGroup), in_half = block % (layout.groups * kPerGroup) * 16 + r16;
-    row[q] = (half * p.rank + (in_half < p.rank ? in_half : p.rank - 1)) * p.down_row_stride;
-  }
-  const int mine = adapter_of(p, m0 + r16);
-  uint32_t remaining = static_cast<uint32_t>(ballot(mine >= 0)) & 0xffffu;
-  for (int turn = 0; remaining != 0; turn = turn + 1 == static_cast<int>(gridDim.z) ? 0 : turn + 1) {
-    const int current = __builtin_amdgcn_readlane(mine, __ffs(static_cast<int>(remaining)) - 1);
-    remaining &= ~static_cast<uint32_t>(ballot(mine == current));
-    if (turn != static_cast<int>(blockIdx.z)) continue;
-    const uint16_t *down = p.down + current * p.down_stride;
-    floatx4 acc[kBlocks];
-#pragma unroll
-    for (int q = 0; q < kBlocks; ++q) acc[q] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
-    // A lane's 16 bytes are chunks g and g + 4 of a stage's eight, in both operands.
-    for (int64_t k = wave * 64; k < p.k; k += kWaves * 64) {
-      u32x4 xs[2], ws[kBlocks][2];
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        xs[i] = load8_of<kWhole>(x, k + (g + 4 * i) * 8, p.k);
-#pragma unroll
-        for (int q = 0; q < kBlocks; ++q) ws[q][i] = load8_of<kWhole>(down + row[q], k + (g + 4 * i) * 8, p.k);
+    for (int i = 0; i < 4; ++i)
+      if (i < blocks) {
+        id[i] = ids[i * 64 + lane_id()];
+        remaining[i] = ballot(id[i] >= 0);
       }
+  }
+  /// Of a workgroup that shares a tile's adapters with gridDim.y - 1 others.
+  __device__ __forceinline__ NamedAdapters(const RankParams &p, int64_t m0, int rows) : share(blockIdx.y), shares(gridDim.y), blocks(1) {
+    id[0] = lane_id() < rows ? adapter_of(p, m0 + lane_id()) : -1;
+    remaining[0] = ballot(id[0] >= 0);
+  }
+  __device__ __forceinline__ bool next() {
+    for (;;) {
+      current = -1;
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
+      for (int i = 3; i >= 0; --i)
+        if (i < blocks && remaining[i] != 0) current = __builtin_amdgcn_readlane(id[i], __ffsll(static_cast<long long>(remaining[i])) - 1);
+      if (current < 0) return false;
 #pragma unroll
-        for (int q = 0; q < kBlocks; ++q) acc[q] = T::mfma(ws[q][i], xs[i], acc[q]);
+      for (int i = 0; i < 4; ++i)
+        if (i < blocks) {
+          members[i] = ballot(id[i] == current);
+          remaining[i] &= ~members[i];
+        }
+      const bool mine = turn == share;
+      turn = turn + 1 == shares ? 0 : turn + 1;
+      if (mine) return true;
     }
-    __syncthreads();  // (the adapter before: its sums have been read)
+  }
+  /// How many there are, from a copy; `mixed`: whether some of the tile's `rows` rows name another than the first, or none.
+  __device__ __forceinline__ int count(int rows, bool &mixed) const {
+    NamedAdapters all = *this;
+    int found = 0, first_rows = 0;
+    while (all.next()) {
+      if (found == 0)
 #pragma unroll
-    for (int q = 0; q < kBlocks; ++q) *reinterpret_cast<floatx4 *>(&sums[wave][q][r16][4 * g]) = acc[q];
-    __syncthreads();
-    // A group's values of one row on neighbouring lanes.
-    constexpr int kLanes = kPerGroup * 16;
-    const float scale = p.scales == nullptr ? 1.0f : p.scales[current];
-    for (int i = threadIdx.x; i < kBlocks / kPerGroup * 16 * kLanes; i += kWaves * kWave) {
-      const int rank = i % kLanes, r = i / kLanes % 16, of = i / kLanes / 16;
-      const int group = first_block / kPerGroup + of;
+        for (int i = 0; i < 4; ++i)
+          if (i < blocks) first_rows += __popcll(all.members[i]);
+      ++found;
+    }
+    mixed = found > 0 && first_rows < rows;
+    return found;
+  }
+  /// The first row of the current adapter.
+  __device__ __forceinline__ int first_row() const {
+    int row = 0;
+#pragma unroll
+    for (int i = 3; i >= 0; --i)
+      if (i < blocks && members[i] != 0) row = i * 64 + __ffsll(static_cast<long long>(members[i])) - 1;
+    return row;
+  }
+  /// Of up to 64 rows: whether row r names the current adapter, and row r, or, if it does not, one that does.
+  __device__ __forceinline__ bool holds(int r) const { return (members[0] >> r) & 1; }
+  __device__ __forceinline__ int row(int r) const { return holds(r) ? r : first_row(); }
+};
+
+__device__ __forceinline__ NamedAdapters named_adapters(const RankParams &p, int64_t m0, int rows) { return NamedAdapters(p, m0, rows); }
+__device__ __forceinline__ int named_adapters(const LinearParams &, int64_t, int) { return 0; }
+
+/// The adapters of a tile's kRows rows and, f16, the factors of their group in either of two buffers.
+template <int kRows, bool kFactors>
+struct RowsAdapters {
+  static constexpr int kIds = (kRows + 63) / 64 * 64;
+  int32_t id[kIds];
+  float factor[2][kFactors ? kRows : 1];
+  __device__ __forceinline__ void load(const AdapterParams &p, int64_t m0) {
+    for (int t = threadIdx.x; t < kIds; t += blockDim.x) id[t] = t < kRows ? adapter_of(p, m0 + t) : -1;
+  }
+  __device__ __forceinline__ void load_factors(const AdapterParams &p, int64_t m0, int buffer, const LowLayout &layout, int halves, int part) {
+    for (int t = threadIdx.x; t < kRows; t += blockDim.x) {
+      const int64_t m = m0 + t < p.m ? m0 + t : p.m - 1;
+      factor[buffer][t] = *reinterpret_cast<const float *>(p.low + m * layout.row_bytes(halves) +
+                                                           static_cast<int64_t>(part) * layout.group_bytes() + 4 * layout.width);
+    }
+  }
+};
+template <bool kFactors>
+struct RowsAdapters<0, kFactors> {};
+
+template <bool kWalked, class Rows>
+__device__ __forceinline__ auto tile_adapters(const Rows &, int rows) {
+  if constexpr (kWalked) return NamedAdapters(rows);
+  else return 0;
+}
+
+/// Makes those of a row's sums of eight columns again, from the row's own operands alone, that are not finite: in a tile
+/// whose rows name several adapters, the walk multiplies the others' up rows by zeros, which gives NaN where they are
+/// not finite. (What the row itself makes infinite or NaN stays so.)
+template <class T, bool kGated>
+__device__ __forceinline__ void remake(const AdapterParams &p, int64_t m, int64_t n, int adapter, floatx4 (&sums)[2], floatx4 (&gates)[2]) {
+  bool finite = true;
+#pragma unroll
+  for (int c = 0; c < 8; ++c) {
+    finite = finite && __builtin_fabsf(sums[c / 4][c % 4]) < __builtin_inff();
+    if (kGated) finite = finite && __builtin_fabsf(gates[c / 4][c % 4]) < __builtin_inff();
+  }
+  if (finite) return;
+  const LowLayout layout(p.rank);
+#pragma unroll 1
+  for (int h = 0; h < (kGated ? 2 : 1); ++h) {
+#pragma unroll 1
+    for (int i = 0; i < 8; ++i) {
+      if (n + i >= p.n) continue;
       float v = 0.0f;
 #pragma unroll
-      for (int w = 0; w < kWaves; ++w) v += sums[w][of * kPerGroup + rank / 16][r][rank % 16];
-      const int in_half = group % layout.groups * layout.width + rank;
-      v = in_half < p.rank ? v * scale : 0.0f;
-      float factor = 1.0f;
-      if constexpr (std::is_same<T, F16>::value) {
-        // The power of two that brings the group's largest value to [1, 2).
-        float most = __builtin_fabsf(v);
-#pragma unroll
-        for (int offset = kLanes / 2; offset > 0; offset /= 2) most = __builtin_fmaxf(most, __shfl_xor(most, offset));
-        if (most > 0.0f && most < __builtin_inff()) {
-          const int power = __builtin_amdgcn_frexp_expf(most) - 1;
-          v = __builtin_ldexpf(v, -power);
-          factor = __builtin_ldexpf(1.0f, power < -126 ? -126 : power);
-          if (power < -126) v = __builtin_ldexpf(v, power + 126);
+      for (int c = 0; c < 8; ++c)
+        if (c == i) v = h == 0 ? sums[c / 4][c % 4] : gates[c / 4][c % 4];
+      if (__builtin_fabsf(v) < __builtin_inff()) continue;
+      const int64_t column = n + i + h * p.n;
+      v = 0.0f;
+      if (adapter >= 0) {
+        const uint16_t *up = p.up + adapter * p.up_stride + column * p.up_row_stride;
+#pragma unroll 1
+        for (int rank = 0; rank < p.rank; ++rank) {
+          const uint16_t *low = reinterpret_cast<const uint16_t *>(p.low + m * layout.row_bytes(kGated ? 2 : 1) +
+                                                                   static_cast<int64_t>(h * layout.groups + rank / layout.width) * layout.group_bytes()) +
+                                rank % layout.width;
+          v = __builtin_fmaf(T::to_f32(low[0]) + T::to_f32(low[layout.width]), T::to_f32(up[rank]), v);
         }
       }
-      const uint16_t high = T::from_f32(v);
-      const float error = v - T::to_f32(high);
-      const int owner = __shfl(mine, r);  // (the lanes of every wavefront hold the 16 rows' adapters)
-      if (owner != current || rank >= layout.width || first_block + of * kPerGroup >= all_blocks) continue;
-      char *at = p.low + (m0 + r) * layout.row_bytes(halves) + static_cast<int64_t>(group) * layout.group_bytes();
-      reinterpret_cast<uint16_t *>(at)[rank] = high;
-      reinterpret_cast<uint16_t *>(at)[layout.width + rank] = T::from_f32(error == error ? error : 0.0f);
-      if (std::is_same<T, F16>::value && rank == 0) *reinterpret_cast<float *>(at + 4 * layout.width) = factor;
+#pragma unroll 1
+      for (int64_t k = 0; k < p.k; ++k)
+        v = __builtin_fmaf(T::to_f32(p.x[m * p.x_stride + k]), T::to_f32(p.w[column * p.w_stride + k]), v);
+#pragma unroll
+      for (int c = 0; c < 8; ++c)
+        if (c == i) {
+          if (h == 0) sums[c / 4][c % 4] = v;
+          else gates[c / 4][c % 4] = v;
+        }
     }
   }
 }
 
-template <class T, bool kWhole, bool kWide, int kWaves, int kBlocks>
-void launch_low_rank_kernel(const AdapterParams &p, int halves, int shares, hipStream_t stream) {
-  const LowLayout layout(p.rank);
-  const int blocks = halves * layout.groups * (kWide ? 2 : 1);
-  const dim3 grid(static_cast<uint32_t>(ceil_div<int64_t>(p.m, 16)), static_cast<uint32_t>(ceil_div(blocks, kBlocks)), static_cast<uint32_t>(shares));
-  hipLaunchKernelGGL((low_rank_kernel<T, kWhole, kWide, kWaves, kBlocks>), grid, dim3(kWaves * kWave), 0, stream, p, halves);
-}
+// ---- the first factor -------------------------------------------------------------------------------------
 
+/// The epilogue of the first factor: eight consecutive rank values of a row, scaled, as elements and their errors.
 template <class T>
-void launch_low_rank(const AdapterParams &p, bool gated, hipStream_t stream) {
-  const int halves = gated ? 2 : 1;
-  const bool wide = LowLayout(p.rank).width == 32;
-  if (p.m <= 256) {
-    const int shares = p.m < 16 ? static_cast<int>(p.m) : 16;
-    if (wide) p.down_whole ? launch_low_rank_kernel<T, true, true, 16, 2>(p, halves, shares, stream)
-                           : launch_low_rank_kernel<T, false, true, 16, 2>(p, halves, shares, stream);
-    else p.down_whole ? launch_low_rank_kernel<T, true, false, 16, 1>(p, halves, shares, stream)
-                      : launch_low_rank_kernel<T, false, false, 16, 1>(p, halves, shares, stream);
-    return;
+struct RankColumns {
+  int64_t at;     ///< of the values in a row's workspace; -1: past the last group
+  int errors_at;  ///< from there
+  int factor_at;
+  int count;      ///< values below the rank
+  __device__ __forceinline__ RankColumns(const RankParams &p, int64_t j) {
+    const LowLayout layout(p.rank);
+    const int group = static_cast<int>(j / p.width), chunk = static_cast<int>(j % p.width) / 8;
+    const int in_half = group % p.groups * p.width + chunk * 8;
+    at = j < p.n ? static_cast<int64_t>(group) * layout.group_bytes() + chunk * 16 : -1;
+    errors_at = 2 * p.width;
+    factor_at = chunk == 0 ? 4 * p.width : -1;
+    count = p.rank - in_half;
   }
-  if (wide) p.down_whole ? launch_low_rank_kernel<T, true, true, 4, 4>(p, halves, 1, stream)
-                         : launch_low_rank_kernel<T, false, true, 4, 4>(p, halves, 1, stream);
-  else p.down_whole ? launch_low_rank_kernel<T, true, false, 4, 2>(p, halves, 1, stream)
-                    : launch_low_rank_kernel<T, false, false, 4, 2>(p, halves, 1, stream);
-}
+  __device__ __forceinline__ void finish(const RankParams &p, int64_t m, int adapter, const floatx4 (&sums)[2]) const {
+    const float scale = p.scales == nullptr ? 1.0f : p.scales[adapter];
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = i < count ? sums[i / 4][i % 4] * scale : 0.0f;
+    float factor = 1.0f;
+    if constexpr (std::is_same<T, F16>::value) {
+      // The power of two that brings the group's largest value to [1, 2); its lanes are neighbours.
+      float most = 0.0f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) most = __builtin_fmaxf(most, __builtin_fabsf(v[i]));
+      for (int offset = 1; offset < p.width / 8; offset *= 2) most = __builtin_fmaxf(most, __shfl_xor(most, offset));
+      if (most > 0.0f && most < __builtin_inff()) {
+        int power = __builtin_amdgcn_frexp_expf(most) - 1;
+        power = power < -126 ? -126 : power;
+        factor = __builtin_ldexpf(1.0f, power);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = __builtin_ldexpf(v[i], -power);
+      }
+    }
+    if (at < 0) return;
+    u32x4 values, errors;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      values[i] = T::pack2(v[2 * i], v[2 * i + 1]);
+      const float low = v[2 * i] - T::low(values[i]), high = v[2 * i + 1] - T::high(values[i]);
+      errors[i] = T::pack2(low == low ? low : 0.0f, high == high ? high : 0.0f);
+    }
+    char *to = p.low + m * LowLayout(p.rank).row_bytes(p.halves) + at;
+    *reinterpret_cast<u32x4 *>(to) = values;
+    *reinterpret_cast<u32x4 *>(to + errors_at) = errors;
+    // (bf16 rows need no factor; 16 zeros stand there)
+    if (factor_at >= 0) *reinterpret_cast<u32x4 *>(to + factor_at) = u32x4{std::is_same<T, F16>::value ? __float_as_uint(factor) : 0, 0, 0, 0};
+  }
+};
 
 // ---- the second factor ------------------------------------------------------------------------------------
 
-/// Adds the adapters' products to a wavefront's sums: token blocks mb from row m_first on, weight blocks nb from
-/// column n_first on (gated: half of them the up rows', then the same columns' gate rows), one adapter that its rows
-/// name after the other; of `teams` wavefronts with the same sums, which are added up later, each takes its share of
-/// the adapters. Two matrix instructions per 32 ranks, over the values and over their errors, or, up to rank 16,
-/// one over both.
+/// Adapters whose loads a wavefront has in flight together, by the blocks that one takes.
+template <int NB, int MB>
+constexpr int adapter_batch() { return NB + 2 * MB <= 4 ? 4 : NB + 2 * MB <= 8 ? 2 : 1; }
+
+/// The adapters of a wavefront's rows: of token block b's row lane % 16.
+template <int MB>
+struct RowAdapters {
+  int of[MB];
+  __device__ __forceinline__ RowAdapters(const AdapterParams &p, int64_t m_first) {
+#pragma unroll
+    for (int b = 0; b < MB; ++b) of[b] = adapter_of(p, m_first + b * 16 + lane_id() % 16);
+  }
+};
+
+/// What add_low_rank needs, for the kernels that call it.
+template <int MB, bool kMany>
+__device__ __forceinline__ auto row_adapters(const AdapterParams &p, int64_t m_first) {
+  if constexpr (kMany) return 0;
+  else return RowAdapters<MB>(p, m_first);
+}
+template <int MB, bool kMany>
+__device__ __forceinline__ int row_adapters(const LinearParams &, int64_t) { return 0; }
+template <int MB, bool kMany>
+__device__ __forceinline__ int row_adapters(const RankParams &, int64_t) { return 0; }
+
+/// Adds the adapters' products to a wavefront's sums: token blocks b from row m_first on, weight blocks nb from
+/// column n_first on (gated: half of them the up rows', then the same columns' gate rows), some of the adapters that
+/// its rows name after the others; of `teams` wavefronts with the same sums, which are added up later, each takes
+/// its share of the adapters. Two matrix instructions per 32 ranks, over the values and over their errors, or, up to
+/// rank 16, one over both.
 template <class T, bool kGated, int NB, int MB>
-__device__ __forceinline__ void add_low_rank(const AdapterParams &p, floatx4 (&acc)[NB][MB], int64_t m_first, int64_t n_first, int team,
-                                             int teams) {
+__device__ __forceinline__ void add_low_rank(const AdapterParams &p, floatx4 (&acc)[NB][MB], const RowAdapters<MB> &mine, int64_t m_first,
+                                             int64_t n_first, int team, int teams) {
   const int lane = lane_id();
   const int r16 = lane & 15, g = lane >> 4;
   const LowLayout layout(p.rank);
-  constexpr int kHalves = kGated ? 2 : 1, kPerHalf = NB / kHalves;
-  int mine[MB];
+  constexpr int kHalves = kGated ? 2 : 1, kPerHalf = NB / kHalves, kBatch = adapter_batch<NB, MB>();
   uint32_t remaining[MB];
 #pragma unroll
-  for (int b = 0; b < MB; ++b) mine[b] = adapter_of(p, m_first + b * 16 + r16);
+  for (int b = 0; b < MB; ++b) remaining[b] = static_cast<uint32_t>(ballot(mine.of[b] >= 0)) & 0xffffu;
+  // The next adapter of this wavefront's share, or -1. (Shares by number: a row's sums do not depend on the other
+  // rows' adapters.)
+  auto next = [&]() {
+    for (;;) {
+      int current = -1;
 #pragma unroll
-  for (int b = 0; b < MB; ++b) remaining[b] = static_cast<uint32_t>(ballot(mine[b] >= 0)) & 0xffffu;
+      for (int b = MB - 1; b >= 0; --b)
+        if (remaining[b] != 0) current = __builtin_amdgcn_readlane(mine.of[b], __ffs(static_cast<int>(remaining[b])) - 1);
+      if (current < 0) return -1;
+#pragma unroll
+      for (int b = 0; b < MB; ++b) remaining[b] &= ~static_cast<uint32_t>(ballot(mine.of[b] == current));
+      if (current % teams == team) return current;
+    }
+  };
+  int current[kBatch];
+#pragma unroll
+  for (int j = 0; j < kBatch; ++j) current[j] = next();
+  if (current[0] < 0) return;
   int64_t row[NB];
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb) {
     const int64_t n = n_first + nb % kPerHalf * 16 + r16;
     row[nb] = ((n < p.n ? n : p.n - 1) + nb / kPerHalf * p.n) * p.up_row_stride;
   }
-  const int64_t row_bytes = layout.row_bytes(kHalves);
-  // The lane's chunk of eight ranks in the up rows, and its chunks of the values and of the errors (`both`: the
-  // chunk that its place holds of either, in one operand).
+  // Where the lane's row of block b has its rank values (rows past the last and rows without an adapter read some
+  // row's, and drop what they make of them).
+  auto low_of = [&](int b) {
+    const int64_t m = m_first + b * 16 + r16;
+    return p.low + (m < p.m ? m : p.m - 1) * layout.row_bytes(kHalves) + 16 * g;
+  };
+  // The lane's chunk of eight ranks in the up rows. Up to rank 16 its place in a group is that of a value or of an error
+  // (the errors follow the values), else one of each.
   const bool both = layout.width <= 16;
-  const int up_chunk = layout.width == 32 ? g : layout.width == 16 ? g & 1 : 0;
-  const int low_at = 16 * g;  // bytes; the errors follow the values
+  const int up_at = (layout.width == 32 ? g : layout.width == 16 ? g & 1 : 0) * 8;
   const bool held = layout.width >= 16 || g < 2;
-  for (;;) {
-    int current = -1;
+  const int factor_at = 4 * layout.width - 16 * g;
+  auto products = [&](auto errors_too, int group) {
+    constexpr bool kErrors = decltype(errors_too)::value;
+    const int64_t at = group * 32 + up_at;
+    u32x4 ws[kBatch][NB];
 #pragma unroll
-    for (int b = MB - 1; b >= 0; --b)
-      if (remaining[b] != 0) current = __builtin_amdgcn_readlane(mine[b], __ffs(static_cast<int>(remaining[b])) - 1);
-    if (current < 0) break;
+    for (int j = 0; j < kBatch; ++j) {
+      const uint16_t *up = p.up + (current[j] < 0 ? current[0] : current[j]) * p.up_stride;
+      if (p.up_whole) {
 #pragma unroll
-    for (int b = 0; b < MB; ++b) remaining[b] &= ~static_cast<uint32_t>(ballot(mine[b] == current));
-    if (current % teams != team) continue;  // (by its number: a row's sums do not depend on the other rows' adapters)
-    const uint16_t *up = p.up + current * p.up_stride;
-    for (int group = 0; group < layout.groups; ++group) {
-      const int64_t at = group * 32 + up_chunk * 8;
-      u32x4 ws[NB];
+        for (int nb = 0; nb < NB; ++nb) ws[j][nb] = load8_of<true>(up + row[nb], at, p.rank);
+      } else {
 #pragma unroll
-      for (int nb = 0; nb < NB; ++nb) {
-        if (p.up_whole) ws[nb] = load8_of<true>(up + row[nb], at, p.rank);
-        else ws[nb] = load8_of<false>(up + row[nb], at, p.rank);
-        if (!held) ws[nb] = u32x4{0, 0, 0, 0};
+        for (int nb = 0; nb < NB; ++nb) ws[j][nb] = load8_of<false>(up + row[nb], at, p.rank);
       }
+    }
+    // Two token blocks at a time: all at once do not fit the registers of the large shapes.
+    constexpr int kPair = MB < 2 ? MB : 2;
+    static_assert(MB == 3 || MB % kPair == 0, "whole pairs");
 #pragma unroll
-      for (int b = 0; b < MB; ++b) {
-        if (ballot(mine[b] == current) == 0) continue;
-        const bool own = mine[b] == current;
+    for (int first = 0; first < MB; first += kPair) {
+      u32x4 values[kHalves][kPair], errors[kHalves][kPair];
+      float factor[kHalves][kPair];
 #pragma unroll
-        for (int h = 0; h < kHalves; ++h) {
-          const char *low = p.low + (m_first + b * 16 + r16) * row_bytes + (h * layout.groups + group) * layout.group_bytes();
-          u32x4 values{0, 0, 0, 0}, errors{0, 0, 0, 0};
-          float factor = 1.0f;
-          if (own) {
-            if (held) values = *reinterpret_cast<const u32x4 *>(low + low_at);
-            if (!both) errors = *reinterpret_cast<const u32x4 *>(low + 64 + low_at);
-            if constexpr (std::is_same<T, F16>::value) factor = *reinterpret_cast<const float *>(low + 4 * layout.width);
-          }
+      for (int h = 0; h < kHalves; ++h) {
+        const int64_t of = static_cast<int64_t>(h * layout.groups + group) * layout.group_bytes();
 #pragma unroll
-          for (int j = 0; j < kPerHalf; ++j) {
-            const int nb = h * kPerHalf + j;
-            floatx4 part = T::mfma(ws[nb], values, floatx4{0.0f, 0.0f, 0.0f, 0.0f});
-            if (!both) part = T::mfma(ws[nb], errors, part);
+        for (int i = 0; i < kPair; ++i) {
+          if (first + i >= MB) continue;
+          const char *from = low_of(first + i) + of;
+          values[h][i] = *reinterpret_cast<const u32x4 *>(from);
+          if constexpr (kErrors) errors[h][i] = *reinterpret_cast<const u32x4 *>(from + 64);
+          if constexpr (std::is_same<T, F16>::value) factor[h][i] = *reinterpret_cast<const float *>(from + factor_at);
+        }
+      }
+      const u32x4 nothing{0, 0, 0, 0};
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              if constexpr (std::is_same<T, F16>::value) acc[nb][b][i] = own ? __builtin_fmaf(part[i], factor, acc[nb][b][i]) : acc[nb][b][i];
-              else acc[nb][b][i] = own ? acc[nb][b][i] + part[i] : acc[nb][b][i];
+      for (int h = 0; h < kHalves; ++h)
+#pragma unroll
+        for (int i = 0; i < kPair; ++i) {
+          const int b = first + i;
+          if (b >= MB) continue;
+          if (!held) values[h][i] = nothing;
+#pragma unroll
+          for (int j = 0; j < kBatch; ++j) {
+            const bool own = current[j] >= 0 && mine.of[b] == current[j];
+            if (ballot(own) == 0) continue;
+#pragma unroll
+            for (int of = 0; of < kPerHalf; ++of) {
+              const int nb = h * kPerHalf + of;
+              const u32x4 w = held ? ws[j][nb] : nothing;
+              floatx4 part = T::mfma(w, values[h][i], floatx4{0.0f, 0.0f, 0.0f, 0.0f});
+              if constexpr (kErrors) part = T::mfma(w, errors[h][i], part);
+#pragma unroll
+              for (int c = 0; c < 4; ++c) {
+                const float v = std::is_same<T, F16>::value ? part[c] * factor[h][i] : part[c];
+                acc[nb][b][c] += own ? v : 0.0f;
+              }
             }
           }
         }
-      }
+      if constexpr (MB > kPair) __builtin_amdgcn_sched_barrier(0);
     }
+  };
+  for (;;) {
+    for (int group = 0; group < layout.groups; ++group) {
+      if (both) products(std::false_type{}, group);
+      else products(std::true_type{}, group);
+    }
+    if (current[kBatch - 1] < 0) return;
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j) current[j] = next();
+    if (current[0] < 0) return;
   }
 }
 

@@ -146,6 +146,17 @@ double cost_of(const LinearParams &p, bool gated, const Cost &c) {
   return c.first + c.round * (rounds - 1.0) + per_stage * stages;
 }
 
+/// A shape's time where it is a product with adapters, or not to be chosen: up rows that the DMA cannot read do not go
+/// through the walk (bf16), and the largest f16 tiles spill sums where they add the adapters' (8192 x 4096 x 2048, ranks
+/// 16, 12 runs of rows: 256 x 256 tiles 160 us, 128 x 256 145).
+template <class T, class S, class P>
+double cost_with(const P &p, bool gated, const Cost &c) {
+  if constexpr (std::is_same<P, AdapterParams>::value && S::kSplit == 1 && S::kMB * S::kNB >= 8) {
+    if (std::is_same<T, F16>::value ? S::kMB * S::kNB > 16 : !p.up_whole) return 1e30;
+  }
+  return cost_of<S>(p, gated, c);
+}
+
 template <int kShapes>
 int cheapest(const double (&costs)[kShapes]) {
   int best = 0;
@@ -190,20 +201,20 @@ void launch(const P &p, hipStream_t stream) {
     }
   }
   const double costs[] = {
-      cost_of<Tile256>(p, kGated, {10.3, 9.4, 1.311}),
-      cost_of<Tile192x256>(p, kGated, {7.87, 7.8, 1.045}),
-      cost_of<Tile128x256>(p, kGated, {6.39, 5.74, 0.763}),
-      cost_of<Tile192x128>(p, kGated, {5.21, 4.98, 0.599}),
-      cost_of<Tile128>(p, kGated, {4.46, 2.07, 0.611, 0.436, 1.75}),
-      cost_of<Tile128Alone>(p, kGated, {4.5, 3.91, 0.434}),
-      cost_of<Tile96x128Alone>(p, kGated, {4.87, 3.98, 0.356}),
-      cost_of<Tile128x64Alone>(p, kGated, {4.06, 2.87, 0.28}),
-      cost_of<Tile64>(p, kGated, {3.67, 0.957, 0.184, 0.168, 1.9}),
-      cost_of<Tile48x64Alone>(p, kGated, {3.81, 2.54, 0.151}),
-      cost_of<Tile32x64Alone>(p, kGated, {3.51, 2.44, 0.118}),
-      cost_of<Tile32Alone>(p, kGated, {3.33, 2.17, 0.08}),
-      cost_of<Tile16x32Alone>(p, kGated, {3.22, 2.09, 0.06}),
-      kGated ? 1e30 : cost_of<Tile16>(p, kGated, {3.22, 0.707, 0.034, 0.038, 1.78}),
+      cost_with<T, Tile256>(p, kGated, {10.3, 9.4, 1.311}),
+      cost_with<T, Tile192x256>(p, kGated, {7.87, 7.8, 1.045}),
+      cost_with<T, Tile128x256>(p, kGated, {6.39, 5.74, 0.763}),
+      cost_with<T, Tile192x128>(p, kGated, {5.21, 4.98, 0.599}),
+      cost_with<T, Tile128>(p, kGated, {4.46, 2.07, 0.611, 0.436, 1.75}),
+      cost_with<T, Tile128Alone>(p, kGated, {4.5, 3.91, 0.434}),
+      cost_with<T, Tile96x128Alone>(p, kGated, {4.87, 3.98, 0.356}),
+      cost_with<T, Tile128x64Alone>(p, kGated, {4.06, 2.87, 0.28}),
+      cost_with<T, Tile64>(p, kGated, {3.67, 0.957, 0.184, 0.168, 1.9}),
+      cost_with<T, Tile48x64Alone>(p, kGated, {3.81, 2.54, 0.151}),
+      cost_with<T, Tile32x64Alone>(p, kGated, {3.51, 2.44, 0.118}),
+      cost_with<T, Tile32Alone>(p, kGated, {3.33, 2.17, 0.08}),
+      cost_with<T, Tile16x32Alone>(p, kGated, {3.22, 2.09, 0.06}),
+      kGated ? 1e30 : cost_with<T, Tile16>(p, kGated, {3.22, 0.707, 0.034, 0.038, 1.78}),
   };
   switch (cheapest(costs)) {
     case 0: return launch_tiles<T, kGated, true, Tile256>(p, stream);
@@ -222,6 +233,32 @@ void launch(const P &p, hipStream_t stream) {
     default:
       if constexpr (!kGated) return launch_tiles<T, kGated, true, Tile16>(p, stream);
   }
+}
+
+// ---- the adapters' first factor ---------------------------------------------------------------------------
+
+using Rank32x16 = TileShape<32, 16, 1, 1, 4, 4>;
+
+template <class T>
+void launch_low_rank(const AdapterParams &a, bool gated, hipStream_t stream) {
+  const LowLayout layout(a.rank);
+  RankParams p{};
+  static_cast<AdapterParams &>(p) = a;
+  p.width = layout.width, p.groups = layout.groups, p.halves = gated ? 2 : 1;
+  p.n = static_cast<int64_t>(p.halves) * layout.groups * layout.width;
+  const bool few = p.m <= 256;
+  const uint32_t shares = few ? static_cast<uint32_t>(p.m < 16 ? p.m : 16) : 1;
+  if (!p.down_by_dma) {
+    if (few) return launch_tiles<T, false, false, Any16x32>(p, stream, shares);
+    return launch_tiles<T, false, false, Any32>(p, stream, shares);
+  }
+  if (few) {
+    if (p.n <= 16) return launch_tiles<T, false, true, Tile16>(p, stream, shares);
+    return launch_tiles<T, false, true, Tile16x32Alone>(p, stream, shares);
+  }
+  if (p.n <= 16) return launch_tiles<T, false, true, Rank32x16>(p, stream, shares);
+  if (p.n <= 32) return launch_tiles<T, false, true, Tile32Alone>(p, stream, shares);
+  return launch_tiles<T, false, true, Tile32x64Alone>(p, stream, shares);
 }
 
 }  // namespace linear

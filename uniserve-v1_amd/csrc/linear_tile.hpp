@@ -93,7 +93,7 @@ __device__ __forceinline__ void wait_stages_but(int stages) {
 
 /// kDma: rows as p.by_dma says, whole 16-byte pieces, a tile's rows within 32-bit byte offsets. Else any rows:
 /// the stages come through registers, by 16-byte loads at any alignment, zeros past the rows' ends.
-/// P: LinearParams, or AdapterParams, whose rows' adapters are added to the sums behind the walk.
+/// P: LinearParams, or AdapterParams, whose rows' adapters are in the sums before the walk, while its first stages arrive.
 template <class T, bool kGated, bool kDma, class S, class P>
 __global__ void __launch_bounds__(S::kThreads) tile_kernel(P p) {
   using prefill::dma16;
@@ -115,6 +115,20 @@ __global__ void __launch_bounds__(S::kThreads) tile_kernel(P p) {
   const int64_t m0 = m_tile * S::kBM, n0 = n_tile * kCols;
   const int rows_left = static_cast<int>(p.m - m0 < S::kBM ? p.m - m0 : S::kBM);
   const int cols_left = static_cast<int>(p.n - n0 < kCols ? p.n - n0 : kCols);
+  constexpr bool kRanks = std::is_same<P, RankParams>::value;      // the adapters' first factor
+  constexpr bool kAdapters = std::is_same<P, AdapterParams>::value;  // a product with the second one's
+  // Where the second one's product is added: in the walk, as stages before K's; through LDS behind the walk; or, of small
+  // wavefront tiles, straight from memory before it.
+  constexpr bool kMany = kAdapters && S::kSplit == 1 && MB * NB >= 8;
+  constexpr bool kWalked = kMany && kDma && std::is_same<T, Bf16>::value;
+  constexpr bool kStaged = kMany && !kWalked;
+  [[maybe_unused]] __shared__ RowsAdapters<kMany ? S::kBM : 0, std::is_same<T, F16>::value> rows_adapters;
+  if constexpr (kMany) rows_adapters.load(p, m0);
+  [[maybe_unused]] typename std::conditional<kRanks, NamedAdapters, int>::type named = named_adapters(p, m0, S::kBM);
+  do {
+  if constexpr (kRanks) {
+    if (!named.next()) return;
+  }
 
   // ---- the loads: instruction i of wavefront w fills LDS rows 8 (w + kWaves i) .. + 7, first the tokens,
   // then the weights (rows past the edge repeat the last one; their sums are never stored). The weights'
@@ -127,31 +141,38 @@ __global__ void __launch_bounds__(S::kThreads) tile_kernel(P p) {
   const char *x_base = reinterpret_cast<const char *>(p.x + m0 * p.x_stride);
   const char *w_base = reinterpret_cast<const char *>(p.w + n0 * p.w_stride);
   auto chunk_of = [&](int i) { return (lane & 7) ^ ((lane >> 4) & 3) ^ (4 * ((wave + S::kWaves * i) & 1)); };
+  auto aim_at_k = [&]() {
 #pragma unroll
-  for (int i = 0; i < S::kLoads; ++i) {
-    const int first = 8 * (wave + S::kWaves * i);
-    const int r = first + lane / 8;
-    const bool token = i < S::kBM / 8 / S::kWaves;
-    int64_t at;
-    if (token) {
-      base[i] = x_base;
-      at = (r < rows_left ? r : rows_left - 1) * p.x_stride;
-    } else {
-      const int j = r - S::kBM;
-      const int of = j / (NB * 16), in = j % (NB * 16);
-      const int column = of * kWaveCols + (kGated ? in % kWaveCols : in);
-      const bool second = kGated && (first - S::kBM) % (NB * 16) >= kWaveCols;
-      base[i] = second ? w_base + p.n * p.w_stride * 2 : w_base;
-      at = (column < cols_left ? column : cols_left - 1) * p.w_stride;
+    for (int i = 0; i < S::kLoads; ++i) {
+      const int first = 8 * (wave + S::kWaves * i);
+      const int r = first + lane / 8;
+      const bool token = i < S::kBM / 8 / S::kWaves;
+      int64_t at;
+      if (token) {
+        base[i] = x_base;
+        if constexpr (kRanks) at = named.row(r) * p.x_stride;
+        else at = (r < rows_left ? r : rows_left - 1) * p.x_stride;
+      } else if constexpr (kRanks) {
+        base[i] = reinterpret_cast<const char *>(p.down + named.current * p.down_stride);
+        at = p.down_row(n0 + r - S::kBM) * p.down_row_stride;
+      } else {
+        const int j = r - S::kBM;
+        const int of = j / (NB * 16), in = j % (NB * 16);
+        const int column = of * kWaveCols + (kGated ? in % kWaveCols : in);
+        const bool second = kGated && (first - S::kBM) % (NB * 16) >= kWaveCols;
+        base[i] = second ? w_base + p.n * p.w_stride * 2 : w_base;
+        at = (column < cols_left ? column : cols_left - 1) * p.w_stride;
+      }
+      row_at[i] = reinterpret_cast<const uint16_t *>(base[i]) + at;
+      base[i] += team * kStageBytes;
+      offset[i] = static_cast<uint32_t>(at * 2) + chunk_of(i) * 16;
     }
-    row_at[i] = reinterpret_cast<const uint16_t *>(base[i]) + at;
-    base[i] += team * kStageBytes;
-    offset[i] = static_cast<uint32_t>(at * 2) + chunk_of(i) * 16;
-  }
+  };
+  if constexpr (!kWalked) aim_at_k();
   // The team's walk takes stages team, team + kSplit, .. of the row; the walks are equally long, and the last
   // stage of a walk holds all eight chunks of a row, the row's last few, or none.
   const int all_stages = static_cast<int>(ceil_div<int64_t>(p.k, kStageK));
-  const int stages = (all_stages + S::kSplit - 1) / S::kSplit;
+  int stages = (all_stages + S::kSplit - 1) / S::kSplit;
   const int last_stage = (stages - 1) * S::kSplit + team;
   const int row_chunks = static_cast<int>(p.k / 8);
   const int last_chunks = !kDma ? 8 : last_stage >= all_stages ? 0 : (row_chunks - last_stage * 8 < 8 ? row_chunks - last_stage * 8 : 8);
@@ -172,6 +193,63 @@ __global__ void __launch_bounds__(S::kThreads) tile_kernel(P p) {
 #pragma unroll
     for (int i = 0; i < S::kLoads; ++i) base[i] += S::kSplit * kStageBytes;
     to = to + S::kRows * kStageBytes == ring_lds + S::kLdsBytes ? ring_lds : to + S::kRows * kStageBytes;
+  };
+
+  // kWalked: the walk's first stages are 32 ranks of one adapter each (gated: of one half's factors), `values, errors`
+  // against twice the same ranks of the up rows. Zeros, a row's padding, stand for the rows of other adapters, for
+  // the other half's weight rows and for a stage's chunks past the values; where a piece of an up row ends, its first
+  // chunk comes again (against zeros).
+  [[maybe_unused]] typename std::conditional<kWalked, NamedAdapters, int>::type adapter_stages = tile_adapters<kWalked>(rows_adapters, S::kBM);
+  [[maybe_unused]] bool mixed = false;  // rows without an adapter, or several adapters
+  [[maybe_unused]] int adapted = 0, stage_group = 0, stage_half = 0;
+  if constexpr (kWalked) {
+    __syncthreads();
+    adapter_stages.find(rows_adapters.id);
+    const LowLayout layout(p.rank);
+    const int named_ones = adapter_stages.count(rows_left, mixed);
+    adapted = named_ones * layout.groups * (kGated ? 2 : 1);
+    stages += adapted;
+    stage_group = layout.groups;
+  }
+  [[maybe_unused]] auto aim = [&](int s) {
+    if constexpr (kWalked) {
+      if (s > adapted) return;
+      if (s == adapted) return aim_at_k();
+      const LowLayout layout(p.rank);
+      if (stage_group == layout.groups) {
+        stage_group = 0;
+        if (stage_half == 1 || !kGated || adapter_stages.current < 0) {
+          stage_half = 0;
+          adapter_stages.next();
+        } else {
+          stage_half = 1;
+        }
+      }
+      const int row_bytes = static_cast<int>(layout.row_bytes(kGated ? 2 : 1));
+      const char *low = p.low + m0 * row_bytes + static_cast<int64_t>(stage_half * layout.groups + stage_group) * layout.group_bytes();
+      const uint16_t *up = p.up + adapter_stages.current * p.up_stride + (n0 + stage_half * p.n) * p.up_row_stride + stage_group * 32;
+      const uint32_t zeros = static_cast<uint32_t>(adapter_stages.first_row() * row_bytes + 4 * layout.width);
+      const int chunks = p.rank - stage_group * 32 < layout.width ? (p.rank - stage_group * 32) / 8 : layout.width / 8;
+#pragma unroll
+      for (int i = 0; i < S::kLoads; ++i) {
+        const int first = 8 * (wave + S::kWaves * i);
+        const int r = first + lane / 8, c = chunk_of(i);
+        if (i < S::kBM / 8 / S::kWaves) {
+          base[i] = low;
+          offset[i] = 4 * c < layout.width && rows_adapters.id[r] == adapter_stages.current ? static_cast<uint32_t>(r * row_bytes + 16 * c) : zeros;
+        } else {
+          const int j = r - S::kBM;
+          const int of = j / (NB * 16), in = j % (NB * 16);
+          const int column = of * kWaveCols + (kGated ? in % kWaveCols : in);
+          const int half = kGated && (first - S::kBM) % (NB * 16) >= kWaveCols ? 1 : 0;
+          const int chunk = c % (layout.width / 8);
+          const uint32_t at = static_cast<uint32_t>(column < cols_left ? column : cols_left - 1) * static_cast<uint32_t>(p.up_row_stride);
+          base[i] = half == stage_half ? reinterpret_cast<const char *>(up) : low;
+          offset[i] = half == stage_half ? at * 2 + (chunk < chunks ? chunk : 0) * 16 : zeros;
+        }
+      }
+      ++stage_group;
+    }
   };
 
   floatx4 acc[NB][MB];
@@ -261,10 +339,13 @@ __global__ void __launch_bounds__(S::kThreads) tile_kernel(P p) {
   constexpr int kBehind = (S::kStages - 2) * S::kLoads;
   static_assert(kBehind + S::kLoads < 64, "vmcnt holds 6 bits");
   constexpr int kWaitLds = 0xc07f;  // lgkmcnt 0, nothing else
+  [[maybe_unused]] typename std::conditional<kAdapters && !kMany, RowAdapters<MB>, int>::type adapters =
+      row_adapters<MB, kMany>(p, m0 + wave_m * MB * 16);
 #pragma unroll
   for (int s = 0; s < S::kStages; ++s) {
     if constexpr (kDma) {
       if (s < stages) {
+        aim(s);
         if (s == stages - 1) begin_stage();
 #pragma unroll
         for (int i = 0; i < S::kLoads; ++i) issue(i);
@@ -275,6 +356,8 @@ __global__ void __launch_bounds__(S::kThreads) tile_kernel(P p) {
       put(s);
     }
   }
+  if constexpr (kAdapters && !kMany)
+    add_low_rank<T, kGated>(p, acc, adapters, m0 + wave_m * MB * 16, n0 + wave_n * kWaveCols, team, S::kSplit);
   if constexpr (kDma) {
     wait_stages_but<S::kStages - 1, S::kLoads>(stages - 1);
   } else {
@@ -301,6 +384,14 @@ __global__ void __launch_bounds__(S::kThreads) tile_kernel(P p) {
   };
   int k = 0;
   if constexpr (kDma) {
+    if constexpr (kWalked) {
+      for (; k + S::kStages <= adapted; ++k) {  // the next loads are an adapter's, or K's first
+        step(no, 0);
+        aim(k + S::kStages);
+        if (k + S::kStages == stages - 1) begin_stage();
+        multiply(second_half, yes, yes, buffer);
+      }
+    }
     for (; k + S::kStages < stages - 1; ++k) {  // the next loads are not the walk's last
       step(no, 0);
       multiply(second_half, yes, yes, buffer);
@@ -320,8 +411,108 @@ __global__ void __launch_bounds__(S::kThreads) tile_kernel(P p) {
   multiply(first_half, yes, no, buffer);
   if (last_chunks < 8) mask(second_half);
   multiply(second_half, no, no, 0);
-  if constexpr (std::is_same<P, AdapterParams>::value)
-    add_low_rank<T, kGated>(p, acc, m0 + wave_m * MB * 16, n0 + wave_n * kWaveCols, team, S::kSplit);
+  if constexpr (kStaged) {
+    // Stage by stage, as above, but multiplied apart from the sums and added to them where a row names the adapter: f16
+    // rows have a factor each, and stages through registers need no padding.
+    const LowLayout layout(p.rank);
+    constexpr int kHalves = kGated ? 2 : 1;
+    NamedAdapters tile(S::kBM);
+    __syncthreads();  // the ring has been read
+    tile.find(rows_adapters.id);
+    const bool wide = layout.width == 32;
+    int buffer_of = 0;
+    auto stage = [&](auto half_of, int group) {
+      constexpr int h = decltype(half_of)::value;
+      const int part = h * layout.groups + group;
+      const char *low = p.low + m0 * layout.row_bytes(kHalves) + static_cast<int64_t>(part) * layout.group_bytes();
+      const uint16_t *up = p.up + tile.current * p.up_stride + (n0 + h * p.n) * p.up_row_stride + group * 32;
+      // (opaque: what the lanes' addresses share from stage to stage is not kept, the sums need the registers)
+      int l = lane;
+      asm volatile("" : "+v"(l));
+      constexpr int kAtOnce = S::kLoads < 8 ? S::kLoads : 8;
+#pragma unroll
+      for (int from = 0; from < S::kLoads; from += kAtOnce) {
+        u32x4 pieces[kAtOnce];
+#pragma unroll
+        for (int u = 0; u < kAtOnce; ++u) {
+          const int i = from + u;
+          if (i >= S::kLoads) continue;
+          const int r = 8 * (wave + S::kWaves * i) + l / 8, c = (l & 7) ^ ((l >> 4) & 3) ^ (4 * ((wave + S::kWaves * i) & 1));
+          const bool filled = 4 * c < layout.width;
+          pieces[u] = u32x4{0, 0, 0, 0};
+          if (i < S::kBM / 8 / S::kWaves) {
+            const uint32_t row = static_cast<uint32_t>(r < rows_left ? r : rows_left - 1);
+            if (filled)
+              pieces[u] = *reinterpret_cast<const u32x4 *>(low + (row * static_cast<uint32_t>(layout.row_bytes(kHalves)) + 16 * c));
+          } else {
+            const int j = r - S::kBM;
+            const int of = j / (NB * 16), in = j % (NB * 16);
+            int column = of * kWaveCols + (kGated ? in % kWaveCols : in);
+            column = column < cols_left ? column : cols_left - 1;
+            const int at = (wide ? c & 3 : layout.width == 16 ? c & 1 : 0) * 8;
+            if (p.up_whole) {
+              if (filled && group * 32 + at < p.rank)
+                pieces[u] = *reinterpret_cast<const u32x4 *>(up + (static_cast<uint32_t>(column) * static_cast<uint32_t>(p.up_row_stride) + at));
+            } else if (filled) {
+              pieces[u] = load8(up + column * p.up_row_stride, at, p.rank - group * 32);
+            }
+          }
+        }
+#pragma unroll
+        for (int u = 0; u < kAtOnce; ++u)
+          if (from + u < S::kLoads) ring[buffer_of][(wave + S::kWaves * (from + u)) * 64 + l] = pieces[u];
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      if constexpr (std::is_same<T, F16>::value) rows_adapters.load_factors(p, m0, buffer_of, layout, kHalves, part);
+      // Two buffers in turn: one barrier a stage (a wavefront writes the other one only after all have read it).
+      __syncthreads();
+      // Both halves of the stage, zeros up to rank 16 (two ways through here would cost registers, and spill sums).
+      const u32x4 *rows = ring[buffer_of];
+      constexpr int kRowsAtOnce = MB % 4 == 0 ? 4 : MB;
+#pragma unroll
+      for (int mb = 0; mb < MB; mb += kRowsAtOnce) {
+        u32x4 x0[kRowsAtOnce], x1[kRowsAtOnce];
+        bool own[kRowsAtOnce];
+        float factor[kRowsAtOnce];
+#pragma unroll
+        for (int j = 0; j < kRowsAtOnce; ++j) {
+          const int row = (wave_m * MB + mb + j) * 16 + r16;
+          x0[j] = rows[tile_slot(x_row, g) + (mb + j) * 128];
+          x1[j] = rows[tile_slot(x_row, 4 + g) + (mb + j) * 128];
+          own[j] = rows_adapters.id[row] == tile.current;
+          factor[j] = 1.0f;
+          if constexpr (std::is_same<T, F16>::value) factor[j] = rows_adapters.factor[buffer_of][row];
+        }
+#pragma unroll
+        for (int nb = h * (NB / kHalves); nb < (h + 1) * (NB / kHalves); ++nb) {
+          const u32x4 w0 = rows[tile_slot(w_row, g) + nb * 128], w1 = rows[tile_slot(w_row, 4 + g) + nb * 128];
+          floatx4 sum[kRowsAtOnce];
+#pragma unroll
+          for (int j = 0; j < kRowsAtOnce; ++j) sum[j] = T::mfma(w0, x0[j], floatx4{0.0f, 0.0f, 0.0f, 0.0f});
+#pragma unroll
+          for (int j = 0; j < kRowsAtOnce; ++j) sum[j] = T::mfma(w1, x1[j], sum[j]);
+#pragma unroll
+          for (int j = 0; j < kRowsAtOnce; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float v = std::is_same<T, F16>::value ? sum[j][e] * factor[j] : sum[j][e];
+              acc[nb][mb + j][e] += own[j] ? v : 0.0f;
+            }
+        }
+        asm volatile("" ::: "memory");  // (the weights are read again, not kept)
+      }
+      buffer_of ^= 1;
+    };
+    for (int group = layout.groups;; ++group) {  // (one loop, not two: that costs registers, too)
+      if (group == layout.groups) {
+        if (!tile.next()) break;
+        group = 0;
+      }
+      stage(first_half, group);
+      if constexpr (kGated) stage(second_half, group);
+    }
+    __syncthreads();
+  }
 
   // ---- the epilogue: each wavefront passes its sums through its own part of the ring (no longer read by
   // anyone), kPassMB token blocks at a time, so that a lane then holds eight consecutive columns of a
@@ -337,7 +528,7 @@ __global__ void __launch_bounds__(S::kThreads) tile_kernel(P p) {
   auto at_chunk = [&](int row, int c) { return row * kRowChunks + (c ^ (row & (kRowChunks < 16 ? kRowChunks - 1 : 15))); };
   const int group = lane % kGroups;
   const int64_t n = n0 + wave_n * kWaveCols + group * 8;
-  const Columns8<T, kGated> columns(p, n);
+  [[maybe_unused]] const typename std::conditional<kRanks, RankColumns<T>, Columns8<T, kGated>>::type columns(p, n);
 #pragma unroll
   for (int pass = 0; pass < MB / kPassMB; ++pass) {
 #pragma unroll
@@ -358,7 +549,7 @@ __global__ void __launch_bounds__(S::kThreads) tile_kernel(P p) {
 #pragma unroll
       for (int j = 0; j < kBatch; ++j) m[j] = m_first + first + j * kStep < p.m ? m_first + first + j * kStep : p.m - 1;
       typename Columns8<T, kGated>::template Extras<kBatch> extras;
-      columns.load(p, m, n, extras);
+      if constexpr (!kRanks) columns.load(p, m, n, extras);
 #pragma unroll
       for (int j = 0; j < kBatch; ++j) {
         const int row = first + j * kStep;
@@ -376,10 +567,19 @@ __global__ void __launch_bounds__(S::kThreads) tile_kernel(P p) {
             if constexpr (kGated) gates[i] += __builtin_bit_cast(floatx4, sums[other * kTeamChunks + d]);
           }
         }
-        columns.finish(p, m[j], n, v, gates, extras.residual[j], extras.factor[j]);
+        if constexpr (kWalked) {
+          if (mixed) remake<T, kGated>(p, m[j], n, rows_adapters.id[static_cast<int>(m[j] - m0)], v, gates);
+        }
+        if constexpr (kRanks) {
+          if (named.holds(static_cast<int>(m[j] - m0))) columns.finish(p, m[j], named.current, v);
+        } else {
+          columns.finish(p, m[j], n, v, gates, extras.residual[j], extras.factor[j]);
+        }
       }
     }
   }
+  if constexpr (kRanks) __syncthreads();  // the ring is free again
+  } while (kRanks);
 }
 
 template <class S>
@@ -388,8 +588,8 @@ int64_t tiles_of(const LinearParams &p, bool gated) {
 }
 
 template <class T, bool kGated, bool kDma, class S, class P>
-void launch_tiles(const P &p, hipStream_t stream) {
-  hipLaunchKernelGGL((tile_kernel<T, kGated, kDma, S, P>), dim3(static_cast<uint32_t>(tiles_of<S>(p, kGated))), dim3(S::kThreads), 0,
+void launch_tiles(const P &p, hipStream_t stream, uint32_t shares = 1) {
+  hipLaunchKernelGGL((tile_kernel<T, kGated, kDma, S, P>), dim3(static_cast<uint32_t>(tiles_of<S>(p, kGated)), shares), dim3(S::kThreads), 0,
                      stream, p);
 }
 
