@@ -26,6 +26,7 @@ from .abi import (  # noqa: F401
     RouteCall,
     RouteFp8Call,
     SortCall,
+    TokenExpertsCall,
     UnpermuteCall,
     LAYOUT_EXPANDED,
     LAYOUT_PERMUTED,

@@ -467,6 +467,34 @@ class AdapterLinearCall(ctypes.Structure):
     ]
 
 
+class TokenExpertsCall(ctypes.Structure):
+    """``uniserve_token_experts_call``."""
+
+    _fields_ = [
+        ("input", _P),
+        ("ids", _P),
+        ("weights", _P),
+        ("up_gate", _P),
+        ("down", _P),
+        ("residual", _P),
+        ("out", _P),
+        ("workspace", _P),
+        ("workspace_bytes", _I64),
+        ("tokens", _I64),
+        ("top", _I64),
+        ("hidden", _I64),
+        ("width", _I64),
+        ("experts", _I64),
+        ("first_expert", _I64),
+        ("input_row_stride", _I64),
+        ("residual_row_stride", _I64),
+        ("out_row_stride", _I64),
+        ("dtype", ctypes.c_int32),
+        ("activation", ctypes.c_int32),
+        ("error", _ERR),
+    ]
+
+
 def max_tiles(tokens, top, local_experts, tile=128):
     """``ops::moe::max_tiles`` (crates/ops/src/moe/mod.rs:63-70)."""
     expanded = tokens * top
@@ -517,6 +545,7 @@ _ENTRIES = {
     "uniserve_linear": LinearCall,
     "uniserve_gated_linear": LinearCall,
     "uniserve_add_norm": AddNormCall,
+    "uniserve_token_experts": TokenExpertsCall,
     "uniserve_adapter_linear": AdapterLinearCall,
     "uniserve_adapter_gated_linear": AdapterLinearCall,
 }
@@ -552,6 +581,8 @@ def library():
     lib.uniserve_moe_layer_step.restype = ctypes.c_int32
     lib.uniserve_moe_layer_views_of.argtypes = [_I64] * 6 + [ctypes.POINTER(LayerViews)]
     lib.uniserve_moe_layer_views_of.restype = ctypes.c_int32
+    lib.uniserve_token_experts_workspace.argtypes = [_I64] * 3
+    lib.uniserve_token_experts_workspace.restype = _I64
     lib.uniserve_adapter_workspace.argtypes = [_I64] * 2
     lib.uniserve_adapter_workspace.restype = _I64
     lib.uniserve_moe_max_tiles.argtypes = [_I64] * 4

@@ -36,6 +36,7 @@ from .abi import (
     RouteCall,
     RouteFp8Call,
     SortCall,
+    TokenExpertsCall,
     UnpermuteCall,
     library,
     max_tiles,
@@ -474,6 +475,60 @@ def moe_unpermute(products, expanded_to_permuted, weights, out=None, layout=LAYO
     call.output_dtype = DTYPE[_TORCH_DTYPE[out.dtype]]
     call.layout = layout
     _check(library().uniserve_moe_unpermute(ctypes.byref(call), _stream(products.device)), call, "moe_unpermute")
+    return out
+
+
+def token_experts_workspace(tokens, top, width):
+    """The bytes of ``token_experts``' workspace."""
+    return library().uniserve_token_experts_workspace(tokens, top, width)
+
+
+def token_experts(x, ids, weights, up_gate, down, activation="silu", residual=None, first=0, out=None, workspace=None):
+    """The routed experts of a layer for up to 64 tokens, in two kernels: ``residual[t] + sum_k weights[t, k] *
+    (act(x[t] @ gate.T) * (x[t] @ up.T)) @ down[e].T`` with ``e = ids[t, k] - first``, ``x`` ``[T, H]`` bf16 or f16,
+    ``up_gate`` ``[E, 2 I, H]`` (an expert's up rows, then its gate rows) and ``down`` ``[E, H, I]`` of its type and
+    ``ids`` (int32), ``weights`` (f32) ``[T, top]`` as ``topk_softmax`` and ``expert_topk`` give them. Routes outside the
+    stacks (-1, other ranks') add nothing. FP32 within, gated values held to 16 bits, one rounding into the
+    output. ``residual`` is ``[T, H]`` of ``x``'s type, ``out`` may be the residual itself.
+
+    ``workspace``: ``token_experts_workspace(T, top, I)`` bytes, for one call at a time; None allocates them."""
+    dtype, index = x.dtype, x.get_device()
+    if x.dim() != 2 or dtype not in _PRODUCT or index < 0:
+        raise ValueError("token_experts: the input is [tokens, hidden] of bf16 or f16 on a GPU")
+    if activation not in ACTIVATION:
+        raise ValueError(f"token_experts: activation is silu or gelu_tanh, got {activation!r}")
+    tokens, hidden = x.shape
+    if up_gate.dim() != 3 or up_gate.shape[1] % 2 != 0:
+        raise ValueError("token_experts: up_gate is [experts, 2 width, hidden], the up rows and then the gate rows")
+    experts, width = up_gate.shape[0], up_gate.shape[1] // 2
+    for stack, shape, what in ((up_gate, (experts, 2 * width, hidden), "up_gate"), (down, (experts, hidden, width), "down")):
+        if tuple(stack.shape) != shape or stack.dtype != dtype or stack.get_device() != index or not stack.is_contiguous():
+            raise ValueError(f"token_experts: {what} is {list(shape)} of {dtype} on device {index}, contiguous")
+    top = ids.shape[1] if ids.dim() == 2 else 0
+    for routes, kind, what in ((ids, torch.int32, "ids"), (weights, torch.float32, "weights")):
+        if routes.shape != (tokens, top) or routes.dtype != kind or routes.get_device() != index or not routes.is_contiguous():
+            raise ValueError(f"token_experts: {what} are [tokens, top] of {kind} on device {index}, contiguous")
+    x_stride = _matrix(x, tokens, hidden, index, "token_experts", "the input")
+    residual_at, residual_stride = None, 0
+    if residual is not None:
+        if residual.dtype != dtype:
+            raise ValueError("token_experts: the residual is of the input's type")
+        residual_at, residual_stride = residual.data_ptr(), _matrix(residual, tokens, hidden, index, "token_experts", "the residual")
+    if out is None:
+        out, out_stride = x.new_empty(tokens, hidden), hidden
+    else:
+        if out.dtype != dtype:
+            raise ValueError("token_experts: the output is of the input's type")
+        out_stride = _matrix(out, tokens, hidden, index, "token_experts", "the output")
+    if workspace is None:
+        workspace = torch.empty(token_experts_workspace(tokens, top, width), dtype=torch.uint8, device=x.device)
+    elif workspace.get_device() != index or not workspace.is_contiguous():
+        raise ValueError(f"token_experts: the workspace is contiguous, on device {index}")
+    call = TokenExpertsCall(x.data_ptr(), ids.data_ptr(), weights.data_ptr(), up_gate.data_ptr(), down.data_ptr(), residual_at,
+                            out.data_ptr(), workspace.data_ptr(), workspace.numel() * workspace.element_size(), tokens, top,
+                            hidden, width, experts, first, x_stride, residual_stride, out_stride, _ELEMENT[dtype],
+                            ACTIVATION[activation])
+    _enter(library().uniserve_token_experts, call, index, "token_experts")
     return out
 
 
