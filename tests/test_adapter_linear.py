@@ -348,6 +348,27 @@ def test_infinities_and_nans_stay_with_their_adapter(device, m, rank, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("gated, shape, m, n, k", [case for case in KERNELS if "2,4," in case[1] or "128,128" in case[1] or "96,128" in case[1]])
+@pytest.mark.parametrize("rank", [8, 40])
+def test_infinities_and_nans_in_large_tiles(device, gated, shape, m, n, k, rank):
+    """Tiles of rows of several adapters, one with up rows that are not finite: the others' rows are as without it."""
+    announce("adapter non-finite tiles", shape, gated, m, n, k, rank)
+    halves = 2 if gated else 1
+    entry = ops.adapter_gated_linear if gated else ops.adapter_linear
+    x, w, adapter = normal((m, k), 1), normal((n * halves, k), 2, 0.05), runs(m, 4)
+    call = dict(stacks(4, rank, n, k, halves=halves), adapter=adapter)
+    want, tolerance = reference(x, w, **call, activation="silu" if gated else None, gated=gated)
+    call["up"][2, 5], call["up"][2, n * halves - 1, rank - 1] = float("nan"), float("inf")
+    got = entry(x, w, **call).double().cpu()
+    clean = adapter.cpu() != 2
+    assert clean.any() and ((got[clean] - want[clean]).abs() <= tolerance[clean]).all()
+    touched = ~clean
+    assert not torch.isfinite(got[touched][:, [5, n - 1]]).any()
+    kept = [c for c in range(n) if c not in (5, n - 1)]
+    assert ((got[touched][:, kept] - want[touched][:, kept]).abs() <= tolerance[touched][:, kept]).all()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("m", [1, 40, 300])
 @pytest.mark.parametrize("size", [2.0**-20, 2.0**-10, 2.0**9])
 def test_f16_rank_values_of_any_size(device, m, size):

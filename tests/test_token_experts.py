@@ -76,7 +76,7 @@ REFUSED = [
     ({"out": None}, "needs"), ({"workspace": None}, "needs"),
     ({"input_row_stride": 63}, "strides"), ({"out_row_stride": 63}, "strides"), ({"residual": 9 << 20, "residual_row_stride": 1}, "strides"),
     ({"out_row_stride": 1 << 60}, "too large"), ({"hidden": (1 << 24) - 1, "width": (1 << 24) - 1, "input_row_stride": 1 << 24, "out_row_stride": 1 << 24}, "too large"),
-    ({"workspace_bytes": 16 + 8 * (32 + 256) - 1}, "workspace of"), ({"workspace": (7 << 20) + 8}, "aligned"),
+    ({"workspace_bytes": 16 + 8 * (16 + 256) - 1}, "workspace of"), ({"workspace": (7 << 20) + 8}, "aligned"),
     ({"out": 1 << 20}, "output overlaps"), ({"out": 2 << 20}, "output overlaps"), ({"out": (3 << 20) + 16}, "output overlaps"),
     ({"out": (4 << 20) + 64}, "output overlaps"), ({"out": (5 << 20) - 32}, "output overlaps"),
     ({"workspace": 1 << 20}, "workspace overlaps one"), ({"workspace": 2 << 20}, "workspace overlaps one"), ({"workspace": 5 << 20}, "workspace overlaps one"),
@@ -112,7 +112,7 @@ def test_no_rows_launch_nothing():
 
 def test_workspace_sizes():
     size = ops.token_experts_workspace
-    assert size(1, 1, 1) == 16 + 32 + 256 and size(4, 2, 64) == 16 + 8 * (32 + 256) and size(64, 8, 768) == 16 + 512 * (32 + 4 * 768)
+    assert size(1, 1, 1) == 16 + 16 + 256 and size(4, 2, 64) == 16 + 8 * (16 + 256) and size(64, 8, 768) == 16 + 512 * (16 + 4 * 768)
     assert size(0, 8, 64) == 0 and size(65, 8, 64) == 0 and size(4, 33, 64) == 0
 
 
@@ -137,7 +137,8 @@ def inputs(tokens, hidden, width, experts, top, dtype=BF16, seed=0):
 #: tokens, hidden, width, experts, top: single ones, odd extents, whole lines and their remainders, few and many experts.
 SHAPES = [(1, 1, 1, 1, 1), (1, 2048, 768, 16, 8), (1, 64, 64, 4, 2), (2, 72, 40, 5, 3), (3, 100, 33, 7, 7), (5, 256, 704, 8, 6),
           (7, 520, 136, 64, 8), (15, 1000, 72, 3, 2), (16, 128, 128, 16, 4), (17, 130, 65, 2, 1), (31, 264, 192, 128, 8),
-          (33, 64, 256, 300, 5), (64, 512, 128, 128, 8), (64, 96, 320, 1, 1), (64, 200, 64, 2, 2), (48, 128, 96, 1024, 32), (64, 64, 63, 40, 32)]
+          (33, 64, 256, 300, 5), (64, 512, 128, 128, 8), (64, 96, 320, 1, 1), (64, 200, 64, 2, 2), (48, 128, 96, 1024, 32), (64, 64, 63, 40, 32),
+          (4, 2120, 72, 6, 2), (20, 2051, 64, 8, 2), (64, 2056, 40, 6, 2), (3, 4100, 193, 9, 4), (64, 2600, 72, 64, 4)]
 
 
 @pytest.mark.gpu

@@ -25,11 +25,12 @@ constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / kWave;
 constexpr int kMostTokens = UNISERVE_TOKEN_EXPERTS_MAX_TOKENS;
 constexpr int kMostExperts = UNISERVE_TOKEN_EXPERTS_MAX_EXPERTS;
-constexpr int kJobTokens = 16;
+constexpr int kMostRoutes = kMostTokens * UNISERVE_TOKEN_EXPERTS_MAX_TOP;
 constexpr int kLine = 64;  // elements
 
 struct Job {
-  int32_t expert, first, count, unused;  ///< entries first .. first + count - 1
+  uint16_t expert, count;
+  int32_t first;  ///< entries first .. first + count - 1
 };
 /// A token of a job: its first route to the expert, and the weights of all of them.
 struct Entry {
@@ -45,19 +46,27 @@ struct Params {
   int32_t *job_count;
   Job *jobs;
   Entry *entries;
-  uint16_t *gated;  ///< [routes, 2, padded]: values, then errors
+  uint16_t *gated;  ///< [routes, lines, 2, 64]: a line's values, then their errors
   int64_t x_stride, residual_stride, out_stride;
   int32_t tokens, top, routes, hidden, width, padded, experts, first_expert, activation;
+  int32_t job_tokens;  ///< the most of a job: 4, 8 or 16
 };
 
 /// Values of f16 pairs are held at this part of themselves.
 template <class T>
 constexpr float kHeld = std::is_same<T, F16>::value ? 0.015625f : 1.0f;
 
+/// Eight elements of a row from `at` on, zeros past its end; kWhole: rows of whole 16-byte pieces.
 template <bool kWhole>
 __device__ __forceinline__ u32x4 piece_of(const uint16_t *row, int64_t at, int64_t width) {
   if constexpr (kWhole) return at < width ? *reinterpret_cast<const u32x4 *>(row + at) : u32x4{0, 0, 0, 0};
   else return load8(row, at, width);
+}
+/// Eight elements of a weight row; kOnce: not kept in the caches.
+template <bool kWhole, bool kOnce>
+__device__ __forceinline__ u32x4 weights_of(const uint16_t *row, int64_t at, int64_t width) {
+  if constexpr (kWhole && kOnce) return at < width ? __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(row + at)) : u32x4{0, 0, 0, 0};
+  else return piece_of<kWhole>(row, at, width);
 }
 
 /// An id's expert in the stacks, or -1.
@@ -69,16 +78,18 @@ __device__ __forceinline__ int expert_of(const Params &p, int id) {
 /// Where the routes lead: the tokens that name each expert, and how many tokens and jobs come before it.
 struct Routing {
   uint64_t tokens[kMostExperts];
+  int16_t experts[kMostRoutes];  ///< of each route, or -1
   uint16_t entries_before[kMostExperts], jobs_before[kMostExperts];
   int32_t wave_entries[kWaves], wave_jobs[kWaves];
   int32_t jobs;
 
   /// Every thread of the workgroup calls it.
   __device__ __forceinline__ void find(const Params &p) {
+    for (int q = threadIdx.x; q < p.routes; q += kThreads) experts[q] = static_cast<int16_t>(expert_of(p, p.ids[q]));
     for (int e = threadIdx.x; e < p.experts; e += kThreads) tokens[e] = 0;
     __syncthreads();
     for (int q = threadIdx.x; q < p.routes; q += kThreads) {
-      const int e = expert_of(p, p.ids[q]);
+      const int e = experts[q];
       if (e >= 0) atomicOr(reinterpret_cast<unsigned long long *>(&tokens[e]), 1ull << (q / p.top));
     }
     __syncthreads();
@@ -89,7 +100,7 @@ struct Routing {
     for (int e = begin; e < begin + each && e < p.experts; ++e) {
       const int count = __popcll(tokens[e]);
       own_entries += count;
-      own_jobs += (count + kJobTokens - 1) / kJobTokens;
+      own_jobs += (count + p.job_tokens - 1) / p.job_tokens;
     }
     int entries = own_entries, upto = own_jobs;
 #pragma unroll
@@ -111,7 +122,7 @@ struct Routing {
       entries_before[e] = static_cast<uint16_t>(entries), jobs_before[e] = static_cast<uint16_t>(upto);
       const int count = __popcll(tokens[e]);
       entries += count;
-      upto += (count + kJobTokens - 1) / kJobTokens;
+      upto += (count + p.job_tokens - 1) / p.job_tokens;
     }
     __syncthreads();
   }
@@ -119,50 +130,52 @@ struct Routing {
   __device__ __forceinline__ void write_job(const Params &p, int n, Job *job) const {
     for (int e = threadIdx.x; e < p.experts; e += kThreads) {
       const int count = __popcll(tokens[e]), run = n - jobs_before[e];
-      if (run < 0 || run * kJobTokens >= count) continue;
-      const int left = count - run * kJobTokens;
-      *job = Job{e, entries_before[e] + run * kJobTokens, left < kJobTokens ? left : kJobTokens, 0};
+      if (run < 0 || run * p.job_tokens >= count) continue;
+      const int left = count - run * p.job_tokens;
+      *job = Job{static_cast<uint16_t>(e), static_cast<uint16_t>(left < p.job_tokens ? left : p.job_tokens), entries_before[e] + run * p.job_tokens};
     }
   }
-  /// Route q's place among the entries and its weight, if it is its token's first to the expert; else place -1.
-  __device__ __forceinline__ int place(const Params &p, int q, float &weight) const {
-    const int id = p.ids[q], e = expert_of(p, id);
-    if (e < 0) return -1;
-    const int t = q / p.top;
-    weight = p.weights[q];
-    for (int k = t * p.top; k < (t + 1) * p.top; ++k) {
-      if (k == q || p.ids[k] != id) continue;
-      if (k < q) return -1;
-      weight += p.weights[k];
-    }
-    return entries_before[e] + __popcll(tokens[e] & ((1ull << t) - 1));
+  /// Whether route q is its token's first to its expert.
+  __device__ __forceinline__ bool first(const Params &p, int q) const {
+    const int start = q / p.top * p.top;
+    bool before = false;
+    for (int k = start; k < q; ++k) before = before || experts[k] == experts[q];
+    return experts[q] >= 0 && !before;
+  }
+  /// Its place among the entries.
+  __device__ __forceinline__ int place(const Params &p, int q) const {
+    const int e = experts[q];
+    return entries_before[e] + __popcll(tokens[e] & ((1ull << (q / p.top)) - 1));
   }
 };
 
 // ---- up and gate ------------------------------------------------------------------------------------------
 
 /// kCols gated columns of one job a workgroup; a wavefront takes a quarter of K's lines.
-template <class T, bool kWhole, int kCols>
+template <class T, bool kWhole, bool kOnce, int kCols>
 __global__ void __launch_bounds__(kThreads) gate_up_kernel(Params p) {
   constexpr int kGroups = 2 * kCols / 8;   // of eight weight rows, the up rows' and then the gate rows'
   constexpr int kBlocks = 2 * kCols / 16;  // of sixteen
   __shared__ Routing routing;
   __shared__ Job job;
-  __shared__ int32_t job_route[kJobTokens];
+  __shared__ int32_t job_route[16];
   __shared__ u32x4 regroup[kWaves][kGroups * 64];
   routing.find(p);
   const int n = static_cast<int>(blockIdx.y);
   if (n == 0 && blockIdx.x == 0) {
-    for (int i = threadIdx.x; i < p.routes; i += kThreads) {
-      float weight;
-      const int at = routing.place(p, i, weight);
-      if (at >= 0) p.entries[at] = Entry{i, weight};
+    for (int q = threadIdx.x; q < p.routes; q += kThreads) {
+      if (!routing.first(p, q)) continue;
+      float weight = p.weights[q];
+      for (int k = q + 1; k < (q / p.top + 1) * p.top; ++k)
+        if (routing.experts[k] == routing.experts[q]) weight += p.weights[k];
+      p.entries[routing.place(p, q)] = Entry{q, weight};
     }
     for (int e = threadIdx.x; e < p.experts; e += kThreads) {
       const int count = __popcll(routing.tokens[e]);
-      for (int run = 0; run * kJobTokens < count; ++run) {
-        const int left = count - run * kJobTokens;
-        p.jobs[routing.jobs_before[e] + run] = Job{e, routing.entries_before[e] + run * kJobTokens, left < kJobTokens ? left : kJobTokens, 0};
+      for (int run = 0; run * p.job_tokens < count; ++run) {
+        const int left = count - run * p.job_tokens;
+        p.jobs[routing.jobs_before[e] + run] =
+            Job{static_cast<uint16_t>(e), static_cast<uint16_t>(left < p.job_tokens ? left : p.job_tokens), routing.entries_before[e] + run * p.job_tokens};
       }
     }
     if (threadIdx.x == 0) *p.job_count = routing.jobs;
@@ -172,9 +185,8 @@ __global__ void __launch_bounds__(kThreads) gate_up_kernel(Params p) {
   __syncthreads();
   // The job's tokens, and their routes.
   for (int q = threadIdx.x; q < p.routes; q += kThreads) {
-    float weight;
-    if (expert_of(p, p.ids[q]) != job.expert) continue;
-    const int at = routing.place(p, q, weight) - job.first;
+    if (routing.experts[q] != job.expert || !routing.first(p, q)) continue;
+    const int at = routing.place(p, q) - job.first;
     if (at >= 0 && at < job.count) job_route[at] = q;
   }
   __syncthreads();
@@ -201,7 +213,7 @@ __global__ void __launch_bounds__(kThreads) gate_up_kernel(Params p) {
   };
   auto load = [&](Stage &s, int line) {
 #pragma unroll
-    for (int i = 0; i < kGroups; ++i) s.w[i] = piece_of<kWhole>(row[i], line * kLine + (lane & 7) * 8, p.hidden);
+    for (int i = 0; i < kGroups; ++i) s.w[i] = weights_of<kWhole, kOnce>(row[i], line * kLine + (lane & 7) * 8, p.hidden);
 #pragma unroll
     for (int ks = 0; ks < 2; ++ks) s.x[ks] = piece_of<kWhole>(x, line * kLine + ks * 32 + g * 8, p.hidden);
   };
@@ -217,7 +229,7 @@ __global__ void __launch_bounds__(kThreads) gate_up_kernel(Params p) {
         acc[b] = T::mfma(regroup[wave][(2 * b + (r16 >> 3)) * 64 + rr * 8 + ((4 * ks + g) ^ rr)], s.x[ks], acc[b]);
       }
   };
-  constexpr int kAhead = 4;
+  constexpr int kAhead = 2;
   Stage stages[kAhead];
 #pragma unroll
   for (int i = 0; i < kAhead; ++i)
@@ -255,30 +267,52 @@ __global__ void __launch_bounds__(kThreads) gate_up_kernel(Params p) {
     if (column + c >= p.padded) continue;
     // (the padding: zeros)
     const float v = column + c < p.width ? up * gate(gated, p.activation) * kHeld<T> : 0.0f;
-    uint16_t *to = p.gated + static_cast<int64_t>(job_route[token]) * 2 * p.padded + column + c;
+    uint16_t *to = p.gated + static_cast<int64_t>(job_route[token]) * 2 * p.padded + (column + c) / kLine * 2 * kLine + (column + c) % kLine;
     const uint16_t value = T::from_f32(v);
     const float error = v - T::to_f32(value);
     to[0] = value;
-    to[p.padded] = T::from_f32(error == error ? error : 0.0f);
+    to[kLine] = T::from_f32(error == error ? error : 0.0f);
   }
 }
 
 // ---- down -------------------------------------------------------------------------------------------------
 
-/// kCols output columns a workgroup; a wavefront takes a quarter of each job's lines and keeps its own sums of all
-/// rows in LDS.
-template <class T, bool kWhole, int kCols>
-__global__ void __launch_bounds__(kThreads) down_kernel(Params p) {
-  constexpr int kGroups = kCols / 8;
-  __shared__ Job jobs[kMostTokens * UNISERVE_TOKEN_EXPERTS_MAX_TOP];
-  __shared__ float totals[kWaves][kMostTokens][kCols];
-  __shared__ u32x4 regroup[kWaves][kGroups * 64];
+/// kCols output columns a workgroup, kSets sets of four wavefronts. A set takes the jobs of the experts whose number is its
+/// own modulo kSets, a wavefront a quarter of each job's lines; it keeps its own sums of all rows in LDS. (By the
+/// experts' numbers: a row's sums come in one order, whatever the other rows name.)
+/// kTokens of a job at most: their gated values come as whole lines, too, and through LDS (in the operand layout
+/// they took four loads of sixteen columns for any number of tokens: T=16 72 us, 50 now).
+template <class T, bool kWhole, bool kOnce, int kCols, int kSets, int kTokens>
+__global__ void __launch_bounds__(kSets *kThreads) down_kernel(Params p) {
+  constexpr int kGroups = kCols / 8, kAllThreads = kSets * kThreads;
+  __shared__ Job jobs[kMostRoutes];  // each set's, one set's after the other's
+  __shared__ Entry entries[kMostRoutes];
+  __shared__ float totals[kSets * kWaves][kMostTokens][kCols];
+  __shared__ u32x4 regroup[kSets * kWaves][kGroups * 64];
+  __shared__ u32x4 lines_of[kSets * kWaves][kTokens * 16];
   const int count = *p.job_count;
-  for (int i = threadIdx.x; i < count; i += kThreads) jobs[i] = p.jobs[i];
-  for (int i = threadIdx.x; i < kWaves * kMostTokens * kCols; i += kThreads) (&totals[0][0][0])[i] = 0.0f;
-  __syncthreads();
-  const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / kWave);
+  const int all_wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / kWave);
+  const int wave = all_wave % kWaves, set = all_wave / kWaves;
   const int lane = lane_id(), r16 = lane & 15, g = lane >> 4;
+  for (int i = threadIdx.x; i < p.routes; i += kAllThreads) entries[i] = p.entries[i];  // (those past the last are not read)
+  for (int i = threadIdx.x; i < kSets * kWaves * kMostTokens * kCols; i += kAllThreads) (&totals[0][0][0])[i] = 0.0f;
+  // Every wavefront counts the jobs of the sets before its own and of its own; the set's first one lists them.
+  int first_job = 0, own_jobs = 0;
+  for (int i = 0; i < count; i += kWave) {
+    const int of = i + lane < count ? p.jobs[i + lane].expert % kSets : kSets;
+    first_job += __popcll(ballot(of < set));
+    own_jobs += __popcll(ballot(of == set));
+  }
+  if (wave == 0) {
+    int at = first_job;
+    for (int i = 0; i < count; i += kWave) {
+      const Job job = p.jobs[i + lane < count ? i + lane : 0];
+      const uint64_t own = ballot(i + lane < count && job.expert % kSets == set);
+      if ((own >> lane) & 1) jobs[at + __popcll(own & ((1ull << lane) - 1))] = job;
+      at += __popcll(own);
+    }
+  }
+  __syncthreads();
   const int column = static_cast<int>(blockIdx.x) * kCols;
   int64_t row[kGroups];
 #pragma unroll
@@ -288,55 +322,67 @@ __global__ void __launch_bounds__(kThreads) down_kernel(Params p) {
   }
   const int lines = p.padded / kLine;
   const int line_first = wave * lines / kWaves, line_count = (wave + 1) * lines / kWaves - line_first;
-  // Units: the wavefront's lines of every job, one job after the other.
+  // Units: the wavefront's lines of every job of its set, one job after the other.
   struct Stage {
-    u32x4 w[kGroups], values[2], errors[2];
+    u32x4 w[kGroups], gated[kTokens / 4];
   };
-  int load_job = 0, load_line = 0;
+  int load_job = first_job, load_line = 0;
+  const uint16_t *weights[kGroups], *gated[kTokens / 4];  // the lane's rows of the job to load
   auto load = [&](Stage &s) {
-    const Job job = jobs[load_job];
-    const uint16_t *weights = p.down + static_cast<int64_t>(__builtin_amdgcn_readfirstlane(job.expert)) * p.hidden * p.width;
-    const int route = p.entries[job.first + (r16 < job.count ? r16 : 0)].route;
+    if (load_line == 0) {
+      const Job job = jobs[load_job++];
+      const uint16_t *down = p.down + static_cast<int64_t>(__builtin_amdgcn_readfirstlane(job.expert)) * p.hidden * p.width;
+#pragma unroll
+      for (int i = 0; i < kGroups; ++i) weights[i] = down + row[i];
+#pragma unroll
+      for (int i = 0; i < kTokens / 4; ++i) {
+        const int token = i * 4 + lane / 16;
+        gated[i] = p.gated + static_cast<int64_t>(entries[job.first + (token < job.count ? token : 0)].route) * 2 * p.padded + (lane & 15) * 8;
+      }
+    }
     const int at = (line_first + load_line) * kLine;
 #pragma unroll
-    for (int i = 0; i < kGroups; ++i) s.w[i] = piece_of<kWhole>(weights + row[i], at + (lane & 7) * 8, p.width);
-    const uint16_t *gated = p.gated + static_cast<int64_t>(route) * 2 * p.padded + at + g * 8;
+    for (int i = 0; i < kGroups; ++i) s.w[i] = weights_of<kWhole, kOnce>(weights[i], at + (lane & 7) * 8, p.width);
 #pragma unroll
-    for (int ks = 0; ks < 2; ++ks) {
-      s.values[ks] = *reinterpret_cast<const u32x4 *>(gated + ks * 32);
-      s.errors[ks] = *reinterpret_cast<const u32x4 *>(gated + p.padded + ks * 32);
-    }
-    if (++load_line == line_count) load_line = 0, ++load_job;
+    for (int i = 0; i < kTokens / 4; ++i) s.gated[i] = *reinterpret_cast<const u32x4 *>(gated[i] + at * 2);
+    load_line = load_line + 1 == line_count ? 0 : load_line + 1;
   };
-  int job_at = 0, line_at = 0;
-  floatx4 acc{0.0f, 0.0f, 0.0f, 0.0f};
+  int job_at = first_job, line_at = 0;
+  floatx4 acc{0.0f, 0.0f, 0.0f, 0.0f}, acc_errors{0.0f, 0.0f, 0.0f, 0.0f};
   auto multiply = [&](const Stage &s) {
     const int r = lane >> 3, piece = lane & 7;
 #pragma unroll
-    for (int i = 0; i < kGroups; ++i) regroup[wave][i * 64 + r * 8 + (piece ^ r)] = s.w[i];
+    for (int i = 0; i < kGroups; ++i) regroup[all_wave][i * 64 + r * 8 + (piece ^ r)] = s.w[i];
+    // Chunk c (eight values, then eight errors) of a token's line lies at c ^ 4 token: four tokens' chunks in all banks.
+#pragma unroll
+    for (int i = 0; i < kTokens / 4; ++i) {
+      const int token = i * 4 + lane / 16;
+      lines_of[all_wave][token * 16 + ((lane & 15) ^ (token * 4 & 15))] = s.gated[i];
+    }
+    const int token = r16 % kTokens;
 #pragma unroll
     for (int ks = 0; ks < 2; ++ks) {
       const int rr = r16 & 7;
-      const u32x4 w = regroup[wave][(kGroups == 1 ? 0 : r16 >> 3) * 64 + rr * 8 + ((4 * ks + g) ^ rr)];
-      acc = T::mfma(w, s.values[ks], acc);
-      acc = T::mfma(w, s.errors[ks], acc);
+      const u32x4 w = regroup[all_wave][(kGroups == 1 ? 0 : r16 >> 3) * 64 + rr * 8 + ((4 * ks + g) ^ rr)];
+      acc = T::mfma(w, lines_of[all_wave][token * 16 + ((4 * ks + g) ^ (token * 4 & 15))], acc);
+      acc_errors = T::mfma(w, lines_of[all_wave][token * 16 + ((8 + 4 * ks + g) ^ (token * 4 & 15))], acc_errors);
     }
     if (++line_at < line_count) return;
     // The job's rows are complete (of this wavefront's lines): lane r16's token, rows 4 g .. 4 g + 3.
     const Job job = jobs[job_at];
     if (r16 < job.count && (kGroups > 1 || g < 2)) {
-      const Entry entry = p.entries[job.first + r16];
-      float *total = &totals[wave][entry.route / p.top][4 * g];
+      const Entry entry = entries[job.first + r16];
+      float *total = &totals[all_wave][entry.route / p.top][4 * g];
       const float weight = entry.weight * (1.0f / kHeld<T>);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) total[i] = __builtin_fmaf(weight, acc[i], total[i]);
+      for (int i = 0; i < 4; ++i) total[i] = __builtin_fmaf(weight, acc[i] + acc_errors[i], total[i]);
     }
-    acc = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+    acc = acc_errors = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
     line_at = 0;
     ++job_at;
   };
-  const int units = count * line_count;
-  constexpr int kAhead = 8;
+  const int units = own_jobs * line_count;
+  constexpr int kAhead = 4;
   Stage stages[kAhead];
 #pragma unroll
   for (int i = 0; i < kAhead; ++i)
@@ -357,33 +403,61 @@ __global__ void __launch_bounds__(kThreads) down_kernel(Params p) {
     }
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < p.tokens * kCols; i += kThreads) {
+  for (int i = threadIdx.x; i < p.tokens * kCols; i += kAllThreads) {
     const int token = i / kCols, c = i % kCols;
     if (column + c >= p.hidden) continue;
     float v = 0.0f;
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) v += totals[w][token][c];
+    for (int w = 0; w < kSets * kWaves; ++w) v += totals[w][token][c];
     if (p.residual != nullptr) v += T::to_f32(p.residual[token * p.residual_stride + column + c]);
     p.out[token * p.out_stride + column + c] = T::from_f32(v);
   }
 }
 
+template <class T, bool kWhole, bool kOnce, int kCols, int kSets, int kTokens>
+void launch_down_kernel(const Params &p, hipStream_t stream) {
+  hipLaunchKernelGGL((down_kernel<T, kWhole, kOnce, kCols, kSets, kTokens>), dim3(static_cast<uint32_t>(ceil_div(p.hidden, kCols))),
+                     dim3(kSets * kThreads), 0, stream, p);
+}
+
+/// Eight columns and sixteen wavefronts a workgroup where each CU gets one at most, else sixteen columns and eight
+/// wavefronts (128 experts of 2048 x 768, T=16: 50 us against 75, T=64 98 against 125; 64 of 4096 x 1408, T=64 185
+/// against 140).
+template <class T, bool kWhole, bool kOnce>
+void launch_down(const Params &p, hipStream_t stream) {
+  const bool narrow = ceil_div(p.hidden, 8) <= 256;
+  switch (p.job_tokens) {
+    case 4: return narrow ? launch_down_kernel<T, kWhole, kOnce, 8, 4, 4>(p, stream) : launch_down_kernel<T, kWhole, kOnce, 16, 2, 4>(p, stream);
+    case 8: return narrow ? launch_down_kernel<T, kWhole, kOnce, 8, 4, 8>(p, stream) : launch_down_kernel<T, kWhole, kOnce, 16, 2, 8>(p, stream);
+    default: return narrow ? launch_down_kernel<T, kWhole, kOnce, 8, 4, 16>(p, stream) : launch_down_kernel<T, kWhole, kOnce, 16, 2, 16>(p, stream);
+  }
+}
+
+template <class T, bool kOnce>
+void launch_both(const Params &p, bool whole_x, bool whole_gated, hipStream_t stream) {
+  constexpr int kCols = 16;  // (32: T=64 134 us against 137, T=1 14.2 against 12.3; 64: 166 and 22.7)
+  const int64_t bound = p.experts + p.routes / p.job_tokens;  // of the jobs, without a look at the ids
+  const dim3 grid(static_cast<uint32_t>(ceil_div(p.padded, kCols)), static_cast<uint32_t>(p.routes < bound ? p.routes : bound));
+  if (whole_x) hipLaunchKernelGGL((gate_up_kernel<T, true, kOnce, kCols>), grid, dim3(kThreads), 0, stream, p);
+  else hipLaunchKernelGGL((gate_up_kernel<T, false, kOnce, kCols>), grid, dim3(kThreads), 0, stream, p);
+  whole_gated ? launch_down<T, true, kOnce>(p, stream) : launch_down<T, false, kOnce>(p, stream);
+}
+
+/// Jobs of at most 4, 8 or 16 tokens, by the tokens that an expert expects: the fewer, the less gated data the second kernel
+/// loads (128 experts, top 8, gate_up and down: T=16, one token an expert, 86 + 50 us with four, 86 + 57 with eight;
+/// T=64, four an expert, 194 + 106, 137 + 98 and with sixteen 146 + 115). Where an expert seldom has a second
+/// job its weights are loaded past the caches (T=64 151 -> 137; eight experts of 16 tokens 15 -> 19).
 template <class T>
-void launch(const Params &p, bool whole_x, bool whole_gated, hipStream_t stream) {
-  const int64_t most_jobs = p.routes < p.experts + p.routes / kJobTokens ? p.routes : p.experts + p.routes / kJobTokens;
-  constexpr int kUpCols = 16, kDownCols = 16;
-  const dim3 up_grid(static_cast<uint32_t>(ceil_div(p.padded, kUpCols)), static_cast<uint32_t>(most_jobs));
-  if (whole_x) hipLaunchKernelGGL((gate_up_kernel<T, true, kUpCols>), up_grid, dim3(kThreads), 0, stream, p);
-  else hipLaunchKernelGGL((gate_up_kernel<T, false, kUpCols>), up_grid, dim3(kThreads), 0, stream, p);
-  const dim3 down_grid(static_cast<uint32_t>(ceil_div(p.hidden, kDownCols)));
-  if (whole_gated) hipLaunchKernelGGL((down_kernel<T, true, kDownCols>), down_grid, dim3(kThreads), 0, stream, p);
-  else hipLaunchKernelGGL((down_kernel<T, false, kDownCols>), down_grid, dim3(kThreads), 0, stream, p);
+void launch(Params &p, bool whole_x, bool whole_gated, hipStream_t stream) {
+  p.job_tokens = p.tokens <= 4 || p.routes <= 2 * p.experts ? 4 : p.tokens <= 8 || p.routes <= 6 * p.experts ? 8 : 16;
+  if (p.tokens <= p.job_tokens || 2 * p.routes <= p.experts * p.job_tokens) launch_both<T, true>(p, whole_x, whole_gated, stream);
+  else launch_both<T, false>(p, whole_x, whole_gated, stream);
 }
 
 int64_t padded_width(int64_t width) { return ceil_div<int64_t>(width, kLine) * kLine; }
 /// The count, the jobs, the entries, the gated pairs.
 int64_t workspace_of(int64_t routes, int64_t width) {
-  return 16 + routes * (static_cast<int64_t>(sizeof(Job)) + ceil_div<int64_t>(sizeof(Entry), 16) * 16 + 4 * padded_width(width));
+  return 16 + routes * (static_cast<int64_t>(sizeof(Job) + sizeof(Entry)) + 4 * padded_width(width));
 }
 
 int32_t run(const uniserve_token_experts_call *call, void *stream) {
