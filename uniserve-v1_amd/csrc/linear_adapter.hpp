@@ -310,15 +310,21 @@ __device__ __forceinline__ void add_low_rank(const AdapterParams &p, floatx4 (&a
     constexpr bool kErrors = decltype(errors_too)::value;
     const int64_t at = group * 32 + up_at;
     u32x4 ws[kBatch][NB];
+    if (p.up_whole) {
+      // (Past the rank the row's first chunk again, against zeros: what it holds, the row has anyway.)
+      const int64_t whole_at = at < p.rank ? at : 0;
 #pragma unroll
-    for (int j = 0; j < kBatch; ++j) {
-      const uint16_t *up = p.up + (current[j] < 0 ? current[0] : current[j]) * p.up_stride;
-      if (p.up_whole) {
+      for (int j = 0; j < kBatch; ++j) {
+        const uint16_t *up = p.up + (current[j] < 0 ? current[0] : current[j]) * p.up_stride;
 #pragma unroll
-        for (int nb = 0; nb < NB; ++nb) ws[j][nb] = load8_of<true>(up + row[nb], at, p.rank);
-      } else {
+        for (int nb = 0; nb < NB; ++nb) ws[j][nb] = *reinterpret_cast<const u32x4 *>(up + (row[nb] + whole_at));
+      }
+    } else {
 #pragma unroll
-        for (int nb = 0; nb < NB; ++nb) ws[j][nb] = load8_of<false>(up + row[nb], at, p.rank);
+      for (int j = 0; j < kBatch; ++j) {
+        const uint16_t *up = p.up + (current[j] < 0 ? current[0] : current[j]) * p.up_stride;
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) ws[j][nb] = load8(up + row[nb], at, p.rank);
       }
     }
     // Two token blocks at a time: all at once do not fit the registers of the large shapes.
@@ -355,9 +361,8 @@ __device__ __forceinline__ void add_low_rank(const AdapterParams &p, floatx4 (&a
 #pragma unroll
             for (int of = 0; of < kPerHalf; ++of) {
               const int nb = h * kPerHalf + of;
-              const u32x4 w = held ? ws[j][nb] : nothing;
-              floatx4 part = T::mfma(w, values[h][i], floatx4{0.0f, 0.0f, 0.0f, 0.0f});
-              if constexpr (kErrors) part = T::mfma(w, errors[h][i], part);
+              floatx4 part = T::mfma(ws[j][nb], values[h][i], floatx4{0.0f, 0.0f, 0.0f, 0.0f});
+              if constexpr (kErrors) part = T::mfma(ws[j][nb], errors[h][i], part);
 #pragma unroll
               for (int c = 0; c < 4; ++c) {
                 const float v = std::is_same<T, F16>::value ? part[c] * factor[h][i] : part[c];

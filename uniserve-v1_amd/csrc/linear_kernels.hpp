@@ -246,19 +246,21 @@ void launch_low_rank(const AdapterParams &a, bool gated, hipStream_t stream) {
   static_cast<AdapterParams &>(p) = a;
   p.width = layout.width, p.groups = layout.groups, p.halves = gated ? 2 : 1;
   p.n = static_cast<int64_t>(p.halves) * layout.groups * layout.width;
+  // Rows of up to sixteen adapters or more are few rows' (a decode step's), and tiles of sixteen rows; of 32 rows and
+  // more tiles, few have several. Workgroups share out a tile's adapters while there are fewer tiles than CUs
+  // (777 x 2048, rank 64 gated, five runs: 9.4 us, one workgroup a tile 14.5; 8192 rows, rank 64, twelve runs: 17.5,
+  // with two a tile 19.5).
+  const auto launch_shape = [&](auto shape, auto by_dma) {
+    using S = decltype(shape);
+    const int64_t spare = 256 / tiles_of<S>(p, false);
+    const int64_t most = p.m < 16 ? p.m : 16;
+    launch_tiles<T, false, decltype(by_dma)::value, S>(p, stream, static_cast<uint32_t>(spare < 1 ? 1 : spare < most ? spare : most));
+  };
   const bool few = p.m <= 256;
-  const uint32_t shares = few ? static_cast<uint32_t>(p.m < 16 ? p.m : 16) : 1;
-  if (!p.down_by_dma) {
-    if (few) return launch_tiles<T, false, false, Any16x32>(p, stream, shares);
-    return launch_tiles<T, false, false, Any32>(p, stream, shares);
-  }
-  if (few) {
-    if (p.n <= 16) return launch_tiles<T, false, true, Tile16>(p, stream, shares);
-    return launch_tiles<T, false, true, Tile16x32Alone>(p, stream, shares);
-  }
-  if (p.n <= 16) return launch_tiles<T, false, true, Rank32x16>(p, stream, shares);
-  if (p.n <= 32) return launch_tiles<T, false, true, Tile32Alone>(p, stream, shares);
-  return launch_tiles<T, false, true, Tile32x64Alone>(p, stream, shares);
+  if (!p.down_by_dma) return few ? launch_shape(Any16x32{}, std::false_type{}) : launch_shape(Any32{}, std::false_type{});
+  if (few) return p.n <= 16 ? launch_shape(Tile16{}, std::true_type{}) : launch_shape(Tile16x32Alone{}, std::true_type{});
+  if (p.n <= 16) return launch_shape(Rank32x16{}, std::true_type{});
+  return p.n <= 32 ? launch_shape(Tile32Alone{}, std::true_type{}) : launch_shape(Tile32x64Alone{}, std::true_type{});
 }
 
 }  // namespace linear

@@ -447,11 +447,9 @@ class AddNormCall(ctypes.Structure):
 
 
 class AdapterLinearCall(ctypes.Structure):
-    """``uniserve_adapter_linear_call``; the product's fields are reached directly, too."""
+    """``uniserve_adapter_linear_call``, whose first field is a whole ``uniserve_linear_call``: its fields, in line."""
 
-    _anonymous_ = ("product",)
-    _fields_ = [
-        ("product", LinearCall),
+    _fields_ = LinearCall._fields_ + [
         ("down", _P),
         ("up", _P),
         ("adapter", _P),

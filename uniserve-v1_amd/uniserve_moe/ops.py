@@ -159,7 +159,7 @@ def expert_topk(scores, top, scoring="sigmoid", bias=None, groups=1, top_groups=
 
 
 def _product_call(name, x, weight, columns, bias, activation, gate, residual, out, out_dtype):
-    """A dense product's call, its output and its device."""
+    """A dense product's call (its fields but the error), its output and its device."""
     dtype, index = x.dtype, x.get_device()
     element = _ELEMENT.get(dtype)
     if x.dim() != 2 or dtype not in _PRODUCT or index < 0:
@@ -195,15 +195,15 @@ def _product_call(name, x, weight, columns, bias, activation, gate, residual, ou
         if residual.dtype != out_dtype:
             raise ValueError(f"{name}: the residual is of the output's type")
         residual_at, residual_stride = residual.data_ptr(), _matrix(residual, tokens, columns, index, name, "the residual")
-    call = LinearCall(x.data_ptr(), weight.data_ptr(), bias_at, gate_at, residual_at, out.data_ptr(), tokens, columns,
-                      width, x_stride, weight_stride, gate_stride, residual_stride, out_stride, element, bias_element,
-                      out_element, LINEAR_ACTIVATION[activation])
+    call = (x.data_ptr(), weight.data_ptr(), bias_at, gate_at, residual_at, out.data_ptr(), tokens, columns, width,
+            x_stride, weight_stride, gate_stride, residual_stride, out_stride, element, bias_element, out_element,
+            LINEAR_ACTIVATION[activation])
     return call, out, index
 
 
 def _product(entry, name, x, weight, columns, bias, activation, gate, residual, out, out_dtype):
     call, out, index = _product_call(name, x, weight, columns, bias, activation, gate, residual, out, out_dtype)
-    _enter(entry, call, index, name)
+    _enter(entry, LinearCall(*call), index, name)
     return out
 
 
@@ -257,7 +257,7 @@ def _adapted(entry, name, x, weight, columns, halves, down, up, adapter, scales,
         workspace = torch.empty(adapter_workspace(x.shape[0], halves * rank), dtype=torch.uint8, device=x.device)
     elif workspace.get_device() != index or not workspace.is_contiguous():
         raise ValueError(f"{name}: the workspace is contiguous, on device {index}")
-    call = AdapterLinearCall(product, down.data_ptr(), up.data_ptr(),
+    call = AdapterLinearCall(*product, b"", down.data_ptr(), up.data_ptr(),
                              _vector(adapter, x.shape[0], (torch.int32,), index, name, "adapter"),
                              _vector(scales, count, (torch.float32,), index, name, "scales"), workspace.data_ptr(),
                              workspace.numel() * workspace.element_size(), count, rank, down_stride, down_row_stride,
