@@ -109,12 +109,14 @@ struct RowsAdapters {
   __device__ __forceinline__ void load(const AdapterParams &p, int64_t m0) {
     for (int t = threadIdx.x; t < kIds; t += blockDim.x) id[t] = t < kRows ? adapter_of(p, m0 + t) : -1;
   }
-  __device__ __forceinline__ void load_factors(const AdapterParams &p, int64_t m0, int buffer, const LowLayout &layout, int halves, int part) {
-    for (int t = threadIdx.x; t < kRows; t += blockDim.x) {
-      const int64_t m = m0 + t < p.m ? m0 + t : p.m - 1;
-      factor[buffer][t] = *reinterpret_cast<const float *>(p.low + m * layout.row_bytes(halves) +
-                                                           static_cast<int64_t>(part) * layout.group_bytes() + 4 * layout.width);
-    }
+  /// A thread's row's factor (a workgroup has as many threads as its tile has rows, or more).
+  __device__ __forceinline__ float load_factor(const AdapterParams &p, int64_t m0, const LowLayout &layout, int halves, int part) const {
+    const int64_t m = static_cast<int>(threadIdx.x) < kRows && m0 + threadIdx.x < p.m ? m0 + threadIdx.x : p.m - 1;
+    return *reinterpret_cast<const float *>(p.low + m * layout.row_bytes(halves) + static_cast<int64_t>(part) * layout.group_bytes() +
+                                            4 * layout.width);
+  }
+  __device__ __forceinline__ void put_factor(int buffer, float f) {
+    if (static_cast<int>(threadIdx.x) < kRows) factor[buffer][threadIdx.x] = f;
   }
 };
 template <bool kFactors>
@@ -161,9 +163,14 @@ __device__ __forceinline__ void remake(const AdapterParams &p, int64_t m, int64_
           v = __builtin_fmaf(T::to_f32(low[0]) + T::to_f32(low[layout.width]), T::to_f32(up[rank]), v);
         }
       }
-#pragma unroll 1
-      for (int64_t k = 0; k < p.k; ++k)
-        v = __builtin_fmaf(T::to_f32(p.x[m * p.x_stride + k]), T::to_f32(p.w[column * p.w_stride + k]), v);
+      const uint16_t *x = p.x + m * p.x_stride, *w = p.w + column * p.w_stride;
+#pragma unroll 2
+      for (int64_t k = 0; k < p.k; k += 8) {
+        const u32x4 xs = load8_of<true>(x, k, p.k), ws = load8_of<true>(w, k, p.k);  // (the walk's rows are whole)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          v = __builtin_fmaf(T::high(xs[e]), T::high(ws[e]), __builtin_fmaf(T::low(xs[e]), T::low(ws[e]), v));
+      }
 #pragma unroll
       for (int c = 0; c < 8; ++c)
         if (c == i) {

@@ -146,15 +146,23 @@ double cost_of(const LinearParams &p, bool gated, const Cost &c) {
   return c.first + c.round * (rounds - 1.0) + per_stage * stages;
 }
 
-/// A shape's time where it is a product with adapters, or not to be chosen: up rows that the DMA cannot read do not go
-/// through the walk (bf16), and the largest f16 tiles spill sums where they add the adapters' (8192 x 4096 x 2048, ranks
-/// 16, 12 runs of rows: 256 x 256 tiles 160 us, 128 x 256 145).
+/// Whether a product with adapters has a shape at all: the largest f16 tiles, which add the adapters' products through
+/// registers, spill sums (8192 x 4096 x 2048, rank 16, twelve runs: 256 x 256 164 us, 128 x 256 158).
+template <class T, class S, class P>
+constexpr bool kServes = !(std::is_same<P, AdapterParams>::value && std::is_same<T, F16>::value) || S::kMB * S::kNB <= 16;
+
+/// A shape's time, or not to be chosen: also where bf16 up rows would go through the walk and the DMA cannot read them.
 template <class T, class S, class P>
 double cost_with(const P &p, bool gated, const Cost &c) {
-  if constexpr (std::is_same<P, AdapterParams>::value && S::kSplit == 1 && S::kMB * S::kNB >= 8) {
-    if (std::is_same<T, F16>::value ? S::kMB * S::kNB > 16 : !p.up_whole) return 1e30;
-  }
+  if constexpr (!kServes<T, S, P>) return 1e30;
+  if constexpr (std::is_same<P, AdapterParams>::value && std::is_same<T, Bf16>::value && S::kSplit == 1 && S::kMB * S::kNB >= 8)
+    if (!p.up_whole) return 1e30;
   return cost_of<S>(p, gated, c);
+}
+
+template <class T, bool kGated, class S, class P>
+void launch_chosen(const P &p, hipStream_t stream) {
+  if constexpr (kServes<T, S, P>) launch_tiles<T, kGated, true, S>(p, stream);
 }
 
 template <int kShapes>
@@ -217,21 +225,21 @@ void launch(const P &p, hipStream_t stream) {
       kGated ? 1e30 : cost_with<T, Tile16>(p, kGated, {3.22, 0.707, 0.034, 0.038, 1.78}),
   };
   switch (cheapest(costs)) {
-    case 0: return launch_tiles<T, kGated, true, Tile256>(p, stream);
-    case 1: return launch_tiles<T, kGated, true, Tile192x256>(p, stream);
-    case 2: return launch_tiles<T, kGated, true, Tile128x256>(p, stream);
-    case 3: return launch_tiles<T, kGated, true, Tile192x128>(p, stream);
-    case 4: return launch_tiles<T, kGated, true, Tile128>(p, stream);
-    case 5: return launch_tiles<T, kGated, true, Tile128Alone>(p, stream);
-    case 6: return launch_tiles<T, kGated, true, Tile96x128Alone>(p, stream);
-    case 7: return launch_tiles<T, kGated, true, Tile128x64Alone>(p, stream);
-    case 8: return launch_tiles<T, kGated, true, Tile64>(p, stream);
-    case 9: return launch_tiles<T, kGated, true, Tile48x64Alone>(p, stream);
-    case 10: return launch_tiles<T, kGated, true, Tile32x64Alone>(p, stream);
-    case 11: return launch_tiles<T, kGated, true, Tile32Alone>(p, stream);
-    case 12: return launch_tiles<T, kGated, true, Tile16x32Alone>(p, stream);
+    case 0: return launch_chosen<T, kGated, Tile256>(p, stream);
+    case 1: return launch_chosen<T, kGated, Tile192x256>(p, stream);
+    case 2: return launch_chosen<T, kGated, Tile128x256>(p, stream);
+    case 3: return launch_chosen<T, kGated, Tile192x128>(p, stream);
+    case 4: return launch_chosen<T, kGated, Tile128>(p, stream);
+    case 5: return launch_chosen<T, kGated, Tile128Alone>(p, stream);
+    case 6: return launch_chosen<T, kGated, Tile96x128Alone>(p, stream);
+    case 7: return launch_chosen<T, kGated, Tile128x64Alone>(p, stream);
+    case 8: return launch_chosen<T, kGated, Tile64>(p, stream);
+    case 9: return launch_chosen<T, kGated, Tile48x64Alone>(p, stream);
+    case 10: return launch_chosen<T, kGated, Tile32x64Alone>(p, stream);
+    case 11: return launch_chosen<T, kGated, Tile32Alone>(p, stream);
+    case 12: return launch_chosen<T, kGated, Tile16x32Alone>(p, stream);
     default:
-      if constexpr (!kGated) return launch_tiles<T, kGated, true, Tile16>(p, stream);
+      if constexpr (!kGated) return launch_chosen<T, kGated, Tile16>(p, stream);
   }
 }
 

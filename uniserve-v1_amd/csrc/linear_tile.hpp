@@ -122,10 +122,11 @@ __global__ void __launch_bounds__(S::kThreads) tile_kernel(P p) {
   constexpr bool kMany = kAdapters && S::kSplit == 1 && MB * NB >= 8;
   constexpr bool kWalked = kMany && kDma && std::is_same<T, Bf16>::value;
   constexpr bool kStaged = kMany && !kWalked;
+  static_assert(!kStaged || S::kThreads >= S::kBM, "a thread for each row's factor");
   [[maybe_unused]] __shared__ RowsAdapters<kMany ? S::kBM : 0, std::is_same<T, F16>::value> rows_adapters;
   if constexpr (kMany) rows_adapters.load(p, m0);
   [[maybe_unused]] typename std::conditional<kRanks, NamedAdapters, int>::type named = named_adapters(p, m0, S::kBM);
-  do {
+  do {  // once, or for each adapter that the tile's rows name (kRanks)
   if constexpr (kRanks) {
     if (!named.next()) return;
   }
@@ -429,41 +430,36 @@ __global__ void __launch_bounds__(S::kThreads) tile_kernel(P p) {
       // (opaque: what the lanes' addresses share from stage to stage is not kept, the sums need the registers)
       int l = lane;
       asm volatile("" : "+v"(l));
-      constexpr int kAtOnce = S::kLoads < 8 ? S::kLoads : 8;
+      u32x4 pieces[S::kLoads];
+      [[maybe_unused]] float factor_of_row = 1.0f;
+      if constexpr (std::is_same<T, F16>::value) factor_of_row = rows_adapters.load_factor(p, m0, layout, kHalves, part);
 #pragma unroll
-      for (int from = 0; from < S::kLoads; from += kAtOnce) {
-        u32x4 pieces[kAtOnce];
-#pragma unroll
-        for (int u = 0; u < kAtOnce; ++u) {
-          const int i = from + u;
-          if (i >= S::kLoads) continue;
-          const int r = 8 * (wave + S::kWaves * i) + l / 8, c = (l & 7) ^ ((l >> 4) & 3) ^ (4 * ((wave + S::kWaves * i) & 1));
-          const bool filled = 4 * c < layout.width;
-          pieces[u] = u32x4{0, 0, 0, 0};
-          if (i < S::kBM / 8 / S::kWaves) {
-            const uint32_t row = static_cast<uint32_t>(r < rows_left ? r : rows_left - 1);
-            if (filled)
-              pieces[u] = *reinterpret_cast<const u32x4 *>(low + (row * static_cast<uint32_t>(layout.row_bytes(kHalves)) + 16 * c));
-          } else {
-            const int j = r - S::kBM;
-            const int of = j / (NB * 16), in = j % (NB * 16);
-            int column = of * kWaveCols + (kGated ? in % kWaveCols : in);
-            column = column < cols_left ? column : cols_left - 1;
-            const int at = (wide ? c & 3 : layout.width == 16 ? c & 1 : 0) * 8;
-            if (p.up_whole) {
-              if (filled && group * 32 + at < p.rank)
-                pieces[u] = *reinterpret_cast<const u32x4 *>(up + (static_cast<uint32_t>(column) * static_cast<uint32_t>(p.up_row_stride) + at));
-            } else if (filled) {
-              pieces[u] = load8(up + column * p.up_row_stride, at, p.rank - group * 32);
-            }
-          }
+      for (int i = 0; i < S::kLoads; ++i) {
+        const int r = 8 * (wave + S::kWaves * i) + l / 8, c = (l & 7) ^ ((l >> 4) & 3) ^ (4 * ((wave + S::kWaves * i) & 1));
+        const bool filled = 4 * c < layout.width;
+        if (i < S::kBM / 8 / S::kWaves) {
+          const uint32_t row = static_cast<uint32_t>(r < rows_left ? r : rows_left - 1);
+          pieces[i] = *reinterpret_cast<const u32x4 *>(low + (row * static_cast<uint32_t>(layout.row_bytes(kHalves)) + (filled ? 16 * c : 0)));
+        } else {
+          const int j = r - S::kBM;
+          const int of = j / (NB * 16), in = j % (NB * 16);
+          int column = of * kWaveCols + (kGated ? in % kWaveCols : in);
+          column = column < cols_left ? column : cols_left - 1;
+          const int at = (wide ? c & 3 : layout.width == 16 ? c & 1 : 0) * 8;
+          // (Past the rank the row's first chunk again, against zeros: what it holds, the row has anyway.)
+          if (p.up_whole)
+            pieces[i] = *reinterpret_cast<const u32x4 *>(up + (static_cast<uint32_t>(column) * static_cast<uint32_t>(p.up_row_stride) +
+                                                               (group * 32 + at < p.rank ? at : 0)));
+          else
+            pieces[i] = load8(up + column * p.up_row_stride, at, p.rank - group * 32);
         }
-#pragma unroll
-        for (int u = 0; u < kAtOnce; ++u)
-          if (from + u < S::kLoads) ring[buffer_of][(wave + S::kWaves * (from + u)) * 64 + l] = pieces[u];
-        __builtin_amdgcn_sched_barrier(0);
       }
-      if constexpr (std::is_same<T, F16>::value) rows_adapters.load_factors(p, m0, buffer_of, layout, kHalves, part);
+#pragma unroll
+      for (int i = 0; i < S::kLoads; ++i) {
+        const int c = (l & 7) ^ ((l >> 4) & 3) ^ (4 * ((wave + S::kWaves * i) & 1));
+        ring[buffer_of][(wave + S::kWaves * i) * 64 + l] = 4 * c < layout.width ? pieces[i] : u32x4{0, 0, 0, 0};
+      }
+      if constexpr (std::is_same<T, F16>::value) rows_adapters.put_factor(buffer_of, factor_of_row);
       // Two buffers in turn: one barrier a stage (a wavefront writes the other one only after all have read it).
       __syncthreads();
       // Both halves of the stage, zeros up to rank 16 (two ways through here would cost registers, and spill sums).
