@@ -280,6 +280,8 @@ __global__ void __launch_bounds__(kThreads) gate_up_kernel(Params p) {
 /// kCols output columns a workgroup, kSets sets of four wavefronts. A set takes the jobs of the experts whose number is its
 /// own modulo kSets, a wavefront a quarter of each job's lines; it keeps its own sums of all rows in LDS. (By the
 /// experts' numbers: a row's sums come in one order, whatever the other rows name.)
+/// (Weights loaded as lane l's chunk of row l % 8, in half l % 16 / 8 of the line, so that the matrix instruction takes them
+/// without LDS, are slower: T=16 52 us against 50, T=64 106 against 98.)
 /// kTokens of a job at most: their gated values come as whole lines, too, and through LDS (in the operand layout
 /// they took four loads of sixteen columns for any number of tokens: T=16 72 us, 50 now).
 template <class T, bool kWhole, bool kOnce, int kCols, int kSets, int kTokens>
@@ -348,36 +350,47 @@ __global__ void __launch_bounds__(kSets *kThreads) down_kernel(Params p) {
     load_line = load_line + 1 == line_count ? 0 : load_line + 1;
   };
   int job_at = first_job, line_at = 0;
-  floatx4 acc{0.0f, 0.0f, 0.0f, 0.0f}, acc_errors{0.0f, 0.0f, 0.0f, 0.0f};
-  auto multiply = [&](const Stage &s) {
-    const int r = lane >> 3, piece = lane & 7;
+  constexpr int kApart = kTokens == 16 ? 2 : 1;  // the errors' columns have sums of their own
+  floatx4 acc[kApart];
+  auto clear = [&]() {
 #pragma unroll
-    for (int i = 0; i < kGroups; ++i) regroup[all_wave][i * 64 + r * 8 + (piece ^ r)] = s.w[i];
+    for (int i = 0; i < kApart; ++i) acc[i] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+  };
+  clear();
+  auto multiply = [&](const Stage &s) {
+#pragma unroll
+    for (int i = 0; i < kGroups; ++i) regroup[all_wave][i * 64 + lane / 8 * 8 + ((lane & 7) ^ (lane / 8))] = s.w[i];
     // Chunk c (eight values, then eight errors) of a token's line lies at c ^ 4 token: four tokens' chunks in all banks.
 #pragma unroll
     for (int i = 0; i < kTokens / 4; ++i) {
       const int token = i * 4 + lane / 16;
       lines_of[all_wave][token * 16 + ((lane & 15) ^ (token * 4 & 15))] = s.gated[i];
     }
-    const int token = r16 % kTokens;
+    // Operand columns: the tokens' values and then their errors, or, of sixteen tokens, one after the other.
+    const int token = r16 % kTokens, errors = kTokens < 16 ? r16 / kTokens % 2 * 8 : 0;
+    const u32x4 *line = &lines_of[all_wave][token * 16];
+    auto chunk = [&](int c) { return line[c ^ (token * 4 & 15)]; };
 #pragma unroll
-    for (int ks = 0; ks < 2; ++ks) {
-      const int rr = r16 & 7;
-      const u32x4 w = regroup[all_wave][(kGroups == 1 ? 0 : r16 >> 3) * 64 + rr * 8 + ((4 * ks + g) ^ rr)];
-      acc = T::mfma(w, lines_of[all_wave][token * 16 + ((4 * ks + g) ^ (token * 4 & 15))], acc);
-      acc_errors = T::mfma(w, lines_of[all_wave][token * 16 + ((8 + 4 * ks + g) ^ (token * 4 & 15))], acc_errors);
+    for (int half = 0; half < 2; ++half) {
+      const u32x4 w = regroup[all_wave][(kGroups == 1 ? 0 : r16 >> 3) * 64 + (r16 & 7) * 8 + ((4 * half + g) ^ (r16 & 7))];
+      acc[0] = T::mfma(w, chunk(errors + 4 * half + g), acc[0]);
+      if constexpr (kApart == 2) acc[1] = T::mfma(w, chunk(8 + 4 * half + g), acc[1]);
     }
     if (++line_at < line_count) return;
     // The job's rows are complete (of this wavefront's lines): lane r16's token, rows 4 g .. 4 g + 3.
     const Job job = jobs[job_at];
-    if (r16 < job.count && (kGroups > 1 || g < 2)) {
-      const Entry entry = entries[job.first + r16];
-      float *total = &totals[all_wave][entry.route / p.top][4 * g];
-      const float weight = entry.weight * (1.0f / kHeld<T>);
+    const Entry entry = entries[job.first + (r16 < job.count ? r16 : 0)];
+    const float weight = entry.weight * (1.0f / kHeld<T>);
+    float *total = totals[all_wave][entry.route / p.top];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) total[i] = __builtin_fmaf(weight, acc[i] + acc_errors[i], total[i]);
+    for (int e = 0; e < 4; ++e) {
+      // (The errors' sum is added to the values' for any kTokens: the order of a row's additions is one.)
+      float v;
+      if constexpr (kApart == 1) v = acc[0][e] + __shfl_xor(acc[0][e], kTokens);
+      else v = acc[0][e] + acc[1][e];
+      if (r16 < job.count && (kGroups > 1 || g < 2)) total[4 * g + e] = __builtin_fmaf(weight, v, total[4 * g + e]);
     }
-    acc = acc_errors = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+    clear();
     line_at = 0;
     ++job_at;
   };
