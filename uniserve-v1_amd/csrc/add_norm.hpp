@@ -87,11 +87,20 @@ struct Eight {
   }
 };
 
-/// The sum of every lane's value, in all lanes.
+/// The sum of every lane's value, in all lanes: over each row of sixteen lanes by DPP moves (as row16_max), then over
+/// pairs of rows and of halves, by gfx950's swaps.
 __device__ __forceinline__ float wave_sum(float v) {
-#pragma unroll
-  for (int offset = kWave / 2; offset > 0; offset /= 2) v += __shfl_xor(v, offset);
-  return v;
+  const auto moved = [](auto of, float x) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), decltype(of)::value, 0xf, 0xf, false));
+  };
+  v += moved(std::integral_constant<int, 0xb1>{}, v);
+  v += moved(std::integral_constant<int, 0x4e>{}, v);
+  v += moved(std::integral_constant<int, 0x141>{}, v);
+  v += moved(std::integral_constant<int, 0x140>{}, v);
+  const auto rows = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = __uint_as_float(rows[0]) + __uint_as_float(rows[1]);
+  const auto halves = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(halves[0]) + __uint_as_float(halves[1]);
 }
 
 /// kTeam threads to a row, kChunks chunks of eight elements a thread: chunk c of a row is thread c % kTeam's.
