@@ -9,6 +9,11 @@
 // also leaves the list of jobs. The second kernel's workgroups own output columns and walk all jobs, adding
 // each one's products, times the routes' weights, to their rows' sums, experts in ascending order: no join across
 // workgroups, no atomics on sums.
+//
+// Bound by the weights: 128 experts of 2048 x 768, 64 tokens (1.2 GB) 136 us, 5.9 TB/s, and 98 us, 4.1 TB/s, where a
+// copy reaches 4.7; one token (75 MB) 12.3 and 9.0 us, a launch and a chain of ids, routing and first weights in each.
+// The second kernel's lines of gated values come from L2, at 64 tokens as many bytes as the weights; neither more
+// wavefronts, deeper loads nor less LDS traffic (operands without a way through it) made it faster.
 #include "extents.hpp"
 #include "linear.hpp"
 #include "uniserve_token_experts.h"
@@ -151,7 +156,8 @@ struct Routing {
 
 // ---- up and gate ------------------------------------------------------------------------------------------
 
-/// kCols gated columns of one job a workgroup; a wavefront takes a quarter of K's lines.
+/// kCols gated columns of one job a workgroup; a wavefront takes a quarter of K's lines, two of them in flight (four:
+/// 146 us against 137 at 64 tokens, fewer workgroups to a CU).
 template <class T, bool kWhole, bool kOnce, int kCols>
 __global__ void __launch_bounds__(kThreads) gate_up_kernel(Params p) {
   constexpr int kGroups = 2 * kCols / 8;   // of eight weight rows, the up rows' and then the gate rows'
@@ -434,8 +440,8 @@ void launch_down_kernel(const Params &p, hipStream_t stream) {
 }
 
 /// Eight columns and sixteen wavefronts a workgroup where each CU gets one at most, else sixteen columns and eight
-/// wavefronts (128 experts of 2048 x 768, T=16: 50 us against 75, T=64 98 against 125; 64 of 4096 x 1408, T=64 185
-/// against 140).
+/// wavefronts (128 experts of 2048 x 768, T=16: 51 us against 78, T=64 98 against 129; 64 of 4096 x 1408, T=64 184
+/// against 141).
 template <class T, bool kWhole, bool kOnce>
 void launch_down(const Params &p, hipStream_t stream) {
   const bool narrow = ceil_div(p.hidden, 8) <= 256;
@@ -448,7 +454,7 @@ void launch_down(const Params &p, hipStream_t stream) {
 
 template <class T, bool kOnce>
 void launch_both(const Params &p, bool whole_x, bool whole_gated, hipStream_t stream) {
-  constexpr int kCols = 16;  // (32: T=64 134 us against 137, T=1 14.2 against 12.3; 64: 166 and 22.7)
+  constexpr int kCols = 16;  // (32: T=64 134 us against 136, T=1 14.2 against 12.3)
   const int64_t bound = p.experts + p.routes / p.job_tokens;  // of the jobs, without a look at the ids
   const dim3 grid(static_cast<uint32_t>(ceil_div(p.padded, kCols)), static_cast<uint32_t>(p.routes < bound ? p.routes : bound));
   if (whole_x) hipLaunchKernelGGL((gate_up_kernel<T, true, kOnce, kCols>), grid, dim3(kThreads), 0, stream, p);
@@ -457,9 +463,10 @@ void launch_both(const Params &p, bool whole_x, bool whole_gated, hipStream_t st
 }
 
 /// Jobs of at most 4, 8 or 16 tokens, by the tokens that an expert expects: the fewer, the less gated data the second kernel
-/// loads (128 experts, top 8, gate_up and down: T=16, one token an expert, 86 + 50 us with four, 86 + 57 with eight;
-/// T=64, four an expert, 194 + 106, 137 + 98 and with sixteen 146 + 115). Where an expert seldom has a second
-/// job its weights are loaded past the caches (T=64 151 -> 137; eight experts of 16 tokens 15 -> 19).
+/// loads (128 experts, top 8, gate_up and down: T=16, one token an expert, 86 + 51 us with four, 85 + 59 with eight;
+/// T=64, four an expert, 159 + 106, 137 + 100 and with sixteen 133 + 116; 64 experts of 4096 x 1408, eight tokens
+/// each, 337 + 230, 281 + 185, 244 + 166). Where an expert seldom has a second job its weights are loaded past the caches
+/// (T=64 151 + 101 us without that, eight experts of 16 tokens 15 + 16 without and 19 + 19 with it).
 template <class T>
 void launch(Params &p, bool whole_x, bool whole_gated, hipStream_t stream) {
   p.job_tokens = p.tokens <= 4 || p.routes <= 2 * p.experts ? 4 : p.tokens <= 8 || p.routes <= 6 * p.experts ? 8 : 16;
