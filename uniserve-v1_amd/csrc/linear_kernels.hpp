@@ -147,7 +147,7 @@ double cost_of(const LinearParams &p, bool gated, const Cost &c) {
 }
 
 /// Whether a product with adapters has a shape at all: the largest f16 tiles, which add the adapters' products through
-/// registers, spill sums (8192 x 4096 x 2048, rank 16, twelve runs: 256 x 256 164 us, 128 x 256 158).
+/// registers, spill sums (8192 x 4096 x 2048, rank 16, twelve runs: 164 us with 256 x 256, 158 with the largest left).
 template <class T, class S, class P>
 constexpr bool kServes = !(std::is_same<P, AdapterParams>::value && std::is_same<T, F16>::value) || S::kMB * S::kNB <= 16;
 
@@ -254,8 +254,7 @@ void launch_low_rank(const AdapterParams &a, bool gated, hipStream_t stream) {
   static_cast<AdapterParams &>(p) = a;
   p.width = layout.width, p.groups = layout.groups, p.halves = gated ? 2 : 1;
   p.n = static_cast<int64_t>(p.halves) * layout.groups * layout.width;
-  // Rows of up to sixteen adapters or more are few rows' (a decode step's), and tiles of sixteen rows; of 32 rows and
-  // more tiles, few have several. Workgroups share out a tile's adapters while there are fewer tiles than CUs
+  // Tiles that name many adapters are those of few rows (a decode step); of many rows' tiles, few name several. Workgroups share out a tile's adapters while there are fewer tiles than CUs
   // (777 x 2048, rank 64 gated, five runs: 9.4 us, one workgroup a tile 14.5; 8192 rows, rank 64, twelve runs: 17.5,
   // with two a tile 19.5).
   const auto launch_shape = [&](auto shape, auto by_dma) {
