@@ -13,7 +13,7 @@
 // in place. Rows without a route are the residual, or zeros.
 //
 // Sums are FP32. Between the products a gated value is held as a pair of the type's elements (the value and its rounding
-// error: 16 bits of significand; f16 pairs at 2^-6 of the value, so that they reach 2^22), and the output is rounded once.
+// error: 16 bits of significand; f16 pairs at 2^-6 of the value, so that they reach 2^22 and are infinite beyond), and the output is rounded once.
 // A row's result does not depend on the other rows. What an expert holds, infinities and NaN too, reaches the rows
 // routed to it and no others.
 //

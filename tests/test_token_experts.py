@@ -245,6 +245,33 @@ def test_infinities_and_nans_stay_with_their_rows(device, tokens, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("tokens", [3, 7, 16])
+def test_gated_values_past_their_pairs_are_infinite(device, tokens, dtype):
+    """Finite in FP32, an infinity in the pair's element: up times gate is 2^24 (f16 pairs reach 2^22) or, in bf16,
+    nearly 2^128. The row is infinite, not NaN; the others are as they were."""
+    announce("token_experts past the pairs", tokens, dtype)
+    hidden, width, experts = 64, 72, 2
+    x = torch.zeros((tokens, hidden), dtype=dtype, device=device)
+    # (silu(g) is g in FP32 for these gates. bf16: 255 * 2^57 times 2^63 + 2^55 is (1 - 2^-16) 2^128, finite, and above
+    # (1 - 2^-9) 2^128, from where bf16 rounds to an infinity.)
+    up, gates = ((4096.0, 0.0), (4096.0, 0.0)) if dtype == F16 else ((255 * 2.0**57, 0.0), (2.0**63, 2.0**55))
+    x[0, :2], x[1:, 2] = 1.0, 1.0
+    up_gate = torch.zeros((experts, 2 * width, hidden), dtype=dtype, device=device)
+    up_gate[:, :width, 0], up_gate[:, :width, 1] = up
+    up_gate[:, width:, 0], up_gate[:, width:, 1] = gates
+    up_gate[:, :, 2] = 1.0
+    down = torch.full((experts, hidden, width), 0.5, dtype=dtype, device=device)
+    ids = (torch.arange(tokens, device=device) % 2).int()[:, None].contiguous()
+    call = dict(ids=ids, weights=torch.ones((tokens, 1), device=device), up_gate=up_gate, down=down)
+    got = ops.token_experts(x, **call)
+    assert (got[0] == float("inf")).all()
+    plain = x.clone()
+    plain[0] = plain[1]
+    assert torch.equal(got[1:], ops.token_experts(plain, **call)[1:]) and got[1:].isfinite().all()
+
+
+@pytest.mark.gpu
 def test_large_gated_values_of_f16(device):
     """Gated values beyond f16's largest number, which the down product brings back."""
     announce("token_experts f16 range")

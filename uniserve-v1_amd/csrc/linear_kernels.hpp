@@ -254,9 +254,9 @@ void launch_low_rank(const AdapterParams &a, bool gated, hipStream_t stream) {
   static_cast<AdapterParams &>(p) = a;
   p.width = layout.width, p.groups = layout.groups, p.halves = gated ? 2 : 1;
   p.n = static_cast<int64_t>(p.halves) * layout.groups * layout.width;
-  // Tiles that name many adapters are those of few rows (a decode step); of many rows' tiles, few name several. Workgroups share out a tile's adapters while there are fewer tiles than CUs
-  // (777 x 2048, rank 64 gated, five runs: 9.4 us, one workgroup a tile 14.5; 8192 rows, rank 64, twelve runs: 17.5,
-  // with two a tile 19.5).
+  // Tiles that name many adapters are those of few rows (a decode step); of many rows' tiles, few name several.
+  // Workgroups share out a tile's adapters while there are fewer tiles than CUs (777 x 2048, rank 64 gated, five runs:
+  // 9.4 us, one workgroup a tile 14.5; 8192 rows, rank 64, twelve runs: 17.5, with two a tile 19.5).
   const auto launch_shape = [&](auto shape, auto by_dma) {
     using S = decltype(shape);
     const int64_t spare = 256 / tiles_of<S>(p, false);

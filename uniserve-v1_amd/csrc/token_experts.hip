@@ -277,7 +277,8 @@ __global__ void __launch_bounds__(kThreads) gate_up_kernel(Params p) {
     const uint16_t value = T::from_f32(v);
     const float error = v - T::to_f32(value);
     to[0] = value;
-    to[kLine] = T::from_f32(error == error ? error : 0.0f);
+    // (a value that is not finite, or rounds to an infinity, has no error: the pair's sum is the value)
+    to[kLine] = T::from_f32(__builtin_fabsf(error) < __builtin_inff() ? error : 0.0f);
   }
 }
 
