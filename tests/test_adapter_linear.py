@@ -385,6 +385,25 @@ def test_f16_rank_values_of_any_size(device, m, size):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("m", [1, 40, 777, 4096])
+def test_rank_values_past_bf16_are_infinite(device, m):
+    """255 * 2^57 times 2^63 + 2^55 is (1 - 2^-16) 2^128: finite in FP32 and above (1 - 2^-9) 2^128, from where bf16 rounds
+    to an infinity. The row is infinite, not NaN; the others are as they were."""
+    announce("adapter past bf16", m)
+    k, n, rank = 64, 2048, 16
+    x = torch.zeros((m, k), dtype=BF16, device=device)
+    x[0, :2], x[1:, 2] = 255 * 2.0**57, 1.0
+    w = torch.zeros((n, k), dtype=BF16, device=device)
+    down = torch.zeros((2, rank, k), dtype=BF16, device=device)
+    down[0, 0, 0], down[0, 0, 1], down[:, :, 2] = 2.0**63, 2.0**55, 1.0
+    up = torch.full((2, n, rank), 0.5, dtype=BF16, device=device)
+    adapter = (torch.arange(m, device=device) % 2).int()
+    got = ops.adapter_linear(x, w, down, up, adapter)
+    assert (got[0] == float("inf")).all()
+    assert (got[1:] == rank / 2).all()
+
+
+@pytest.mark.gpu
 def test_stacks_past_4_gib(device):
     """An adapter whose factors lie past 4 GiB, and rows of one that are 8 MiB apart."""
     announce("adapter far stacks")

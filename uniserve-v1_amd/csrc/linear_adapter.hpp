@@ -225,7 +225,8 @@ struct RankColumns {
     for (int i = 0; i < 4; ++i) {
       values[i] = T::pack2(v[2 * i], v[2 * i + 1]);
       const float low = v[2 * i] - T::low(values[i]), high = v[2 * i + 1] - T::high(values[i]);
-      errors[i] = T::pack2(low == low ? low : 0.0f, high == high ? high : 0.0f);
+      // (a value that is not finite, or rounds to an infinity, has no error: the pair's sum is the value)
+      errors[i] = T::pack2(__builtin_fabsf(low) < __builtin_inff() ? low : 0.0f, __builtin_fabsf(high) < __builtin_inff() ? high : 0.0f);
     }
     char *to = p.low + m * LowLayout(p.rank).row_bytes(p.halves) + at;
     *reinterpret_cast<u32x4 *>(to) = values;
