@@ -251,7 +251,8 @@ void launch_shape(const AddNormParams &p, hipStream_t stream) {
 /// wavefront a row 60 and 99 (its registers leave room for one wavefront a SIMD); 64 x 4096: 2.9 and 3.5, 3.3
 /// and 4.0, 4.1 and 5.2, 6.5 and 8.6. Bound by the bytes from some hundred rows on (8192 x 4096 at 6.8 TB/s
 /// on the same tensors again and again, 4.5 over three sets, where a copy of 4 GiB runs at 4.7), below by the launch
-/// and the row's chain of loads and sums (one row of 2048 2.4 us, 2.9 with both norms). Rows of more than 16384 elements spill registers.
+/// and the row's chain of loads and sums (one row of 2048 2.4 us, 2.9 with both norms). Rows of more than 16384
+/// elements spill registers.
 template <class X, class R>
 void launch(const AddNormParams &p, hipStream_t stream) {
   const int32_t chunks = ceil_div(p.width, 8);
