@@ -11,6 +11,8 @@ Behind the sum follow the activation, the gate, the residual and the rounding of
 """
 
 import ctypes
+import subprocess
+from pathlib import Path
 
 import pytest
 import torch
@@ -154,6 +156,36 @@ def test_workspace_sizes():
     size = ops.adapter_workspace
     assert size(1, 1) == 2 * 48 and size(10, 8) == 10 * 2 * 48 and size(1, 16) == 2 * 48 and size(3, 64) == 3 * 2 * 144
     assert size(2, 96) == 2 * 2 * 2 * 144 and size(0, 8) == 0 and size(-1, 8) == 0 and size(4, 1025) == 0
+
+
+def test_lanes_read_within_their_row(tmp_path):
+    """Every address that the second product's lanes take from a row's rank values, for each rank and half: the bytes
+    read end within the row, as the workspace ends with the last one."""
+    (tmp_path / "reads.cpp").write_text("""
+#include <cstdio>
+#include "low_layout.hpp"
+int main() {
+  for (int rank = 1; rank <= 512; ++rank) {
+    const uniserve::linear::LowLayout layout(rank);
+    for (int halves = 1; halves <= 2; ++halves)
+      for (int part = 0; part < halves * layout.groups; ++part) {
+        const int64_t group = static_cast<int64_t>(part) * layout.group_bytes(), row = layout.row_bytes(halves);
+        for (int g = 0; g < 4; ++g) {
+          int64_t end = group + layout.piece_at(g) + 16;
+          if (layout.width == 32 && group + layout.errors_at(g) + 16 > end) end = group + layout.errors_at(g) + 16;
+          if (group + layout.factor_at() + 4 > end) end = group + layout.factor_at() + 4;
+          if (end > row || layout.piece_at(g) < 0 || (layout.has_piece(g) && layout.piece_at(g) != 16 * g))
+            return std::printf("rank %d, %d halves, group %d, lanes %d: %lld of %lld bytes", rank, halves, part, g,
+                               static_cast<long long>(end), static_cast<long long>(row)), 1;
+        }
+      }
+  }
+}
+""")
+    csrc = Path(__file__).resolve().parent.parent / "uniserve-v1_amd" / "csrc"
+    subprocess.run(["g++", "-std=c++17", "-I", csrc, tmp_path / "reads.cpp", "-o", tmp_path / "reads"], check=True)
+    ran = subprocess.run([tmp_path / "reads"], capture_output=True, text=True)
+    assert ran.returncode == 0, ran.stdout
 
 
 def test_python_refusals():

@@ -5,6 +5,7 @@
 #pragma once
 
 #include "common.hpp"
+#include "low_layout.hpp"
 #include "uniserve_adapter_linear.h"
 
 namespace uniserve {
@@ -23,18 +24,6 @@ struct LinearParams {
   int32_t out_f32;
   int32_t activation;
   int32_t by_dma;        ///< input and weight rows suit the tile kernels' loads
-};
-
-/// Where a row's rank values lie between the adapters' two products, group by group of at most 32 ranks (gated: the
-/// up half's groups, then the gate half's): `width` elements that hold the values rounded, as many their errors, and
-/// the group's factor (FP32, f16 only: the power of two that both were divided by), padded to 16 bytes.
-struct LowLayout {
-  int32_t width;   ///< ranks of a group: 8, 16 or 32
-  int32_t groups;  ///< of a half
-  __host__ __device__ explicit LowLayout(int64_t rank)
-      : width(rank <= 8 ? 8 : rank <= 16 ? 16 : 32), groups(static_cast<int32_t>((rank + width - 1) / width)) {}
-  __host__ __device__ int32_t group_bytes() const { return 4 * width + 16; }
-  __host__ __device__ int64_t row_bytes(int halves) const { return static_cast<int64_t>(halves) * groups * group_bytes(); }
 };
 
 /// A product whose rows have low-rank adapters.

@@ -306,14 +306,13 @@ __device__ __forceinline__ void add_low_rank(const AdapterParams &p, floatx4 (&a
   // row's, and drop what they make of them).
   auto low_of = [&](int b) {
     const int64_t m = m_first + b * 16 + r16;
-    return p.low + (m < p.m ? m : p.m - 1) * layout.row_bytes(kHalves) + 16 * g;
+    return p.low + (m < p.m ? m : p.m - 1) * layout.row_bytes(kHalves);
   };
   // The lane's chunk of eight ranks in the up rows. Up to rank 16 its place in a group is that of a value or of an error
   // (the errors follow the values), else one of each.
   const bool both = layout.width <= 16;
   const int up_at = (layout.width == 32 ? g : layout.width == 16 ? g & 1 : 0) * 8;
-  const bool held = layout.width >= 16 || g < 2;
-  const int factor_at = 4 * layout.width - 16 * g;
+  const bool held = layout.has_piece(g);
   auto products = [&](auto errors_too, int group) {
     constexpr bool kErrors = decltype(errors_too)::value;
     const int64_t at = group * 32 + up_at;
@@ -349,9 +348,9 @@ __device__ __forceinline__ void add_low_rank(const AdapterParams &p, floatx4 (&a
         for (int i = 0; i < kPair; ++i) {
           if (first + i >= MB) continue;
           const char *from = low_of(first + i) + of;
-          values[h][i] = *reinterpret_cast<const u32x4 *>(from);
-          if constexpr (kErrors) errors[h][i] = *reinterpret_cast<const u32x4 *>(from + 64);
-          if constexpr (std::is_same<T, F16>::value) factor[h][i] = *reinterpret_cast<const float *>(from + factor_at);
+          values[h][i] = *reinterpret_cast<const u32x4 *>(from + layout.piece_at(g));
+          if constexpr (kErrors) errors[h][i] = *reinterpret_cast<const u32x4 *>(from + layout.errors_at(g));
+          if constexpr (std::is_same<T, F16>::value) factor[h][i] = *reinterpret_cast<const float *>(from + layout.factor_at());
         }
       }
       const u32x4 nothing{0, 0, 0, 0};
