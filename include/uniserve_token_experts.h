@@ -15,7 +15,7 @@
 // Sums are FP32. Between the products a gated value is held as a pair of the type's elements (the value and its rounding
 // error: 16 bits of significand; f16 pairs at 2^-6 of the value, so that they reach 2^22 and are infinite beyond), and the output is rounded once.
 // A row's result does not depend on the other rows. What an expert holds, infinities and NaN too, reaches the rows
-// routed to it and no others.
+// routed to it and no others, and is there what the formula makes of it.
 //
 // `workspace` is uniserve_token_experts_workspace(tokens, top, width) bytes, 16-byte aligned; its contents before the
 // call do not matter and after it are of no use. Calls that may overlap in time need one each. Nothing is allocated and

@@ -244,6 +244,42 @@ def test_infinities_and_nans_stay_with_their_rows(device, tokens, dtype):
     assert torch.equal(got[~touched], want[~touched]) and torch.isnan(got[touched]).all()
 
 
+def assert_as_the_formula(got, y):
+    """NaN and either infinity exactly where the formula in 64 bits has them."""
+    got = got.double().cpu()
+    assert torch.equal(torch.isnan(got), torch.isnan(y))
+    assert torch.equal(got == float("inf"), y == float("inf")) and torch.equal(got == float("-inf"), y == float("-inf"))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tokens", [1, 3, 7, 20, 64])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("exact", [False, True])
+def test_infinite_weights_give_the_formula_s_infinities(device, tokens, dtype, exact):
+    """One infinity in a row of `down` is an infinity of the gated value's sign, two that oppose are NaN; gated values that
+    one element holds (of which nothing is left for the pair's other one), and any."""
+    announce("token_experts infinite weights", tokens, dtype, exact)
+    call = inputs(tokens, 136, 70, 6, 2, dtype)
+    if exact:  # up 1, -1 or 2, gate 64: gelu_tanh(64) is 64
+        call["x"].zero_()[:, 0] = torch.tensor([1.0, -1.0, 2.0], dtype=dtype, device=device).repeat(22)[:tokens]
+        call["x"][:, 1] = 64.0
+        call["up_gate"][:] = 0
+        call["up_gate"][:, :70, 0] = 1.0
+        call["up_gate"][:, 70:, 1] = 1.0
+    call["activation"] = "gelu_tanh"
+    want = ops.token_experts(**call)
+    inf = float("inf")
+    call["down"][:, 5, 7], call["down"][:, 9, 64], call["down"][3, 135, 69] = inf, -inf, inf
+    call["down"][:, 11], call["down"][2, 20, 3] = inf, float("nan")
+    call["down"][:, 12, :2] = torch.tensor([inf, -inf], dtype=dtype)
+    got = ops.token_experts(**call)
+    y = reference(**call)[0]
+    assert_as_the_formula(got, y)
+    assert not torch.isfinite(y[:, [5, 9, 11, 12]]).any() and torch.isinf(y[:, [5, 9]]).any()
+    finite = torch.isfinite(y).to(device)
+    assert torch.equal(got[finite], want[finite])
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [F16, BF16])
 @pytest.mark.parametrize("tokens", [3, 7, 16])

@@ -391,10 +391,13 @@ __global__ void __launch_bounds__(kSets *kThreads) down_kernel(Params p) {
     float *total = totals[all_wave][entry.route / p.top];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      // (The errors' sum is added to the values' for any kTokens: the order of a row's additions is one.)
-      float v;
-      if constexpr (kApart == 1) v = acc[0][e] + __shfl_xor(acc[0][e], kTokens);
-      else v = acc[0][e] + acc[1][e];
+      // (The errors' sum is added to the values' for any kTokens: the order of a row's additions is one. Where it is not
+      // finite a weight is not: the values' sum alone is what the weights make of the row - an exact value's error
+      // times an infinity would be NaN, another's may be the other infinity.)
+      float errors;
+      if constexpr (kApart == 1) errors = __shfl_xor(acc[0][e], kTokens);
+      else errors = acc[1][e];
+      const float v = acc[0][e] + (__builtin_fabsf(errors) < __builtin_inff() ? errors : 0.0f);
       if (r16 < job.count && (kGroups > 1 || g < 2)) total[4 * g + e] = __builtin_fmaf(weight, v, total[4 * g + e]);
     }
     clear();
