@@ -182,6 +182,15 @@ __device__ __forceinline__ float row16_max(float x) {
 
 __device__ __forceinline__ int lane_id() { return static_cast<int>(threadIdx.x & (kWave - 1)); }
 
+/// Between LDS writes of a wavefront's lanes and what its other lanes read of them. The hardware keeps a wavefront's order;
+/// without this the compiler may take a lane's earlier value for one that another lane has written since (it does, where
+/// only some lanes write). Costs no instruction.
+__device__ __forceinline__ void wave_fence() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront", "local");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront", "local");
+}
+
 __device__ __forceinline__ uint64_t ballot(bool predicate) { return __ballot(predicate); }
 
 /// The lanes of the wave whose `key` equals this lane's, for keys below 2^bits.

@@ -225,8 +225,10 @@ __global__ void __launch_bounds__(kThreads) gate_up_kernel(Params p) {
   };
   auto multiply = [&](const Stage &s) {
     const int r = lane >> 3, piece = lane & 7;
+    wave_fence();  // (the stage before has been read)
 #pragma unroll
     for (int i = 0; i < kGroups; ++i) regroup[wave][i * 64 + r * 8 + (piece ^ r)] = s.w[i];
+    wave_fence();
 #pragma unroll
     for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
@@ -256,6 +258,7 @@ __global__ void __launch_bounds__(kThreads) gate_up_kernel(Params p) {
     }
   }
   // The wavefronts' sums, each in its own buffer: [block][token][row].
+  wave_fence();
   float *sums = reinterpret_cast<float *>(&regroup[0][0]);
   constexpr int kWaveSums = kGroups * 64 * 4;
   static_assert(kWaveSums >= kBlocks * 256, "a wavefront's sums fit its buffer");
@@ -365,6 +368,7 @@ __global__ void __launch_bounds__(kSets *kThreads) down_kernel(Params p) {
   };
   clear();
   auto multiply = [&](const Stage &s) {
+    wave_fence();  // (the stage before has been read)
 #pragma unroll
     for (int i = 0; i < kGroups; ++i) regroup[all_wave][i * 64 + lane / 8 * 8 + ((lane & 7) ^ (lane / 8))] = s.w[i];
     // Chunk c (eight values, then eight errors) of a token's line lies at c ^ 4 token: four tokens' chunks in all banks.
@@ -373,6 +377,7 @@ __global__ void __launch_bounds__(kSets *kThreads) down_kernel(Params p) {
       const int token = i * 4 + lane / 16;
       lines_of[all_wave][token * 16 + ((lane & 15) ^ (token * 4 & 15))] = s.gated[i];
     }
+    wave_fence();
     // Operand columns: the tokens' values and then their errors, or, of sixteen tokens, one after the other.
     const int token = r16 % kTokens, errors = kTokens < 16 ? r16 / kTokens % 2 * 8 : 0;
     const u32x4 *line = &lines_of[all_wave][token * 16];
