@@ -12,8 +12,9 @@
 // is UNISERVE_ACTIVATION_SILU or _GELU_TANH. residual (the output's type, or null) may be the output itself,
 // in place. Rows without a route are the residual, or zeros.
 //
-// Sums are FP32. Between the products a gated value is held as a pair of the type's elements (the value and its rounding
-// error: 16 bits of significand; f16 pairs at 2^-6 of the value, so that they reach 2^22 and are infinite beyond), and the output is rounded once.
+// Sums are FP32. In the second product a gated value is a pair of the type's elements, the value and its rounding error,
+// and the output is rounded once. bf16: 16 bits of significand. f16: 64 consecutive values of a route share a power of two,
+// so that values of any size are served; 22 bits, or 2^-25 of the largest of the 64 where a value is small beside it.
 // A row's result does not depend on the other rows. What an expert holds, infinities and NaN too, reaches the rows
 // routed to it and no others, and is there what the formula makes of it.
 //

@@ -317,6 +317,57 @@ def test_large_gated_values_of_f16(device):
     assert_near(ops.token_experts(**call), reference(**call))
 
 
+def reference_of_f16(x, ids, weights, up_gate, down, activation="silu"):
+    """The output in 64 bits and how far the f16 kernels may be from it, by the tolerance above but for the gated values: a
+    line's (64 of a route) are FP32 until they are split into two elements, by a power of two that brings the line's
+    largest to [1, 2). The first element leaves at most 2^-11 of a value, the second is off by half a step of that, 2^-23
+    of the value, or by half a subnormal step, 2^-25 of at most the line's largest. A line's products are scaled back,
+    2 u, and added: the 2 (2 I + 2) u hold that many additions twice."""
+    x, weights, ids = x.double().cpu(), weights.double().cpu(), ids.cpu().long()
+    tokens, hidden = x.shape
+    experts, width = up_gate.shape[0], up_gate.shape[1] // 2
+    y, size, off = (torch.zeros(tokens, hidden, dtype=torch.float64) for _ in range(3))
+    for e in range(experts):
+        rows, places = torch.nonzero(ids == e, as_tuple=True)
+        if rows.numel() == 0:
+            continue
+        w1, w2 = up_gate[e].double().cpu(), down[e].double().cpu()
+        both, s = x[rows] @ w1.t(), x[rows].abs() @ w1.abs().t()
+        d = 2 * (hidden + 1) * U * s
+        up, gate = both[:, :width], both[:, width:]
+        act = activated(gate, activation)
+        h = up * act
+        d = act.abs() * d[:, :width] + 1.13 * d[:, width:] * (up.abs() + d[:, :width]) + 128 * U * h.abs()
+        most = torch.cat([line.amax(1, keepdim=True).expand_as(line) for line in (h.abs() + d).split(64, 1)], 1)
+        d = d + 2.0**-23 * (h.abs() + d) + 2.0**-25 * most
+        w = weights[rows, places][:, None]
+        part = (h.abs() + d) @ w2.abs().t()
+        y.index_add_(0, rows, w * (h @ w2.t()))
+        size.index_add_(0, rows, w.abs() * part)
+        off.index_add_(0, rows, w.abs() * (d @ w2.abs().t() + (2 * (2 * width + 2) + 4) * U * part))
+    off = off + (ids.shape[1] + 6) * U * size
+    return y, off + rounding(y.abs() + off, F16)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tokens, experts", [(1, 8), (4, 8), (8, 8), (16, 8), (40, 8), (64, 128)])
+@pytest.mark.parametrize("size", [2.0**-12, 2.0**-8, 2.0**-5, 2.0**-2, 2.0**2, 2.0**6])
+def test_f16_gated_values_of_any_size(device, tokens, experts, size):
+    """Gated values from some 2^-26 to some 2^20, lines of one size and of many, brought to ordinary outputs by `down`."""
+    announce("token_experts f16 sizes", tokens, experts, size)
+    call = inputs(tokens, 264, 200, experts, 4, F16)
+    call["x"] = (call["x"].float() * size).to(F16)
+    h = reference_of_f16(**{**call, "down": torch.eye(200, dtype=F16).repeat(2, 1)[None, :264].expand(experts, -1, -1)})[0]
+    call["down"] = (call["down"].float() / (0.05 * h.abs().mean().item() * 8)).clamp(-60000, 60000).to(F16)
+    got, want = ops.token_experts(**call), reference_of_f16(**call)
+    assert 2.0**-8 < want[0].abs().mean() < 2.0**12
+    assert_near(got, want, "one size")
+    up_gate = call["up_gate"].float()
+    up_gate[:, :200] *= 2.0 ** -(torch.arange(200, device=device) * 7 % 13).float()[:, None]
+    call["up_gate"] = up_gate.to(F16)
+    assert_near(ops.token_experts(**call), reference_of_f16(**call), "many sizes")
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("tokens", [1, 12, 64])
 def test_results_repeat_and_rows_do_not_depend_on_the_others(device, tokens):

@@ -180,6 +180,18 @@ __device__ __forceinline__ float row16_max(float x) {
   return x;
 }
 
+/// The same of unsigned integers (zeros from absent lanes drop out, so each step is one instruction).
+__device__ __forceinline__ uint32_t row16_max(uint32_t x) {
+  const auto with = [](auto of, uint32_t v) {
+    const uint32_t other = static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), decltype(of)::value, 0xf, 0xf, false));
+    return v > other ? v : other;
+  };
+  x = with(std::integral_constant<int, 0xb1>{}, x);
+  x = with(std::integral_constant<int, 0x4e>{}, x);
+  x = with(std::integral_constant<int, 0x141>{}, x);
+  return with(std::integral_constant<int, 0x140>{}, x);
+}
+
 __device__ __forceinline__ int lane_id() { return static_cast<int>(threadIdx.x & (kWave - 1)); }
 
 /// Between LDS writes of a wavefront's lanes and what its other lanes read of them. The hardware keeps a wavefront's order;

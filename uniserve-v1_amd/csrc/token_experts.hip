@@ -51,15 +51,18 @@ struct Params {
   int32_t *job_count;
   Job *jobs;
   Entry *entries;
-  uint16_t *gated;  ///< [routes, lines, 2, 64]: a line's values, then their errors
+  uint16_t *gated;  ///< [routes, lines, 2, 64]: a line's values, then their errors; f16: [routes, lines, 64] of FP32
   int64_t x_stride, residual_stride, out_stride;
   int32_t tokens, top, routes, hidden, width, padded, experts, first_expert, activation;
   int32_t job_tokens;  ///< the most of a job: 4, 8 or 16
 };
 
-/// Values of f16 pairs are held at this part of themselves.
+/// Whether the gated values are FP32 between the kernels: f16's range does not hold them, so the second kernel splits each
+/// line into two elements by a power of two of the line's own. bf16's does, and the first kernel splits them once.
+/// (The first kernel's workgroups see sixteen columns of a line each, not its largest value. The split costs the second kernel
+/// 1 to 10 us: f16, T=1 22.6 us for both kernels against 21.6 with bf16 pairs, T=16 142 against 135, T=64 243 against 234.)
 template <class T>
-constexpr float kHeld = std::is_same<T, F16>::value ? 0.015625f : 1.0f;
+constexpr bool kSplitLate = std::is_same<T, F16>::value;
 
 /// Eight elements of a row from `at` on, zeros past its end; kWhole: rows of whole 16-byte pieces.
 template <bool kWhole>
@@ -275,7 +278,11 @@ __global__ void __launch_bounds__(kThreads) gate_up_kernel(Params p) {
     }
     if (column + c >= p.padded) continue;
     // (the padding: zeros)
-    const float v = column + c < p.width ? up * gate(gated, p.activation) * kHeld<T> : 0.0f;
+    const float v = column + c < p.width ? up * gate(gated, p.activation) : 0.0f;
+    if constexpr (kSplitLate<T>) {
+      reinterpret_cast<float *>(p.gated)[static_cast<int64_t>(job_route[token]) * p.padded + column + c] = v;
+      continue;
+    }
     uint16_t *to = p.gated + static_cast<int64_t>(job_route[token]) * 2 * p.padded + (column + c) / kLine * 2 * kLine + (column + c) % kLine;
     const uint16_t value = T::from_f32(v);
     const float error = v - T::to_f32(value);
@@ -286,6 +293,34 @@ __global__ void __launch_bounds__(kThreads) gate_up_kernel(Params p) {
 }
 
 // ---- down -------------------------------------------------------------------------------------------------
+
+/// A lane's four of a line's sixty-four FP32 values (sixteen lanes in a row hold one) as f16 elements and their errors, in
+/// parts of the power of two that brings the line's largest to [1, 2). At most 2^126, also where an infinity is the
+/// largest; NaN is passed over. What is not finite has NaN for its error, whose sum is then left out.
+struct LineSplit {
+  uint2 values, errors;
+  float factor;
+  __device__ __forceinline__ explicit LineSplit(floatx4 v) {
+    typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+    const float own = __builtin_fmaxf(__builtin_fmaxf(__builtin_fabsf(v[0]), __builtin_fabsf(v[1])),
+                                      __builtin_fmaxf(__builtin_fabsf(v[2]), __builtin_fabsf(v[3])));
+    uint32_t power = row16_max(__float_as_uint(own)) & 0x7f800000u;
+    power = power < (1u << 23) ? 1u << 23 : power;
+    power = power > (253u << 23) ? 253u << 23 : power;
+    factor = __uint_as_float(power);
+    const float scale = __uint_as_float((254u << 23) - power);
+    const auto pair = [](float lo, float hi) {
+      uint32_t bits = __builtin_bit_cast(uint32_t, f16x2{static_cast<_Float16>(lo), static_cast<_Float16>(hi)});
+      asm("" : "+v"(bits));  // (opaque: the elements are taken from the pair, not rounded a second time each)
+      return __builtin_bit_cast(f16x2, bits);
+    };
+    const f16x2 a = pair(v[0] * scale, v[1] * scale), b = pair(v[2] * scale, v[3] * scale);
+    const auto left = [&](float of, _Float16 value) { return static_cast<_Float16>(__builtin_fmaf(of, scale, -static_cast<float>(value))); };
+    const f16x2 c{left(v[0], a[0]), left(v[1], a[1])}, d{left(v[2], b[0]), left(v[3], b[1])};
+    values = uint2{__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b)};
+    errors = uint2{__builtin_bit_cast(uint32_t, c), __builtin_bit_cast(uint32_t, d)};
+  }
+};
 
 /// kCols output columns a workgroup, kSets sets of four wavefronts. A set takes the jobs of the experts whose number is its
 /// own modulo kSets, a wavefront a quarter of each job's lines; it keeps its own sums of all rows in LDS. (By the
@@ -302,6 +337,7 @@ __global__ void __launch_bounds__(kSets *kThreads) down_kernel(Params p) {
   __shared__ float totals[kSets * kWaves][kMostTokens][kCols];
   __shared__ u32x4 regroup[kSets * kWaves][kGroups * 64];
   __shared__ u32x4 lines_of[kSets * kWaves][kTokens * 16];
+  [[maybe_unused]] __shared__ float line_factor[kSets * kWaves][kTokens];
   const int count = *p.job_count;
   const int all_wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / kWave);
   const int wave = all_wave % kWaves, set = all_wave / kWaves;
@@ -375,24 +411,42 @@ __global__ void __launch_bounds__(kSets *kThreads) down_kernel(Params p) {
 #pragma unroll
     for (int i = 0; i < kTokens / 4; ++i) {
       const int token = i * 4 + lane / 16;
-      lines_of[all_wave][token * 16 + ((lane & 15) ^ (token * 4 & 15))] = s.gated[i];
+      if constexpr (kSplitLate<T>) {
+        const LineSplit split(__builtin_bit_cast(floatx4, s.gated[i]));
+        uint2 *line = reinterpret_cast<uint2 *>(&lines_of[all_wave][token * 16]);
+        const int piece = (lane & 15) >> 1, swap = token * 4 & 15;
+        line[(piece ^ swap) * 2 + (lane & 1)] = split.values;
+        line[((piece + 8) ^ swap) * 2 + (lane & 1)] = split.errors;
+        if ((lane & 15) == 0) line_factor[all_wave][token] = split.factor;
+      } else {
+        lines_of[all_wave][token * 16 + ((lane & 15) ^ (token * 4 & 15))] = s.gated[i];
+      }
     }
     wave_fence();
     // Operand columns: the tokens' values and then their errors, or, of sixteen tokens, one after the other.
     const int token = r16 % kTokens, errors = kTokens < 16 ? r16 / kTokens % 2 * 8 : 0;
     const u32x4 *line = &lines_of[all_wave][token * 16];
     auto chunk = [&](int c) { return line[c ^ (token * 4 & 15)]; };
+    floatx4 line_acc[kApart];
+#pragma unroll
+    for (int i = 0; i < kApart; ++i) line_acc[i] = kSplitLate<T> ? floatx4{0.0f, 0.0f, 0.0f, 0.0f} : acc[i];
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
       const u32x4 w = regroup[all_wave][(kGroups == 1 ? 0 : r16 >> 3) * 64 + (r16 & 7) * 8 + ((4 * half + g) ^ (r16 & 7))];
-      acc[0] = T::mfma(w, chunk(errors + 4 * half + g), acc[0]);
-      if constexpr (kApart == 2) acc[1] = T::mfma(w, chunk(8 + 4 * half + g), acc[1]);
+      line_acc[0] = T::mfma(w, chunk(errors + 4 * half + g), line_acc[0]);
+      if constexpr (kApart == 2) line_acc[1] = T::mfma(w, chunk(8 + 4 * half + g), line_acc[1]);
     }
+    [[maybe_unused]] float factor = 1.0f;
+    if constexpr (kSplitLate<T>) factor = line_factor[all_wave][token];
+#pragma unroll
+    for (int i = 0; i < kApart; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[i][e] = kSplitLate<T> ? __builtin_fmaf(line_acc[i][e], factor, acc[i][e]) : line_acc[i][e];
     if (++line_at < line_count) return;
     // The job's rows are complete (of this wavefront's lines): lane r16's token, rows 4 g .. 4 g + 3.
     const Job job = jobs[job_at];
     const Entry entry = entries[job.first + (r16 < job.count ? r16 : 0)];
-    const float weight = entry.weight * (1.0f / kHeld<T>);
+    const float weight = entry.weight;
     float *total = totals[all_wave][entry.route / p.top];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
@@ -410,7 +464,7 @@ __global__ void __launch_bounds__(kSets *kThreads) down_kernel(Params p) {
     ++job_at;
   };
   const int units = own_jobs * line_count;
-  constexpr int kAhead = 4;
+  constexpr int kAhead = kSplitLate<T> && kTokens == 16 ? 3 : 4;  // (four spill 31 to 82 registers there)
   Stage stages[kAhead];
 #pragma unroll
   for (int i = 0; i < kAhead; ++i)
