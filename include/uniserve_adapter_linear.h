@@ -11,7 +11,7 @@
 // own: down [adapters, 2 rank, k], the up half's rows and then the gate half's; up [adapters, 2 n, rank]
 // likewise. Adapters of a smaller rank than the stack's are padded with zeros. An index below 0 or not below
 // `adapters` names none: such a row gets the product alone, and no adapter is read for it. What an adapter
-// holds, infinities and NaN too, reaches the rows that name it and no others.
+// holds, infinities and NaN too, reaches the rows that name it and no others, and is there what the formula makes of it.
 //
 // down, up and the rows are of one type (bf16 or f16), their last axes contiguous; scales are FP32, or null
 // for ones. Sums are FP32; between the factors a row's rank values are held as a pair of the type's elements

@@ -81,6 +81,13 @@ def assert_operator_bound(got, want, n, what, envelope=True):
     assert (diff <= atol + rtol * peak).all(), f"{what}: max diff {diff.max():.3e} > {atol + rtol * peak:.3e}"
 
 
+def assert_as_the_formula(got, y):
+    """NaN and either infinity exactly where the formula in 64 bits has them."""
+    got = got.double().cpu()
+    assert torch.equal(torch.isnan(got), torch.isnan(y))
+    assert torch.equal(got == float("inf"), y == float("inf")) and torch.equal(got == float("-inf"), y == float("-inf"))
+
+
 def sort_on_host(maps, tokens, top):
     """The device maps tensor as the oracle's dict."""
     m = maps.cpu().numpy()

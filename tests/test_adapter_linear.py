@@ -17,7 +17,7 @@ from pathlib import Path
 import pytest
 import torch
 
-from gpu_helpers import announce, kernels_of
+from gpu_helpers import announce, assert_as_the_formula, kernels_of
 from test_linear import BF16, F16, F32, KERNELS, U, activated, assert_near, normal, rounding
 from uniserve_moe import abi, ops
 
@@ -398,6 +398,72 @@ def test_infinities_and_nans_in_large_tiles(device, gated, shape, m, n, k, rank)
     assert not torch.isfinite(got[touched][:, [5, n - 1]]).any()
     kept = [c for c in range(n) if c not in (5, n - 1)]
     assert ((got[touched][:, kept] - want[touched][:, kept]).abs() <= tolerance[touched][:, kept]).all()
+
+
+#: The shapes that f16 rows have, too (the largest tiles do not serve them), and calls of one and two rows.
+F16_KERNELS = [case for case in KERNELS if not case[1].startswith(("256,256", "192,256"))]
+FEW = [(False, "", 1, 520, 136), (False, "", 2, 72, 264), (True, "", 1, 72, 136), (True, "", 2, 520, 72)]
+
+
+def columns_of(call, w, columns, halves):
+    """The call on some output columns alone."""
+    n = w.shape[0] // halves
+    rows = torch.tensor([c + h * n for h in range(halves) for c in columns], device=w.device)
+    return {**call, "w": w[rows], "up": call["up"][:, rows]}
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype, gated, shape, m, n, k", [(BF16, *case) for case in KERNELS + FEW] + [(F16, *case) for case in F16_KERNELS + FEW])
+@pytest.mark.parametrize("rank", [8, 24])
+def test_infinite_up_weights_give_the_formula_s_infinities(device, dtype, gated, shape, m, n, k, rank):
+    """Infinities and NaN in a few up rows, with rank values that one element holds (of which nothing is left for the pair's
+    other one) and with any, in tiles of one adapter and of several: NaN and either infinity where the formula has them, the
+    columns' other rows within the tolerance (large tiles make them again) and the other columns as they were."""
+    announce("adapter infinite up weights", dtype, shape, gated, m, n, k, rank)
+    halves, inf = 2 if gated else 1, float("inf")
+    entry = ops.adapter_gated_linear if gated else ops.adapter_linear
+    x, w = normal((m, k), 1, dtype=dtype), normal((n * halves, k), 2, 0.05, dtype)
+    for order, exact in ((lambda m, _: torch.zeros(m, dtype=torch.int32, device=device), True), (runs, False), (each_other, True)):
+        call = dict(stacks(4, rank, n, k, dtype, halves=halves), adapter=order(m, 4))
+        if exact:  # rank values 1, 2, .. 5 times the row's first element
+            call["down"][:] = 0
+            call["down"][:, :, 0] = (torch.arange(halves * rank, device=device) % 5 + 1).to(dtype)
+            call["scales"] = None
+        want = entry(x, w, **call)
+        columns = [0, 3, n // 2, n - 3, n - 1]
+        for i, c in enumerate(columns):
+            place = c + (n if gated and i % 2 else 0)
+            for a in (0, 2):
+                call["up"][a, place, (i * 5 + a) % rank] = (inf, -inf, inf, float("nan"), -inf)[i]
+        call["up"][0, n // 2, 0] = inf
+        got = entry(x, w, **call)
+        y, tolerance = reference(x, **columns_of(call, w, columns, halves), activation="silu" if gated else None, gated=gated)
+        assert_as_the_formula(got[:, columns], y)
+        finite = torch.isfinite(y)
+        assert ((got[:, columns].double().cpu() - y).abs()[finite] <= tolerance[finite]).all()
+        kept = torch.ones(n, dtype=torch.bool, device=device)
+        kept[columns] = False
+        assert torch.equal(got[:, kept], want[:, kept])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype, shape, m, n, k", [(BF16, *case[1:]) for case in KERNELS + FEW if case[0]] + [(F16, *case[1:]) for case in F16_KERNELS + FEW if case[0]])
+@pytest.mark.parametrize("rank", [8, 40])
+def test_infinite_rank_values_stay_in_their_half(device, dtype, shape, m, n, k, rank):
+    """An infinity in one half's first factor makes that half's sums infinite, and not the other's, in tiles of one adapter
+    and of several."""
+    announce("adapter infinite rank values", dtype, shape, m, n, k, rank)
+    x, w = normal((m, k), 1, dtype=dtype), normal((2 * n, k), 2, 0.05, dtype)
+    columns = sorted({0, 1, n // 3, n // 2, n - 2, n - 1})
+    for order in (lambda m, _: torch.zeros(m, dtype=torch.int32, device=device), runs, each_other):
+        call = dict(stacks(4, rank, n, k, dtype, halves=2), adapter=order(m, 4))
+        want = ops.adapter_gated_linear(x, w, **call)
+        call["down"][0, 1, 3], call["down"][2, rank + rank - 1, 5] = float("inf"), float("-inf")
+        got = ops.adapter_gated_linear(x, w, **call)
+        y = reference(x, **columns_of(call, w, columns, 2), activation="silu", gated=True)[0]
+        assert_as_the_formula(got[:, columns], y)
+        clean = (call["adapter"] != 0) & (call["adapter"] != 2)
+        assert torch.equal(got[clean], want[clean])
 
 
 @pytest.mark.gpu

@@ -15,7 +15,7 @@ import pytest
 import torch
 
 import test_expert_topk
-from gpu_helpers import announce, kernels_of
+from gpu_helpers import announce, assert_as_the_formula, kernels_of
 from test_linear import BF16, F16, F32, U, activated, assert_near, normal, rounding
 from uniserve_moe import abi, ops
 
@@ -242,13 +242,6 @@ def test_infinities_and_nans_stay_with_their_rows(device, tokens, dtype):
     touched = (call["ids"] == 4).any(1)
     touched[0] = True
     assert torch.equal(got[~touched], want[~touched]) and torch.isnan(got[touched]).all()
-
-
-def assert_as_the_formula(got, y):
-    """NaN and either infinity exactly where the formula in 64 bits has them."""
-    got = got.double().cpu()
-    assert torch.equal(torch.isnan(got), torch.isnan(y))
-    assert torch.equal(got == float("inf"), y == float("inf")) and torch.equal(got == float("-inf"), y == float("-inf"))
 
 
 @pytest.mark.gpu

@@ -26,6 +26,22 @@ __device__ __forceinline__ u32x4 load8_of(const uint16_t *row, int64_t at, int64
   else return load8(row, at, width);
 }
 
+/// Eight elements with zeros for those that are infinite or NaN, where `drop` says so. (What a value's error meets: the value
+/// itself meets the element, and an infinity times the error would be NaN or the other infinity.)
+template <class T>
+__device__ __forceinline__ u32x4 finite_only(u32x4 w, bool drop) {
+  typedef int16_t i16x2 __attribute__((ext_vector_type(2)));
+  constexpr bool kF16 = std::is_same<T, F16>::value;
+  constexpr uint32_t kExponents = kF16 ? 0x7c007c00u : 0x7f807f80u, kOne = kF16 ? 0x04000400u : 0x00800080u;
+  const uint32_t dropped = drop ? ~0u : 0u;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const i16x2 past = __builtin_bit_cast(i16x2, (w[i] & kExponents) + kOne);  // negative where all of the exponent is set
+    w[i] &= ~(__builtin_bit_cast(uint32_t, past >> 15) & dropped);
+  }
+  return w;
+}
+
 // ---- which adapters a tile names ---------------------------------------------------------------------------
 
 /// The distinct adapters of a tile's rows, one after the other, found by every wavefront alike.
@@ -70,18 +86,11 @@ struct NamedAdapters {
       if (mine) return true;
     }
   }
-  /// How many there are, from a copy; `mixed`: whether some of the tile's `rows` rows name another than the first, or none.
-  __device__ __forceinline__ int count(int rows, bool &mixed) const {
+  /// How many there are, from a copy.
+  __device__ __forceinline__ int count() const {
     NamedAdapters all = *this;
-    int found = 0, first_rows = 0;
-    while (all.next()) {
-      if (found == 0)
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (i < blocks) first_rows += __popcll(all.members[i]);
-      ++found;
-    }
-    mixed = found > 0 && first_rows < rows;
+    int found = 0;
+    while (all.next()) ++found;
     return found;
   }
   /// The first row of the current adapter.
@@ -128,9 +137,10 @@ __device__ __forceinline__ auto tile_adapters(const Rows &, int rows) {
   else return 0;
 }
 
-/// Makes those of a row's sums of eight columns again, from the row's own operands alone, that are not finite: in a tile
-/// whose rows name several adapters, the walk multiplies the others' up rows by zeros, which gives NaN where they are
-/// not finite. (What the row itself makes infinite or NaN stays so.)
+/// Makes those of a row's sums of eight columns again, from the row's own operands alone, that are not finite: the walk
+/// multiplies other adapters' up rows, pieces past a rank and, gated, one half's rank values by zeros, which gives NaN
+/// where they are not finite, and a weight by a value and by its error, which gives NaN where the weight is an
+/// infinity. (What the row itself makes infinite or NaN stays so.)
 template <class T, bool kGated>
 __device__ __forceinline__ void remake(const AdapterParams &p, int64_t m, int64_t n, int adapter, floatx4 (&sums)[2], floatx4 (&gates)[2]) {
   bool finite = true;
@@ -267,7 +277,8 @@ __device__ __forceinline__ int row_adapters(const RankParams &, int64_t) { retur
 /// column n_first on (gated: half of them the up rows', then the same columns' gate rows), some of the adapters that
 /// its rows name after the others; of `teams` wavefronts with the same sums, which are added up later, each takes
 /// its share of the adapters. Two matrix instructions per 32 ranks, over the values and over their errors, or, up to
-/// rank 16, one over both.
+/// rank 16, one over both. (What keeps infinite up rows from the errors: 64 rows of 64 adapters, 2048 x 4096, rank 64 28.2 us
+/// against 25.9, rank 16 18.4 against 18.0; 256 rows 31.8 against 29.8.)
 template <class T, bool kGated, int NB, int MB>
 __device__ __forceinline__ void add_low_rank(const AdapterParams &p, floatx4 (&acc)[NB][MB], const RowAdapters<MB> &mine, int64_t m_first,
                                              int64_t n_first, int team, int teams) {
@@ -318,7 +329,6 @@ __device__ __forceinline__ void add_low_rank(const AdapterParams &p, floatx4 (&a
     const int64_t at = group * 32 + up_at;
     u32x4 ws[kBatch][NB];
     if (p.up_whole) {
-      // (Past the rank the row's first chunk again, against zeros: what it holds, the row has anyway.)
       const int64_t whole_at = at < p.rank ? at : 0;
 #pragma unroll
       for (int j = 0; j < kBatch; ++j) {
@@ -334,6 +344,16 @@ __device__ __forceinline__ void add_low_rank(const AdapterParams &p, floatx4 (&a
         for (int nb = 0; nb < NB; ++nb) ws[j][nb] = load8(up + row[nb], at, p.rank);
       }
     }
+    // Zeros past the rank (where the row's first chunk was read) and for lanes without a piece; no infinities and NaN against
+    // errors.
+    const bool kept = held && at < p.rank, against_errors = layout.errors(g);
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j)
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) {
+        if (!kept) ws[j][nb] = u32x4{0, 0, 0, 0};
+        if constexpr (!kErrors) ws[j][nb] = finite_only<T>(ws[j][nb], against_errors);
+      }
     // Two token blocks at a time: all at once do not fit the registers of the large shapes.
     constexpr int kPair = MB < 2 ? MB : 2;
     static_assert(MB == 3 || MB % kPair == 0, "whole pairs");
@@ -369,7 +389,13 @@ __device__ __forceinline__ void add_low_rank(const AdapterParams &p, floatx4 (&a
             for (int of = 0; of < kPerHalf; ++of) {
               const int nb = h * kPerHalf + of;
               floatx4 part = T::mfma(ws[j][nb], values[h][i], floatx4{0.0f, 0.0f, 0.0f, 0.0f});
-              if constexpr (kErrors) part = T::mfma(ws[j][nb], errors[h][i], part);
+              if constexpr (kErrors) {
+                // Not finite only where an up weight is not, and the values' sum is not then either: any finite number leaves it
+                // as it is.
+                const floatx4 rest = T::mfma(ws[j][nb], errors[h][i], floatx4{0.0f, 0.0f, 0.0f, 0.0f});
+#pragma unroll
+                for (int c = 0; c < 4; ++c) part[c] += __builtin_amdgcn_fmed3f(rest[c], -3.402823466e38f, 3.402823466e38f);
+              }
 #pragma unroll
               for (int c = 0; c < 4; ++c) {
                 const float v = std::is_same<T, F16>::value ? part[c] * factor[h][i] : part[c];
@@ -386,11 +412,14 @@ __device__ __forceinline__ void add_low_rank(const AdapterParams &p, floatx4 (&a
       if (both) products(std::false_type{}, group);
       else products(std::true_type{}, group);
     }
-    if (current[kBatch - 1] < 0) return;
+    if (current[kBatch - 1] < 0) break;
 #pragma unroll
     for (int j = 0; j < kBatch; ++j) current[j] = next();
-    if (current[0] < 0) return;
+    if (current[0] < 0) break;
   }
+  // The last loads, which not every wavefront uses (vmcnt 0, nothing else): else the compiler waits for them, and the
+  // stages in flight, in every turn of the walk, where a register is used again (256 x 4096 x 2048 39 us, 30 so).
+  __builtin_amdgcn_s_waitcnt(0x0f70);
 }
 
 /// The same for column n's (gated: and its gate row's) sums of the first rows, whose lanes' sums meet later: a lane

@@ -201,14 +201,12 @@ __global__ void __launch_bounds__(S::kThreads) tile_kernel(P p) {
   // the other half's weight rows and for a stage's chunks past the values; where a piece of an up row ends, its first
   // chunk comes again (against zeros).
   [[maybe_unused]] typename std::conditional<kWalked, NamedAdapters, int>::type adapter_stages = tile_adapters<kWalked>(rows_adapters, S::kBM);
-  [[maybe_unused]] bool mixed = false;  // rows without an adapter, or several adapters
   [[maybe_unused]] int adapted = 0, stage_group = 0, stage_half = 0;
   if constexpr (kWalked) {
     __syncthreads();
     adapter_stages.find(rows_adapters.id);
     const LowLayout layout(p.rank);
-    const int named_ones = adapter_stages.count(rows_left, mixed);
-    adapted = named_ones * layout.groups * (kGated ? 2 : 1);
+    adapted = adapter_stages.count() * layout.groups * (kGated ? 2 : 1);
     stages += adapted;
     stage_group = layout.groups;
   }
@@ -446,7 +444,6 @@ __global__ void __launch_bounds__(S::kThreads) tile_kernel(P p) {
           int column = of * kWaveCols + (kGated ? in % kWaveCols : in);
           column = column < cols_left ? column : cols_left - 1;
           const int at = (wide ? c & 3 : layout.width == 16 ? c & 1 : 0) * 8;
-          // (Past the rank the row's first chunk again, against zeros: what it holds, the row has anyway.)
           if (p.up_whole)
             pieces[i] = *reinterpret_cast<const u32x4 *>(up + (static_cast<uint32_t>(column) * static_cast<uint32_t>(p.up_row_stride) +
                                                                (group * 32 + at < p.rank ? at : 0)));
@@ -457,7 +454,14 @@ __global__ void __launch_bounds__(S::kThreads) tile_kernel(P p) {
 #pragma unroll
       for (int i = 0; i < S::kLoads; ++i) {
         const int c = (l & 7) ^ ((l >> 4) & 3) ^ (4 * ((wave + S::kWaves * i) & 1));
-        ring[buffer_of][(wave + S::kWaves * i) * 64 + l] = 4 * c < layout.width ? pieces[i] : u32x4{0, 0, 0, 0};
+        bool filled = 4 * c < layout.width;
+        if (i >= S::kBM / 8 / S::kWaves) {
+          // Zeros past the rank (where the row's first chunk was read); no infinities and NaN against errors.
+          const int at = (wide ? c & 3 : layout.width == 16 ? c & 1 : 0) * 8;
+          filled = filled && group * 32 + at < p.rank;
+          pieces[i] = finite_only<T>(pieces[i], 8 * c >= layout.width);
+        }
+        ring[buffer_of][(wave + S::kWaves * i) * 64 + l] = filled ? pieces[i] : u32x4{0, 0, 0, 0};
       }
       if constexpr (std::is_same<T, F16>::value) rows_adapters.put_factor(buffer_of, factor_of_row);
       // Two buffers in turn: one barrier a stage (a wavefront writes the other one only after all have read it).
@@ -564,7 +568,7 @@ __global__ void __launch_bounds__(S::kThreads) tile_kernel(P p) {
           }
         }
         if constexpr (kWalked) {
-          if (mixed) remake<T, kGated>(p, m[j], n, rows_adapters.id[static_cast<int>(m[j] - m0)], v, gates);
+          if (adapted > 0) remake<T, kGated>(p, m[j], n, rows_adapters.id[static_cast<int>(m[j] - m0)], v, gates);
         }
         if constexpr (kRanks) {
           if (named.holds(static_cast<int>(m[j] - m0))) columns.finish(p, m[j], named.current, v);

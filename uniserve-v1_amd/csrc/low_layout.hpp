@@ -23,6 +23,7 @@ struct LowLayout {
   // bytes of values and errors: the lanes behind them read the first piece, which is dropped (their own would
   // end past the last row of the workspace).
   constexpr bool has_piece(int g) const { return width >= 16 || g < 2; }
+  constexpr bool errors(int g) const { return has_piece(g) && 8 * g >= width; }  ///< whether that piece holds errors
   constexpr int32_t piece_at(int g) const { return has_piece(g) ? 16 * g : 0; }
   constexpr int32_t errors_at(int g) const { return piece_at(g) + 2 * width; }  ///< of width 32, an operand of their own
   constexpr int32_t factor_at() const { return 4 * width; }
