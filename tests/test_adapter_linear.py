@@ -467,6 +467,24 @@ def test_infinite_rank_values_stay_in_their_half(device, dtype, shape, m, n, k, 
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("m, n", [(1, 72), (2, 72), (40, 72), (513, 4104)])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_finite_rank_values_beside_an_infinite_one(device, m, n, dtype):
+    """180000 is no f16 number; beside an infinity, from which it is subtracted, it is finite all the same."""
+    announce("adapter beside an infinite rank value", m, n, dtype)
+    k, rank = 72, 8
+    x, w = torch.zeros((m, k), dtype=dtype, device=device), normal((n, k), 2, 0.05, dtype)
+    x[:, 0], x[:, 1] = 1.0, 2.0
+    call = dict(stacks(2, rank, n, k, dtype), adapter=(torch.arange(m) % 2).int().to(device), scales=None)
+    call["down"][:, :, :2] = 0
+    call["down"][0, 0, 0], call["down"][:, 1, :2] = float("inf"), 60000.0
+    call["up"][:, :, :2] = torch.tensor([1.0, -1.0], dtype=dtype)
+    got, (y, tolerance) = ops.adapter_linear(x, w, **call, out_dtype=F32), reference(x, w, **call, out_dtype=F32)
+    assert (got[0::2] == float("inf")).all() and torch.isfinite(got[1::2]).all()
+    assert ((got.double().cpu() - y).abs()[1::2] <= tolerance[1::2]).all()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("m", [1, 40, 300])
 @pytest.mark.parametrize("size", [2.0**-20, 2.0**-10, 2.0**9])
 def test_f16_rank_values_of_any_size(device, m, size):

@@ -216,12 +216,13 @@ struct RankColumns {
     for (int i = 0; i < 8; ++i) v[i] = i < count ? sums[i / 4][i % 4] * scale : 0.0f;
     float factor = 1.0f;
     if constexpr (std::is_same<T, F16>::value) {
-      // The power of two that brings the group's largest value to [1, 2); its lanes are neighbours.
+      // The power of two that brings the group's largest finite value to [1, 2); its lanes are neighbours. (An infinity or
+      // NaN stays what it is; the values beside it would be infinities, too, if it decided.)
       float most = 0.0f;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) most = __builtin_fmaxf(most, __builtin_fabsf(v[i]));
+      for (int i = 0; i < 8; ++i) most = __builtin_fmaxf(most, __builtin_fabsf(v[i]) < __builtin_inff() ? __builtin_fabsf(v[i]) : 0.0f);
       for (int offset = 1; offset < p.width / 8; offset *= 2) most = __builtin_fmaxf(most, __shfl_xor(most, offset));
-      if (most > 0.0f && most < __builtin_inff()) {
+      if (most > 0.0f) {
         int power = __builtin_amdgcn_frexp_expf(most) - 1;
         power = power < -126 ? -126 : power;
         factor = __builtin_ldexpf(1.0f, power);
