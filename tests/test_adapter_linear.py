@@ -467,6 +467,27 @@ def test_infinite_rank_values_stay_in_their_half(device, dtype, shape, m, n, k, 
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("gated, shape, m, n, k", [case for case in KERNELS if case[2] >= 100 and case[1] != "64,64,2,2,4,1"])
+def test_rows_that_are_not_finite(device, gated, shape, m, n, k):
+    """Rows of NaN, with a NaN and with an infinity, beside others, in tiles of one adapter and of several, one of them with
+    an infinite up weight: what the formula makes of each."""
+    announce("adapter rows not finite", shape, gated, m, n, k)
+    halves, rank = 2 if gated else 1, 16
+    entry = ops.adapter_gated_linear if gated else ops.adapter_linear
+    x, w = normal((m, k), 1), normal((n * halves, k), 2, 0.05)
+    x[3], x[7::11, k - 1], x[5, 2], x[8::13, 4] = float("nan"), float("nan"), float("inf"), float("-inf")
+    columns = sorted({0, 1, n // 3, n - 2, n - 1})
+    for order in (lambda m, _: torch.zeros(m, dtype=torch.int32, device=device), runs, each_other):
+        call = dict(stacks(4, rank, n, k, halves=halves), adapter=order(m, 4))
+        for poisoned in (False, True):
+            if poisoned:
+                call["up"][0, n - 1, 3], call["up"][1, n // 3, 9] = float("inf"), float("nan")
+            got = entry(x, w, **call)
+            y = reference(x, **columns_of(call, w, columns, halves), activation="silu" if gated else None, gated=gated)[0]
+            assert_as_the_formula(got[:, columns], y)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("m, n", [(1, 72), (2, 72), (40, 72), (513, 4104)])
 @pytest.mark.parametrize("dtype", [F16, BF16])
 def test_finite_rank_values_beside_an_infinite_one(device, m, n, dtype):

@@ -124,6 +124,8 @@ __global__ void __launch_bounds__(S::kThreads) tile_kernel(P p) {
   constexpr bool kStaged = kMany && !kWalked;
   static_assert(!kStaged || S::kThreads >= S::kBM, "a thread for each row's factor");
   [[maybe_unused]] __shared__ RowsAdapters<kMany ? S::kBM : 0, std::is_same<T, F16>::value> rows_adapters;
+  [[maybe_unused]] __shared__ uint32_t columns_known[kWalked ? S::kThreads : 1];  // (in LDS: a register would spill a sum)
+  if constexpr (kWalked) columns_known[threadIdx.x] = ~0u;
   if constexpr (kMany) rows_adapters.load(p, m0);
   [[maybe_unused]] typename std::conditional<kRanks, NamedAdapters, int>::type named = named_adapters(p, m0, S::kBM);
   do {  // once, or for each adapter that the tile's rows name (kRanks)
@@ -568,7 +570,7 @@ __global__ void __launch_bounds__(S::kThreads) tile_kernel(P p) {
           }
         }
         if constexpr (kWalked) {
-          if (adapted > 0) remake<T, kGated>(p, m[j], n, rows_adapters.id[static_cast<int>(m[j] - m0)], v, gates);
+          if (adapted > 0) remake<kGated>(p, m[j], n, rows_adapters.id, S::kBM, static_cast<int>(m[j] - m0), columns_known[threadIdx.x], v, gates);
         }
         if constexpr (kRanks) {
           if (named.holds(static_cast<int>(m[j] - m0))) columns.finish(p, m[j], named.current, v);
