@@ -277,6 +277,21 @@ def test_in_place(device, rows, width, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("norm", ["rms", "layer"])
+@pytest.mark.parametrize("rows", [1, 33])
+def test_in_place_with_nothing_to_join(device, rows, norm):
+    """The total is the rows before their norm, also where the norm overwrites them."""
+    announce("add_norm in place alone", rows, norm)
+    made = inputs(rows, 264, BF16, seed=3)
+    x, weight = made["x"], made["weight"]
+    before = x.clone()
+    want, unjoined = ops.add_norm(x, weight, norm=norm)
+    assert unjoined is x and torch.equal(x, before)
+    out, total = ops.add_norm(x, weight, norm=norm, out=x)
+    assert out is x and torch.equal(out, want) and torch.equal(total, before)
+
+
+@pytest.mark.gpu
 def test_rows_past_4_gib(device):
     announce("add_norm far rows")
     rows, width = 5, 264

@@ -324,7 +324,8 @@ def add_norm(x, weight, residual=None, post=None, gate=None, channels=None, scal
     the biases ``bias`` and ``post_bias``, both of which may be absent. ``gate`` is one logit per row (``[T, 1]``),
     ``channels`` a factor per column. ``residual`` and ``total`` are of ``x``'s type or f32, ``out`` of ``x``'s; the
     vectors are all of ``x``'s type or all f32. FP32 within, one rounding into each output. Either output may be
-    given, also as ``x`` or ``residual`` itself, in place. With nothing to join, ``total`` is ``x`` unless it is given."""
+    given, also as ``x`` or ``residual`` itself, in place. With nothing to join, ``total`` is ``x`` unless it is given or
+    ``out`` overwrites ``x``."""
     dtype, index = x.dtype, x.get_device()
     element = _ELEMENT.get(dtype)
     if x.dim() != 2 or element is None or index < 0:
@@ -357,7 +358,8 @@ def add_norm(x, weight, residual=None, post=None, gate=None, channels=None, scal
         if total.dtype != stream:
             raise ValueError("add_norm: the total is of the residual's type")
         total_stride = _matrix(total, rows, width, index, "add_norm", "the total")
-    elif residual is not None or post is not None or gate is not None or channels is not None or scale != 1.0:
+    elif (residual is not None or post is not None or gate is not None or channels is not None or scale != 1.0
+          or (out is not None and out.data_ptr() == x.data_ptr())):
         returned = total = torch.empty(rows, width, dtype=stream, device=x.device)
         total_stride = width
     else:
