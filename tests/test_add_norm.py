@@ -277,6 +277,26 @@ def test_in_place(device, rows, width, dtype):
 
 
 @pytest.mark.gpu
+def test_gates_of_fp32_rows(device):
+    """sigmoid(g) = 1 / (1 + e) with e = exp(-g) off by 2 u (an ulp), the sum, the quotient and the product by u each, and
+    the scales' one: 6 u, to first order; 8 are granted."""
+    announce("add_norm f32 gates")
+    rows, width = 481, 72
+    x, gate = normal((rows, width), 1, dtype=F32), torch.linspace(-80.0, 40.0, rows, device=device)[:, None]
+    _, total = ops.add_norm(x, None, gate=gate)
+    want = x.double().cpu() * torch.special.expit(gate.double().cpu())
+    assert ((total.double().cpu() - want).abs() <= 8 * U * want.abs()).all()
+    x, gate = x.to(BF16), gate.to(BF16)
+    _, total = ops.add_norm(x, None, gate=gate, total=torch.empty((rows, width), dtype=F32, device=device))
+    want = x.double().cpu() * torch.special.expit(gate.double().cpu())
+    assert ((total.double().cpu() - want).abs() <= 8 * U * want.abs()).all(), "f32 total of bf16 rows"
+    x = x.float()
+    ends = torch.tensor([float("-inf"), -1000.0, float("inf"), 1000.0, float("nan")], device=device)[:, None]
+    _, total = ops.add_norm(x[:5].contiguous(), None, gate=ends)
+    assert (total[:2] == 0).all() and torch.equal(total[2:4], x[2:4]) and torch.isnan(total[4]).all()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("norm", ["rms", "layer"])
 @pytest.mark.parametrize("rows", [1, 33])
 def test_in_place_with_nothing_to_join(device, rows, norm):

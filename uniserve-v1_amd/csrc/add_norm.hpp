@@ -196,7 +196,11 @@ __global__ void __launch_bounds__(kTeam < 128 ? 256 : kTeam) add_norm_kernel(Add
       float logit;
       if constexpr (sizeof(g) == 4) logit = g;
       else logit = X::widen(g);
-      factor *= __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-logit * 1.4426950408889634f));
+      // The hardware's exponential of a rounded product is off by the logit's size in u, 80 of them at -80: nothing beside the
+      // rounding of 16-bit outputs. FP32 ones take expf and a quotient, four u at most (64 x 4096 on an FP32 stream 3.6 us
+      // against 3.5).
+      if constexpr (sizeof(typename X::type) == 4 || sizeof(typename R::type) == 4) factor *= 1.0f / (1.0f + expf(-logit));
+      else factor *= __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-logit * 1.4426950408889634f));
     }
     float v[kChunks][8];
 #pragma unroll
