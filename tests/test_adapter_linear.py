@@ -316,6 +316,44 @@ def test_unaligned_rows(device, gated, m, n, k):
     assert_near(got, reference(x, w, **call, activation="silu" if gated else None, gated=gated))
 
 
+#: The shapes that f16 rows have, too (the largest tiles do not serve them).
+F16_KERNELS = [case for case in KERNELS if not case[1].startswith(("256,256", "192,256"))]
+#: Shapes through registers, for rows that are not whole 16-byte pieces.
+UNALIGNED_KERNELS = [(False, "96,128,2,2,2,1", 2000, 3001, 123), (True, "96,128,2,2,2,1", 2000, 3001, 123),
+                     (False, "128,128,2,4,2,1", 1100, 3001, 507), (True, "128,128,2,4,2,1", 1100, 3001, 507),
+                     (False, "64,64,2,2,2,1", 130, 3001, 5), (True, "32,32,1,1,2,4", 130, 1001, 2047), (False, "16,32,1,1,2,4", 8, 40, 2047)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("gated, shape, m, n, k", F16_KERNELS + UNALIGNED_KERNELS)
+@pytest.mark.parametrize("rank", [5, 8, 16, 40])
+def test_each_tile_kernel_of_f16(device, gated, shape, m, n, k, rank):
+    """f16 rows have a factor for each group of ranks, in the large tiles through LDS behind the walk: the shapes by DMA and
+    through registers, each with rows of many adapters and with runs of a few; a row's rank values of far apart sizes in
+    its halves and groups."""
+    announce("adapter f16 kernel", shape, gated, m, n, k, rank)
+    halves = 2 if gated else 1
+    x, w, out = normal((m, k), 1, dtype=F16), normal((n * halves, k), 2, 0.05, F16), normal((m, n), 3, dtype=F16)
+    call = dict(stacks(5, rank, n, k, F16, halves=halves), adapter=each_other(m, 5))
+    sizes = 2.0 ** torch.tensor([-9.0, 6.0, 0.0, -3.0], device=device)[(torch.arange(halves * rank, device=device) * 5 // rank) % 4]
+    call["down"] = (call["down"].float() * sizes[:, None]).to(F16)
+    up_sizes = 1.0 / sizes.view(halves, rank).repeat_interleave(n, 0)  # (halves' rows by halves' ranks)
+    call["up"] = (call["up"].float() * up_sizes).to(F16)
+    workspace = torch.empty(ops.adapter_workspace(m, rank * halves), dtype=torch.uint8, device=device)
+
+    def run():
+        entry = ops.adapter_gated_linear if gated else ops.adapter_linear
+        return entry(x, w, **call, out=out, workspace=workspace)
+
+    mangled = "TileShapeI" + "".join(f"Li{d}E" for d in shape.split(","))
+    names = kernels_of(run)
+    assert len(names) == 2 and "RankParams" in names[0] and mangled in names[1], names
+    for order in (each_other, runs):
+        call["adapter"].copy_(order(m, 5))
+        run()
+        assert_near(out, reference(x, w, **call, activation="silu" if gated else None, gated=gated))
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("m", [1, 20, 300])
 @pytest.mark.parametrize("shift", [0, 1, 8])
@@ -400,8 +438,7 @@ def test_infinities_and_nans_in_large_tiles(device, gated, shape, m, n, k, rank)
     assert ((got[touched][:, kept] - want[touched][:, kept]).abs() <= tolerance[touched][:, kept]).all()
 
 
-#: The shapes that f16 rows have, too (the largest tiles do not serve them), and calls of one and two rows.
-F16_KERNELS = [case for case in KERNELS if not case[1].startswith(("256,256", "192,256"))]
+#: Calls of one and two rows.
 FEW = [(False, "", 1, 520, 136), (False, "", 2, 72, 264), (True, "", 1, 72, 136), (True, "", 2, 520, 72)]
 
 
