@@ -180,13 +180,13 @@ template <bool kGated>
 __device__ __forceinline__ void remake(const AdapterParams &p, int64_t m, int64_t n, const int32_t *ids, int rows, int row, uint32_t &known,
                                        floatx4 (&sums)[2], floatx4 (&gates)[2]) {
   using T = Bf16;
-  bool finite = true;
+  float none = 0.0f;  // NaN if a sum is not finite
 #pragma unroll
   for (int c = 0; c < 8; ++c) {
-    finite = finite && __builtin_fabsf(sums[c / 4][c % 4]) < __builtin_inff();
-    if (kGated) finite = finite && __builtin_fabsf(gates[c / 4][c % 4]) < __builtin_inff();
+    none = __builtin_fmaf(sums[c / 4][c % 4], 0.0f, none);
+    if (kGated) none = __builtin_fmaf(gates[c / 4][c % 4], 0.0f, none);
   }
-  if (finite) return;
+  if (none == 0.0f) return;
   constexpr uint32_t kUnknown = ~0u;
   uint32_t weights = known;
   if (weights == kUnknown) known = weights = columns_not_finite<kGated>(p, n, ids, rows);
