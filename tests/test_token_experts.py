@@ -377,6 +377,20 @@ def test_results_repeat_and_rows_do_not_depend_on_the_others(device, tokens):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("tokens, experts", [(4, 24), (12, 24), (40, 8), (64, 24)])
+def test_f16_rows_do_not_depend_on_the_others(device, tokens, experts):
+    """Jobs of 4, 8 and 16 tokens, and the row alone: the same bits."""
+    announce("token_experts f16 rows", tokens, experts)
+    call = inputs(tokens, 512, 200, experts, 4, F16)
+    call["x"] *= 2.0 ** -(torch.arange(tokens, device=device) % 9)[:, None]
+    together = ops.token_experts(**call)
+    assert torch.equal(ops.token_experts(**call), together)
+    for row in range(0, tokens, 3):
+        alone = {**call, **{k: call[k][row:row + 1].contiguous() for k in ("x", "ids", "weights")}}
+        assert torch.equal(ops.token_experts(**alone)[0], together[row]), row
+
+
+@pytest.mark.gpu
 def test_two_kernels(device):
     announce("token_experts kernels")
     call = inputs(8, 256, 128, 16, 4)
