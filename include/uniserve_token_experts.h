@@ -15,7 +15,8 @@
 // Sums are FP32. In the second product a gated value is a pair of the type's elements, the value and its rounding error,
 // and the output is rounded once. bf16: 16 bits of significand. f16: 64 consecutive values of a route share a power of two,
 // so that values of any size are served; 22 bits, or 2^-25 of the largest of the 64 where a value is small beside it.
-// A row's result does not depend on the other rows. What an expert holds, infinities and NaN too, reaches the rows
+// A row's result does not depend on the other rows. (From some 32 tokens on, bf16 layers that uniserve_gather_gemm and
+// uniserve_route_gemm serve are computed faster by those.) What an expert holds, infinities and NaN too, reaches the rows
 // routed to it and no others, and is there what the formula makes of it.
 //
 // `workspace` is uniserve_token_experts_workspace(tokens, top, width) bytes, 16-byte aligned; its contents before the

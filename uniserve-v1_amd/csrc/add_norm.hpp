@@ -256,7 +256,7 @@ void launch_shape(const AddNormParams &p, hipStream_t stream) {
 /// and 4.0, 4.1 and 5.2, 6.5 and 8.6. Bound by the bytes from some hundred rows on (8192 x 4096 at 6.8 TB/s
 /// on the same tensors again and again, 4.5 over three sets, where a copy of 4 GiB runs at 4.7), below by the launch
 /// and the row's chain of loads and sums (one row of 2048 2.4 us, 2.9 with both norms). Rows of more than 16384
-/// elements spill registers.
+/// elements spill 46 to 357 registers, bf16 ones of more than 8192 on an FP32 stream 8, of no whole eights 6 to 16.
 template <class X, class R>
 void launch(const AddNormParams &p, hipStream_t stream) {
   const int32_t chunks = ceil_div(p.width, 8);

@@ -1,7 +1,7 @@
 // SPDX-License-Identifier: Apache-2.0
 //
-// Low-rank adapters beside the dense products: the first factor's kernel, which leaves each row's rank values in the
-// workspace, and the second factor's product, which the product kernels add to their sums behind the walk over K.
+// Low-rank adapters beside the dense products: the first factor's epilogue, which leaves each row's rank values in the
+// workspace, and the second factor's product, which the product kernels add to their sums before, in or behind the walk over K.
 //
 // Rows of one adapter are found where they are used: a wavefront takes the adapters that its rows name in turn, each
 // once, multiplies that adapter's factor by all of its rows and keeps the sums of the rows that name it (a matrix
@@ -174,8 +174,9 @@ __device__ __forceinline__ uint32_t columns_not_finite(const AdapterParams &p, i
 /// which gives NaN where they are not finite, and a weight by a value and by its error, which gives NaN where the weight
 /// is an infinity. What the row itself makes of its operands stays so: without such weights in the column (`known`: found
 /// once a lane, when its first sum asks, ~0 before) or such rank values in the other half, nothing is made again, and
-/// what has come to NaN is not carried on. (8192 x 4096 x 2048, rank 16, runs of 300 rows: finite 0.144 ms, all rows NaN 0.30, where
-/// making every sum again took 18.3; one of eight adapters NaN 16, its tiles' other rows made again, a lane a sum.)
+/// what has come to NaN is not carried on. (8192 x 4096 x 2048, rank 16, runs of 300 rows: finite 0.144 ms, all rows NaN
+/// 0.30, where making every sum again took 18.3; one of eight adapters NaN 16, its tiles' other rows made again, a lane a
+/// sum.)
 template <bool kGated>
 __device__ __forceinline__ void remake(const AdapterParams &p, int64_t m, int64_t n, const int32_t *ids, int rows, int row, uint32_t &known,
                                        floatx4 (&sums)[2], floatx4 (&gates)[2]) {
@@ -326,8 +327,8 @@ __device__ __forceinline__ int row_adapters(const RankParams &, int64_t) { retur
 /// column n_first on (gated: half of them the up rows', then the same columns' gate rows), some of the adapters that
 /// its rows name after the others; of `teams` wavefronts with the same sums, which are added up later, each takes
 /// its share of the adapters. Two matrix instructions per 32 ranks, over the values and over their errors, or, up to
-/// rank 16, one over both. (What keeps infinite up rows from the errors: 64 rows of 64 adapters, 2048 x 4096, rank 64 28.2 us
-/// against 25.9, rank 16 18.4 against 18.0; 256 rows 31.8 against 29.8.)
+/// rank 16, one over both. (What keeps infinite up rows from the errors, rows by one of 64 adapters: 64 x 4096 x
+/// 2048, rank 64, 28.2 us against 25.9; 64 x 2048 x 4096, rank 16, 18.4 and 18.0; 256 x 4096 x 2048, rank 16, 31.8 and 29.8.)
 template <class T, bool kGated, int NB, int MB>
 __device__ __forceinline__ void add_low_rank(const AdapterParams &p, floatx4 (&acc)[NB][MB], const RowAdapters<MB> &mine, int64_t m_first,
                                              int64_t n_first, int team, int teams) {

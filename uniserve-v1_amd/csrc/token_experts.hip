@@ -10,8 +10,11 @@
 // each one's products, times the routes' weights, to their rows' sums, experts in ascending order: no join across
 // workgroups, no atomics on sums.
 //
-// Bound by the weights: 128 experts of 2048 x 768, 64 tokens (1.2 GB) 136 us, 5.9 TB/s, and 98 us, 4.1 TB/s, where a
-// copy reaches 4.7; one token (75 MB) 12.3 and 9.0 us, a launch and a chain of ids, routing and first weights in each.
+// Bound by the weights: 128 experts of 2048 x 768, 64 tokens (1.2 GB, one pass among others, traced) 129 us, 6.2 TB/s, and 90 us,
+// 4.5 TB/s, where a stream that is only read reaches 6.9; one token (75 MB) 13.2 and 8.8 us, a launch and a chain of ids,
+// routing and first weights in each. (The figures further down compare variants in one run each, from graphs over several
+// sets of ids, which take some 15 us longer at 64 tokens.) From 32 tokens on the sorted operators, whose second product has
+// workgroups by expert and row slice, take less in bf16: 64 tokens 195 us where these two take 218.
 // The second kernel's lines of gated values come from L2, at 64 tokens as many bytes as the weights; neither more
 // wavefronts, deeper loads nor less LDS traffic (operands without a way through it) made it faster.
 #include "extents.hpp"
@@ -59,8 +62,9 @@ struct Params {
 
 /// Whether the gated values are FP32 between the kernels: f16's range does not hold them, so the second kernel splits each
 /// line into two elements by a power of two of the line's own. bf16's does, and the first kernel splits them once.
-/// (The first kernel's workgroups see sixteen columns of a line each, not its largest value. The split costs the second kernel
-/// 1 to 10 us: f16, T=1 22.6 us for both kernels against 21.6 with bf16 pairs, T=16 142 against 135, T=64 243 against 234.)
+/// (The first kernel's workgroups see sixteen columns of a line each, not its largest value. Both kernels of 128 experts of
+/// 2048 x 768, f16 with the split and with pairs at one fixed power, which lose small values: T=1 22.6 and 21.6 us, T=16 142 and
+/// 135, T=64 243 and 234; 64 experts of 4096 x 1408, T=64 445 and 412.)
 template <class T>
 constexpr bool kSplitLate = std::is_same<T, F16>::value;
 
@@ -328,7 +332,8 @@ struct LineSplit {
 /// (Weights loaded as lane l's chunk of row l % 8, in half l % 16 / 8 of the line, so that the matrix instruction takes them
 /// without LDS, are slower: T=16 52 us against 50, T=64 106 against 98.)
 /// kTokens of a job at most: their gated values come as whole lines, too, and through LDS (in the operand layout
-/// they took four loads of sixteen columns for any number of tokens: T=16 72 us, 50 now).
+/// they took four loads of sixteen columns for any number of tokens: T=16 72 us, 50 now). With eight columns and
+/// sixteen tokens the bf16 kernels spill 4 registers (of rows that are not whole pieces 13).
 template <class T, bool kWhole, bool kOnce, int kCols, int kSets, int kTokens>
 __global__ void __launch_bounds__(kSets *kThreads) down_kernel(Params p) {
   constexpr int kGroups = kCols / 8, kAllThreads = kSets * kThreads;
