@@ -22,9 +22,9 @@
 // two halves, 32 x 32 x 16 MFMAs, four wavefronts of 128 x 128. The 256 x 256 kernels without adapters use all 256
 // registers and spill 8 (gated 2): written before the walk and in its last stages, read back there and in the epilogue;
 // the loops over the stages access no scratch. With adapters they spill 19 and 32, some in the adapters' stages. Smaller
-// products: what a CU can load, 115 to 135 GB/s from L2 and 60 to 70 from beyond, so the shape with the fewest rows per CU that still gives every CU a tile
-// (gated 200 x 1408 x 4096: 220 tiles of 48 x 64, 0.9 MB each, 14.0 us). By registers and 128-byte rows the loads
-// are no faster, in operand layout (16 rows of 64 bytes) 38 GB/s.
+// products: what a CU can load, 115 to 135 GB/s from L2 and 60 to 70 from beyond, so the shape with the fewest rows per CU
+// that still gives every CU a tile (gated 200 x 1408 x 4096: 220 tiles of 48 x 64, 0.9 MB each, 14.0 us). By registers and
+// 128-byte rows the loads are no faster, in operand layout (16 rows of 64 bytes) 38 GB/s.
 #pragma once
 
 #include <type_traits>
