@@ -534,6 +534,7 @@ __global__ void __launch_bounds__(S::kThreads) tile_kernel(P p) {
   [[maybe_unused]] const typename std::conditional<kRanks, RankColumns<T>, Columns8<T, kGated>>::type columns(p, n);
 #pragma unroll
   for (int pass = 0; pass < MB / kPassMB; ++pass) {
+    if (pass > 0) wave_fence();  // (the one before has been read)
 #pragma unroll
     for (int b = 0; b < kPassMB; ++b)
 #pragma unroll
@@ -542,6 +543,8 @@ __global__ void __launch_bounds__(S::kThreads) tile_kernel(P p) {
     if constexpr (S::kSplit > 1) {
       __syncthreads();
       sums = &rings[0][0][0] + wave * kPassMB * 16 * kRowChunks;
+    } else {
+      wave_fence();
     }
     constexpr int kStep = S::kSplit * (kWave / kGroups);  // rows the lanes (and teams) finish at a time
     constexpr int kBatch = kPassMB * 16 / kStep >= 4 ? 4 : (kPassMB * 16 / kStep >= 2 ? 2 : 1);
